@@ -9,5 +9,7 @@ from .mbmm import MBMMCUDA, MBMMSoftmaxCUDA, make_masks
 from .minbmm import MinBMMCUDA
 from .topkbmm import TopkBMMCUDA
 from .kmeans import KMeansCUDA
+from .mx import CheckpointBMMCUDA, MXBMMCUDA, MXDenseBMMCUDA, MXQuantizeCUDA, MXTensor
 
-__all__ = ["BMMCUDA", "MBMMCUDA", "MBMMSoftmaxCUDA", "MinBMMCUDA", "TopkBMMCUDA", "KMeansCUDA", "make_masks"]
+__all__ = ["BMMCUDA", "MBMMCUDA", "MBMMSoftmaxCUDA", "MinBMMCUDA", "TopkBMMCUDA", "KMeansCUDA", "make_masks",
+           "MXTensor", "MXQuantizeCUDA", "MXBMMCUDA", "MXDenseBMMCUDA", "CheckpointBMMCUDA"]

@@ -11,6 +11,7 @@
 #include <mutex>
 
 #include "../../include/fbmm.h"
+#include "fbmm_host.h"
 #include "fbmm_kernel.cuh"
 #include "fbmm_l1_kernel.cuh"
 
@@ -160,7 +161,7 @@ bool is_broadcast(const Operand& op, int l) { return l > 1 && op.stride == 0; }
 struct TensorMapKey {
   const void* ptr;
   long long ld, stride;
-  int rows, k, l, box_rows, kind;  // kind: 0 fp32 K-major, 1 fp32 MN-major, 2 fp16, 3 bf16
+  int rows, k, l, box_rows, kind;  // kind: 0 fp32 K-major, 1 fp32 MN-major, 2 fp16, 3 bf16, 4 mask, 16 and up: tensor_map_3d
   bool operator==(const TensorMapKey& o) const {
     return ptr == o.ptr && ld == o.ld && stride == o.stride && rows == o.rows && k == o.k && l == o.l &&
            box_rows == o.box_rows && kind == o.kind;
@@ -194,6 +195,23 @@ void tensor_map_remember(const TensorMapKey& key, const CUtensorMap& map) {
   g_tm_cache.maps[at] = map;
   g_tm_cache.next = (at + 1) % kTensorMapCacheSize;
   if (g_tm_cache.used < kTensorMapCacheSize) ++g_tm_cache.used;
+}
+
+int encode_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base, const cuuint64_t dims[3],
+              const cuuint64_t strides[2], const cuuint32_t box[3], bool swizzle128) {
+  const TensorMapKey key{base, static_cast<long long>(strides[0]), static_cast<long long>(strides[1]),
+                         static_cast<int>(dims[1]), static_cast<int>(dims[0]), static_cast<int>(dims[2]),
+                         static_cast<int>(box[1]),
+                         16 + static_cast<int>(type) * 1024 + static_cast<int>(box[0]) * 2 + (swizzle128 ? 1 : 0)};
+  if (tensor_map_lookup(key, map)) return FBMM_OK;
+  cuuint32_t elem_strides[3] = {1, 1, 1};
+  const CUresult r = g_encode(map, type, 3, const_cast<void*>(base), dims, strides, box, elem_strides,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FBMM_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r));
+  tensor_map_remember(key, *map);
+  return FBMM_OK;
 }
 
 int make_tensor_map(CUtensorMap* map, const Operand& op, int k, int l, int box_rows) {
@@ -610,13 +628,16 @@ const char* fbmm_last_error(void) { return g_err; }
 
 int fbmm_check(void* stream) {
   FBMM_CUDA(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
-  unsigned int status[4] = {0, 0, 0, 0};
+  unsigned int status[4] = {0, 0, 0, 0}, mx = 0;
   FBMM_CUDA(cudaMemcpyFromSymbol(status, fbmm::g_fbmm_status, sizeof(status)));
+  const int rc = fbmm_host::mx_status(&mx);
+  if (rc != FBMM_OK) return rc;
   if (status[0] != 0) {
     const unsigned int zero[4] = {0, 0, 0, 0};
     FBMM_CUDA(cudaMemcpyToSymbol(fbmm::g_fbmm_status, zero, sizeof(zero)));
-    return fail(FBMM_ERR_DEVICE, "a kernel gave up on a bounded wait (status 0x%x)", status[0]);
   }
+  if ((status[0] | mx) != 0)
+    return fail(FBMM_ERR_DEVICE, "a kernel gave up on a bounded wait (status 0x%x)", status[0] | mx);
   return FBMM_OK;
 }
 
@@ -1342,6 +1363,26 @@ int launch_norms_x16(cudaStream_t stream, const RowProblem& p, void* scratch, Ep
 }
 
 }  // namespace
+
+namespace fbmm_host {
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+int device_sms(int* sms) {
+  DeviceState* st;
+  const int rc = device_state(&st);
+  if (rc == FBMM_OK) *sms = st->sms;
+  return rc;
+}
+int tensor_map_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base, const cuuint64_t dims[3],
+                  const cuuint64_t strides[2], const cuuint32_t box[3], bool swizzle128) {
+  return encode_3d(map, type, base, dims, strides, box, swizzle128);
+}
+}  // namespace fbmm_host
 
 extern "C" int fbmm_min_bmm_x16(void* stream_, const void* A, long long lda, long long stride_a, const void* B,
                                 long long ldb, long long stride_b, int dtype, float* values, long long* indices, int l,

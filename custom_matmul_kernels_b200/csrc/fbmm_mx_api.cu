@@ -1,0 +1,212 @@
+// Host side of the microscaled entry points: quantisation, its inverse and the 4-bit product.
+#include <algorithm>
+#include <cstdint>
+
+#include "../../include/fbmm.h"
+#include "fbmm_host.h"
+#include "fbmm_mx_gemm.cuh"
+#include "fbmm_mx_quant.cuh"
+
+namespace {
+
+using namespace fbmm;
+using fbmm_host::fail;
+
+int check_shape(int l, int rows, int k) {
+  if (l <= 0 || rows <= 0 || k <= 0) return fail(FBMM_ERR_INVALID, "l, rows, k must be positive, got %d %d %d", l, rows, k);
+  const long long groups = static_cast<long long>(l) * ((rows + 127) / 128) * ((k + 127) / 128);
+  if (groups > 0x7fffffffLL) return fail(FBMM_ERR_INVALID, "matrix of %d x %d x %d is too large", l, rows, k);
+  if (k > (1 << 29)) return fail(FBMM_ERR_INVALID, "k = %d is too large", k);
+  return FBMM_OK;
+}
+
+int check_bits(int bits) {
+  if (bits != 4 && bits != 8) return fail(FBMM_ERR_INVALID, "bits must be 4 or 8, got %d", bits);
+  return FBMM_OK;
+}
+
+int check_type(int dtype) {
+  if (dtype != FBMM_F32 && dtype != FBMM_F16 && dtype != FBMM_BF16)
+    return fail(FBMM_ERR_INVALID, "dtype must be FBMM_F32 (0), FBMM_F16 (1) or FBMM_BF16 (2), got %d", dtype);
+  return FBMM_OK;
+}
+
+int elem_size(int dtype) { return dtype == FBMM_F32 ? 4 : 2; }
+
+// A microscaled operand as the entry points take it.
+int check_mx(const char* name, const unsigned char* codes, long long stride_codes, const unsigned char* scales,
+             long long stride_scales, int l) {
+  if (codes == nullptr || scales == nullptr) return fail(FBMM_ERR_INVALID, "%s codes or scales are null", name);
+  if (((reinterpret_cast<uintptr_t>(codes) | reinterpret_cast<uintptr_t>(scales)) & 15u) != 0)
+    return fail(FBMM_ERR_ALIGN, "%s codes or scales are not 16-byte aligned", name);
+  if (l > 1 && (stride_codes < 0 || stride_scales < 0 || (stride_codes & 15) != 0 || (stride_scales & 15) != 0))
+    return fail(FBMM_ERR_ALIGN, "%s batch strides %lld and %lld are not non-negative multiples of 16 bytes", name,
+                stride_codes, stride_scales);
+  return FBMM_OK;
+}
+
+unsigned group_count(int l, int rows, int k) {
+  return static_cast<unsigned>(static_cast<long long>(l) * ((rows + 127) / 128) * ((k + 127) / 128));
+}
+
+template <int BITS, typename T>
+int launch_quantize(cudaStream_t stream, const MxQuantArgs& a, bool transposed) {
+  const unsigned grid = group_count(a.l, a.rows, a.k);
+  if (transposed) mx_quantize_t_kernel<BITS, T><<<grid, 256, 0, stream>>>(a);
+  else mx_quantize_kernel<BITS, T><<<grid, 256, 0, stream>>>(a);
+  FBMM_HOST_CUDA(cudaGetLastError());
+  return FBMM_OK;
+}
+
+template <int BITS, typename T>
+int launch_dequantize(cudaStream_t stream, const MxDequantArgs& a) {
+  mx_dequantize_kernel<BITS, T><<<group_count(a.l, a.rows, a.k), 256, 0, stream>>>(a);
+  FBMM_HOST_CUDA(cudaGetLastError());
+  return FBMM_OK;
+}
+
+// Tensor map over the codes of [l][rows][k] 4-bit elements: boxes of 128 bytes x box_rows rows.
+int codes_map(CUtensorMap* map, const unsigned char* codes, long long stride, int l, int rows, int k, int box_rows) {
+  const cuuint64_t pitch = static_cast<cuuint64_t>(mx_pitch(k, 4));
+  const bool one = l == 1 || stride == 0;
+  const cuuint64_t dims[3] = {pitch, static_cast<cuuint64_t>(rows), one ? 1u : static_cast<cuuint64_t>(l)};
+  const cuuint64_t strides[2] = {pitch, one ? pitch * static_cast<cuuint64_t>(rows) : static_cast<cuuint64_t>(stride)};
+  const cuuint32_t box[3] = {kMxRowBytes, static_cast<cuuint32_t>(box_rows), 1};
+  return fbmm_host::tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, dims, strides, box, true);
+}
+
+struct MxSide {
+  const unsigned char* codes;
+  long long stride;
+  const unsigned char* scales;
+  long long scale_stride;
+  int rows;
+};
+
+template <int BN, bool SWAP>
+int launch_mx_gemm(cudaStream_t stream, int sms, const MxSide& p, const MxSide& q, MxGemmArgs a) {
+  CUtensorMap mp, mq;
+  int rc;
+  if ((rc = codes_map(&mp, p.codes, p.stride, a.l, p.rows, a.k, kMxM)) != FBMM_OK) return rc;
+  if ((rc = codes_map(&mq, q.codes, q.stride, a.l, q.rows, a.k, BN)) != FBMM_OK) return rc;
+  a.p = MxOperand{p.scales, a.l > 1 ? p.scale_stride : 0, p.rows, a.l > 1 && p.stride == 0};
+  a.q = MxOperand{q.scales, a.l > 1 ? q.scale_stride : 0, q.rows, a.l > 1 && q.stride == 0};
+  a.p_tiles = (p.rows + kMxM - 1) / kMxM;
+  a.q_tiles = (q.rows + BN - 1) / BN;
+  const long long units = static_cast<long long>(a.p_tiles) * a.q_tiles * a.l;
+  using S = MxShape<BN, SWAP>;
+  FBMM_HOST_CUDA(cudaFuncSetAttribute(mx_gemm_kernel<BN, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  mx_gemm_kernel<BN, SWAP><<<static_cast<unsigned>(std::min<long long>(units, sms)), kMxThreads, S::kSmem, stream>>>(mp, mq, a);
+  FBMM_HOST_CUDA(cudaGetLastError());
+  return FBMM_OK;
+}
+
+}  // namespace
+
+namespace fbmm_host {
+int mx_status(unsigned int* bits) {
+  const unsigned int zero = 0;
+  FBMM_HOST_CUDA(cudaMemcpyFromSymbol(bits, fbmm::g_mx_status, sizeof(*bits)));
+  if (*bits != 0) FBMM_HOST_CUDA(cudaMemcpyToSymbol(fbmm::g_mx_status, &zero, sizeof(zero)));
+  return FBMM_OK;
+}
+}  // namespace fbmm_host
+
+extern "C" {
+
+size_t fbmm_mx_codes_bytes(int l, int rows, int k, int bits) {
+  if (l <= 0 || rows <= 0 || k <= 0 || (bits != 4 && bits != 8)) return 0;
+  return static_cast<size_t>(l) * rows * static_cast<size_t>(mx_pitch(k, bits));
+}
+
+size_t fbmm_mx_scales_bytes(int l, int rows, int k) {
+  if (l <= 0 || rows <= 0 || k <= 0) return 0;
+  return static_cast<size_t>(l) * static_cast<size_t>(mx_scale_bytes(rows, k));
+}
+
+int fbmm_mx_quantize(void* stream_, const void* X, int dtype, int layout, long long ldx, long long stride_x, int bits,
+                     unsigned char* codes, unsigned char* scales, int l, int rows, int k) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  int rc, sms;
+  if ((rc = check_shape(l, rows, k)) != FBMM_OK) return rc;
+  if ((rc = check_bits(bits)) != FBMM_OK) return rc;
+  if ((rc = check_type(dtype)) != FBMM_OK) return rc;
+  if (layout != 'n' && layout != 't') return fail(FBMM_ERR_INVALID, "layout must be 'n' or 't', got %d", layout);
+  if (X == nullptr) return fail(FBMM_ERR_INVALID, "X is null");
+  if ((reinterpret_cast<uintptr_t>(X) & static_cast<uintptr_t>(elem_size(dtype) - 1)) != 0)
+    return fail(FBMM_ERR_ALIGN, "X is not aligned to its element type");
+  if (ldx < (layout == 'n' ? k : rows)) return fail(FBMM_ERR_INVALID, "X pitch %lld smaller than its row length", ldx);
+  if (l > 1 && stride_x < 0) return fail(FBMM_ERR_INVALID, "X batch stride is negative");
+  if ((rc = check_mx("output", codes, 0, scales, 0, 1)) != FBMM_OK) return rc;
+  if ((rc = fbmm_host::device_sms(&sms)) != FBMM_OK) return rc;
+  const MxQuantArgs a{X, ldx, l > 1 ? stride_x : 0, codes, scales, rows, k, l};
+  const bool t = layout == 't';
+  if (bits == 4) {
+    if (dtype == FBMM_F32) return launch_quantize<4, float>(stream, a, t);
+    if (dtype == FBMM_F16) return launch_quantize<4, __half>(stream, a, t);
+    return launch_quantize<4, __nv_bfloat16>(stream, a, t);
+  }
+  if (dtype == FBMM_F32) return launch_quantize<8, float>(stream, a, t);
+  if (dtype == FBMM_F16) return launch_quantize<8, __half>(stream, a, t);
+  return launch_quantize<8, __nv_bfloat16>(stream, a, t);
+}
+
+int fbmm_mx_dequantize(void* stream_, const unsigned char* codes, long long stride_codes, const unsigned char* scales,
+                       long long stride_scales, int bits, void* out, int dtype, long long ldo, long long stride_o, int l,
+                       int rows, int k) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  int rc, sms;
+  if ((rc = check_shape(l, rows, k)) != FBMM_OK) return rc;
+  if ((rc = check_bits(bits)) != FBMM_OK) return rc;
+  if ((rc = check_type(dtype)) != FBMM_OK) return rc;
+  if ((rc = check_mx("input", codes, stride_codes, scales, stride_scales, l)) != FBMM_OK) return rc;
+  if (out == nullptr) return fail(FBMM_ERR_INVALID, "out is null");
+  if ((reinterpret_cast<uintptr_t>(out) & static_cast<uintptr_t>(elem_size(dtype) - 1)) != 0)
+    return fail(FBMM_ERR_ALIGN, "out is not aligned to its element type");
+  if (ldo < k) return fail(FBMM_ERR_INVALID, "out pitch %lld smaller than k = %d", ldo, k);
+  if (l > 1 && stride_o < static_cast<long long>(rows - 1) * ldo + k)
+    return fail(FBMM_ERR_INVALID, "out batches overlap (stride %lld)", stride_o);
+  if ((rc = fbmm_host::device_sms(&sms)) != FBMM_OK) return rc;
+  const MxDequantArgs a{codes, scales, l > 1 ? stride_codes : 0, l > 1 ? stride_scales : 0, out, ldo,
+                        l > 1 ? stride_o : 0, rows, k, l};
+  if (bits == 4) {
+    if (dtype == FBMM_F32) return launch_dequantize<4, float>(stream, a);
+    if (dtype == FBMM_F16) return launch_dequantize<4, __half>(stream, a);
+    return launch_dequantize<4, __nv_bfloat16>(stream, a);
+  }
+  if (dtype == FBMM_F32) return launch_dequantize<8, float>(stream, a);
+  if (dtype == FBMM_F16) return launch_dequantize<8, __half>(stream, a);
+  return launch_dequantize<8, __nv_bfloat16>(stream, a);
+}
+
+int fbmm_mx4_bmm(void* stream_, const unsigned char* a_codes, long long stride_a, const unsigned char* a_scales,
+                 long long stride_as, const unsigned char* b_codes, long long stride_b, const unsigned char* b_scales,
+                 long long stride_bs, void* C, int dtype, long long ldc, long long stride_c, int l, int m, int n, int k) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  int rc, sms;
+  if ((rc = check_shape(l, m, k)) != FBMM_OK) return rc;
+  if ((rc = check_shape(l, n, k)) != FBMM_OK) return rc;
+  if ((rc = check_type(dtype)) != FBMM_OK) return rc;
+  if ((rc = check_mx("A", a_codes, stride_a, a_scales, stride_as, l)) != FBMM_OK) return rc;
+  if ((rc = check_mx("B", b_codes, stride_b, b_scales, stride_bs, l)) != FBMM_OK) return rc;
+  if (C == nullptr) return fail(FBMM_ERR_INVALID, "C is null");
+  if ((reinterpret_cast<uintptr_t>(C) & static_cast<uintptr_t>(elem_size(dtype) - 1)) != 0)
+    return fail(FBMM_ERR_ALIGN, "C is not aligned to its element type");
+  if (ldc < n) return fail(FBMM_ERR_INVALID, "ldc %lld smaller than n = %d", ldc, n);
+  if (l > 1 && stride_c < static_cast<long long>(m - 1) * ldc + n)
+    return fail(FBMM_ERR_INVALID, "batches of C overlap (stride %lld)", stride_c);
+  if (static_cast<long long>((m + 127) / 128) * ((n + 127) / 128) > 0x7fffffffLL)
+    return fail(FBMM_ERR_INVALID, "product of %d x %d is too large", m, n);
+  if ((rc = fbmm_host::device_sms(&sms)) != FBMM_OK) return rc;
+  MxGemmArgs a{};
+  a.C = C; a.ldc = ldc; a.stride_c = l > 1 ? stride_c : 0;
+  a.l = l; a.k = k; a.out_type = dtype;
+  const long long size = elem_size(dtype);
+  a.vec_ok = ((reinterpret_cast<uintptr_t>(C) | (ldc * size) | (a.stride_c * size)) & 15) == 0;
+  const MxSide A{a_codes, stride_a, a_scales, stride_as, m}, B{b_codes, stride_b, b_scales, stride_bs, n};
+  if (m <= 16) return launch_mx_gemm<16, true>(stream, sms, B, A, a);
+  if (m <= 64) return launch_mx_gemm<64, true>(stream, sms, B, A, a);
+  return launch_mx_gemm<128, false>(stream, sms, A, B, a);
+}
+
+}  // extern "C"

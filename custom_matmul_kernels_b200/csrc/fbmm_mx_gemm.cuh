@@ -1,0 +1,347 @@
+// Product of two 4-bit microscaled operands on the block-scaled tensor cores:
+//   C[b][m][n] = sum_k 2^(Ea + Eb - 254) a[m][k] b[n][k],  scales per 32 elements of k.
+//
+// tcgen05.mma.kind::mxf4.block_scale multiplies the 4-bit elements and applies both scales itself;
+// products and scales are exact, the sum is kept in fp32 in tensor memory. A k-block of a stage is
+// 256 elements: 128 bytes of codes per row (one 128-byte swizzle row, four MMAs of 64 elements) and
+// two 512-byte groups of scales per 128 rows, which tcgen05.cp moves from shared to tensor memory
+// in the order they are stored in (fbmm_mx_quant.cuh). The tensor-memory columns of the scales
+// belong to the ring stage, so they are rewritten only after the commit that frees the stage.
+// Elements behind k are zero by the tensor maps' fill, but a group of scales behind the last one
+// does not exist and holds whatever the stage held before (255 would be NaN): the MMAs of such
+// groups are not issued.
+//
+// Roles of a CTA: warp 0 (one lane) issues the copies, warp 1 (one lane) the scale copies and MMAs,
+// warps 2-5 move accumulators to global memory. Persistent, one CTA per SM.
+#pragma once
+#include "fbmm_mx_quant.cuh"
+#include "sm100_primitives.cuh"
+
+namespace fbmm {
+
+__device__ unsigned int g_mx_status[1];  // bit 0: a bounded wait ran out
+
+constexpr int kMxM = 128;              // rows of the MMA's first operand per tile
+constexpr int kMxStageK = 256;         // elements of k per ring stage
+constexpr int kMxRowBytes = 128;       // their codes
+constexpr int kMxScaleStage = 1024;    // scale bytes of 128 rows per stage (two groups)
+constexpr uint32_t kMxSmemLimit = 227 * 1024;
+constexpr int kMxMaxStages = 8;
+constexpr int kMxThreads = 192;
+constexpr int kMxEpiBytes = 4 * 4096;  // staging, 4 KB per epilogue warp
+
+// One operand seen as rows x k.
+struct MxOperand {
+  const uint8_t* scales;
+  long long scale_stride;  // bytes between batches, 0 = shared
+  int rows;
+  int shared;              // codes are one matrix for every batch
+};
+
+struct MxGemmArgs {
+  MxOperand p, q;  // p supplies the 128-row operand of the MMA, q the other one
+  void* C;
+  long long ldc, stride_c;  // elements
+  int l, k;
+  int out_type;  // 0 fp32, 1 fp16, 2 bf16
+  int p_tiles, q_tiles;
+  int vec_ok;    // C's rows are 16-byte aligned
+};
+
+template <int BN, bool SWAP>
+struct MxShape {
+  static constexpr int kQGroups = (BN + 127) / 128;
+  static constexpr int kPBytes = kMxM * kMxRowBytes, kQBytes = BN * kMxRowBytes;
+  static constexpr int kSfCols = 8 + 8 * kQGroups;  // tensor-memory columns of a stage's scales
+  static constexpr int kStageBytes = kPBytes + kQBytes + kMxScaleStage * (1 + kQGroups);
+  static constexpr int kAccStages = BN > 128 ? 1 : 2;
+  static constexpr int kSfBase = BN * kAccStages;
+  static constexpr int kStagesFit = static_cast<int>((kMxSmemLimit - 1024 - 256 - kMxEpiBytes) / kStageBytes);
+  static constexpr int kStagesTmem = (512 - kSfBase) / kSfCols;
+  static constexpr int kStages0 = kStagesFit < kStagesTmem ? kStagesFit : kStagesTmem;
+  static constexpr int kStages = kStages0 < kMxMaxStages ? kStages0 : kMxMaxStages;
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + kMxEpiBytes + 256;
+  static constexpr uint32_t kTmemCols = 512;
+};
+
+struct MxBarriers {
+  uint64_t full[kMxMaxStages], empty[kMxMaxStages], acc_full[2], acc_empty[2];
+  uint32_t tmem_base, abort_flag;
+};
+static_assert(sizeof(MxBarriers) <= 256, "barrier block");
+
+// Instruction descriptor of kind::mxf4 with one UE8M0 scale per 32 elements: A and B e2m1 (1 at bits
+// 7 and 10), N >> 3 at 17, scale type UE8M0 at 23, M >> 4 at 24; bits 4 and 29 pick the pair of
+// bytes (0 or 2) of the scale words that belongs to an MMA.
+__host__ __device__ constexpr uint32_t mx_idesc(uint32_t m, uint32_t n, uint32_t sf) {
+  return (sf << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24) | (sf << 29);
+}
+// K-major codes, 128-byte swizzle, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t mx_desc_codes(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr >> 4) & 0x3fffu) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+         (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+// A 512-byte group of scales, no swizzle: 32 rows of 16 bytes, 8-row groups 128 bytes apart.
+__device__ __forceinline__ uint64_t mx_desc_scales(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr >> 4) & 0x3fffu) | (static_cast<uint64_t>(16 >> 4) << 16) |
+         (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
+}
+__device__ __forceinline__ void mx_umma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa,
+                                        uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
+      "}\n"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+// 512 bytes of scales -> 4 columns of tensor memory, in all four lane quarters.
+__device__ __forceinline__ void mx_copy_scales(uint32_t tmem, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+// Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) into shared memory.
+__device__ __forceinline__ void mx_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t mx_pack_out(int out_type, float a, float b) {
+  if (out_type == 2) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void mx_store_one(void* C, int out_type, long long at, float v) {
+  if (out_type == 0) static_cast<float*>(C)[at] = v;
+  else if (out_type == 1) static_cast<__half*>(C)[at] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(C)[at] = __float2bfloat16_rn(v);
+}
+
+// 32 rows x 32 columns of a warp (lane = row, v = its columns) -> row-major C. The lanes' 16-byte
+// pieces cross the warp's staging area (chunk index xor row, free of bank conflicts) so that a store
+// instruction covers whole 64- or 128-byte row pieces. `C0`: element (row 0, column 0) of the block.
+__device__ __forceinline__ void mx_store_rows(uint8_t* stage, const uint32_t (&v)[32], void* C, long long c0, long long ldc,
+                                              int out_type, int rows, int cols, bool vec) {
+  const int lane = static_cast<int>(lane_id());
+  uint4* st = reinterpret_cast<uint4*>(stage);
+  __syncwarp();
+  if (out_type == 0) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) st[lane * 8 + (c ^ (lane & 7))] = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+    __syncwarp();
+    float* out = static_cast<float*>(C) + c0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (lane >> 3), c = lane & 7;
+      const uint4 x = st[r * 8 + (c ^ (r & 7))];
+      if (r < rows) {
+        float* at = out + r * ldc + c * 4;
+        if (vec && c * 4 + 4 <= cols) {
+          *reinterpret_cast<uint4*>(at) = x;
+        } else {
+          const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) if (c * 4 + j < cols) at[j] = __uint_as_float(e[j]);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint32_t p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        p[j] = mx_pack_out(out_type, __uint_as_float(v[8 * c + 2 * j]), __uint_as_float(v[8 * c + 2 * j + 1]));
+      st[lane * 4 + (c ^ ((lane >> 1) & 3))] = make_uint4(p[0], p[1], p[2], p[3]);
+    }
+    __syncwarp();
+    uint16_t* out = static_cast<uint16_t*>(C) + c0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2), c = lane & 3;
+      const uint4 x = st[r * 4 + (c ^ ((r >> 1) & 3))];
+      if (r < rows) {
+        uint16_t* at = out + r * ldc + c * 8;
+        if (vec && c * 8 + 8 <= cols) {
+          *reinterpret_cast<uint4*>(at) = x;
+        } else {
+          const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) if (c * 8 + j < cols) at[j] = static_cast<uint16_t>(e[j >> 1] >> (16 * (j & 1)));
+        }
+      }
+    }
+  }
+}
+
+// SWAP = false: p = A, q = B, accumulator lanes are rows of C. SWAP = true: p = B, q = A (few rows
+// of A: the weights fill the 128-row side of the MMA), lanes are columns of C.
+template <int BN, bool SWAP>
+__global__ void __launch_bounds__(kMxThreads, 1)
+mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const MxGemmArgs a) {
+  using S = MxShape<BN, SWAP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* epi = smem + S::kStages * S::kStageBytes;
+  MxBarriers* bars = reinterpret_cast<MxBarriers*>(epi + kMxEpiBytes);
+  volatile uint32_t* abort_flag = &bars->abort_flag;
+  const uint32_t warp = threadIdx.x >> 5, lane = lane_id();
+  if (threadIdx.x == 0) {
+    bars->abort_flag = 0;
+    for (int s = 0; s < S::kStages; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
+    for (int s = 0; s < 2; ++s) { mbar_init(&bars->acc_full[s], 1); mbar_init(&bars->acc_empty[s], 4); }
+    fence_barrier_init();
+    tma_prefetch_desc(&map_p);
+    tma_prefetch_desc(&map_q);
+  }
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem_base, S::kTmemCols);
+    tmem_relinquish_alloc_permit();
+  }
+  tcgen05_fence_before_sync();
+  __syncthreads();
+  tcgen05_fence_after_sync();
+  const uint32_t tmem = bars->tmem_base;
+
+  const int kblocks = (a.k + kMxStageK - 1) / kMxStageK;
+  const int kgroups = (a.k + kMxGroupK - 1) / kMxGroupK;
+  const long long per_batch = static_cast<long long>(a.p_tiles) * a.q_tiles;
+  const long long units = per_batch * a.l;
+  auto decode = [&](long long u, int& b, int& pt, int& qt) {
+    b = static_cast<int>(u / per_batch);
+    const int r = static_cast<int>(u - b * per_batch);
+    pt = r % a.p_tiles;
+    qt = r / a.p_tiles;
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      for (long long u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        int b, pt, qt;
+        decode(u, b, pt, qt);
+        const uint8_t* sp = a.p.scales + b * a.p.scale_stride + static_cast<long long>(pt) * kgroups * kMxGroupBytes;
+        const int q_group = qt * BN / 128;  // first group of 128 rows of the q tile
+        const int q_groups = min(S::kQGroups, (a.q.rows + 127) / 128 - q_group);
+        const uint8_t* sq = a.q.scales + b * a.q.scale_stride + static_cast<long long>(q_group) * kgroups * kMxGroupBytes;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          ok = mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag);
+          if (!ok) break;
+          uint8_t* st = smem + stage * S::kStageBytes;
+          uint8_t* sf = st + S::kPBytes + S::kQBytes;
+          const uint32_t sf_bytes = static_cast<uint32_t>(min(2, kgroups - 2 * kb)) * kMxGroupBytes;
+          mbar_arrive_expect_tx(&bars->full[stage],
+                                S::kPBytes + S::kQBytes + sf_bytes * static_cast<uint32_t>(1 + q_groups));
+          tma_load_3d(st, &map_p, &bars->full[stage], kb * kMxRowBytes, pt * kMxM, a.p.shared ? 0 : b,
+                      SWAP ? kL2EvictFirst : kL2EvictLast);
+          tma_load_3d(st + S::kPBytes, &map_q, &bars->full[stage], kb * kMxRowBytes, qt * BN, a.q.shared ? 0 : b,
+                      kL2EvictLast);
+          mx_bulk_load(sf, sp + static_cast<long long>(kb) * kMxScaleStage, sf_bytes, &bars->full[stage]);
+          for (int g = 0; g < q_groups; ++g)
+            mx_bulk_load(sf + kMxScaleStage * (1 + g),
+                         sq + (static_cast<long long>(g) * kgroups + 2 * kb) * kMxGroupBytes, sf_bytes, &bars->full[stage]);
+          if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok) {  // copies in flight land before the CTA leaves
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) {}
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      bool ok = true;
+      for (long long u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        ok = mbar_wait(&bars->acc_empty[acc], acc_phase ^ 1u, abort_flag);
+        if (!ok) break;
+        tcgen05_fence_after_sync();
+        const uint32_t d = tmem + acc * BN;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          ok = mbar_wait(&bars->full[stage], phase, abort_flag);
+          if (!ok) break;
+          tcgen05_fence_after_sync();
+          const uint32_t st = smem_u32(smem + stage * S::kStageBytes);
+          const uint32_t sf = st + S::kPBytes + S::kQBytes;
+          const uint32_t t_sf = tmem + S::kSfBase + stage * S::kSfCols;
+          const int groups = min(2, kgroups - 2 * kb);
+          // columns of a stage: p's two groups, then for each group of k all of q's rows side by side
+          for (int g = 0; g < groups; ++g) {
+            mx_copy_scales(t_sf + g * 4, mx_desc_scales(sf + g * kMxGroupBytes));
+#pragma unroll
+            for (int r = 0; r < S::kQGroups; ++r)
+              mx_copy_scales(t_sf + 8 + g * 4 * S::kQGroups + r * 4,
+                             mx_desc_scales(sf + kMxScaleStage * (1 + r) + g * kMxGroupBytes));
+          }
+          const uint64_t pd = mx_desc_codes(st), qd = mx_desc_codes(st + S::kPBytes);
+          for (int g = 0; g < groups; ++g)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t step = static_cast<uint32_t>(g * 2 + j) * 2;  // 32 bytes of codes, in units of 16
+              mx_umma(d, pd + step, qd + step, mx_idesc(kMxM, BN, j * 2), t_sf + g * 4, t_sf + 8 + g * 4 * S::kQGroups,
+                      (kb | g | j) != 0 ? 1u : 0u);
+            }
+          umma_commit(&bars->empty[stage]);
+          if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        umma_commit(&bars->acc_full[acc]);
+        if (++acc == S::kAccStages) { acc = 0; acc_phase ^= 1u; }
+      }
+    }
+  } else {
+    const uint32_t quarter = warp & 3u;
+    uint8_t* stage_mem = epi + (warp - 2) * 4096;
+    uint32_t acc = 0, acc_phase = 0;
+    bool ok = true;
+    for (long long u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      int b, pt, qt;
+      decode(u, b, pt, qt);
+      ok = mbar_wait(&bars->acc_full[acc], acc_phase, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tcgen05_fence_after_sync();
+      const uint32_t t = tmem + acc * BN + ((quarter * 32u) << 16);
+      const int p0 = pt * kMxM + static_cast<int>(quarter) * 32;
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(t + c, v);
+        tmem_ld_wait();
+        const int q0 = qt * BN + c;
+        if (SWAP) {
+          const int n = p0 + static_cast<int>(lane);
+          if (n < a.p.rows) {
+            const long long at = b * a.stride_c + static_cast<long long>(q0) * a.ldc + n;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c + j < BN && q0 + j < a.q.rows) mx_store_one(a.C, a.out_type, at + j * a.ldc, __uint_as_float(v[j]));
+          }
+        } else {
+          mx_store_rows(stage_mem, v, a.C, b * a.stride_c + static_cast<long long>(p0) * a.ldc + q0, a.ldc, a.out_type,
+                        a.p.rows - p0, min(32, a.q.rows - q0), a.vec_ok != 0);
+        }
+      }
+      tcgen05_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->acc_empty[acc]);
+      if (++acc == S::kAccStages) { acc = 0; acc_phase ^= 1u; }
+    }
+  }
+  tcgen05_fence_before_sync();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag != 0) atomicOr(&g_mx_status[0], 1u);
+  if (warp == 1) {
+    tcgen05_fence_after_sync();
+    tmem_dealloc(tmem, S::kTmemCols);
+  }
+}
+
+}  // namespace fbmm

@@ -95,6 +95,14 @@ SIGNATURES = {
     "fbmm_kmeans_update_workspace_bytes": (_c_size, [_c_int, _c_int]),
     "fbmm_kmeans_update_f32": (_c_int, [_c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_int, _c_int, _c_ptr, _c_ll, _c_ptr,
                                         _c_ptr, _c_size]),
+    "fbmm_mx_codes_bytes": (_c_size, [_c_int] * 4),
+    "fbmm_mx_scales_bytes": (_c_size, [_c_int] * 3),
+    "fbmm_mx_quantize": (_c_int, [_c_ptr, _c_ptr, _c_int, _c_int, _c_ll, _c_ll, _c_int, _c_ptr, _c_ptr, _c_int, _c_int,
+                                  _c_int]),
+    "fbmm_mx_dequantize": (_c_int, [_c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_int, _c_ptr, _c_int, _c_ll, _c_ll, _c_int,
+                                    _c_int, _c_int]),
+    "fbmm_mx4_bmm": (_c_int, [_c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_int, _c_ll,
+                              _c_ll, _c_int, _c_int, _c_int, _c_int]),
 }
 
 _lib = None
@@ -163,7 +171,7 @@ def operand(X: torch.Tensor):
     return buf, False, cp, r * cp
 
 
-FBMM_F16, FBMM_BF16 = 1, 2
+FBMM_F32, FBMM_F16, FBMM_BF16 = 0, 1, 2
 
 
 def dtype_code_x16(dtype: torch.dtype) -> int:

@@ -54,7 +54,8 @@ extern "C" {
 #define FBMM_DIST_L2 1
 #define FBMM_DIST_L1 2   /* sum_k |a - b| (kernels/bmm_helpers.cu:46-52): fp32 min and top-k only, a SIMT kernel */
 
-/* Element types of the *_x16 entry points. */
+/* Element types of the *_x16 entry points; FBMM_F32 too for the fbmm_mx_* ones. */
+#define FBMM_F32 0
 #define FBMM_F16 1
 #define FBMM_BF16 2
 
@@ -286,6 +287,36 @@ size_t fbmm_kmeans_update_workspace_bytes(int k, int d);
 int fbmm_kmeans_update_f32(void* stream, const float* X, long long ldx, const long long* assignment,
                            long long n, int d, int k, float* centroids, long long ldc, float* counts_out,
                            void* workspace, size_t workspace_bytes);
+
+/* ---- microscaled operands ---------------------------------------------------------------
+ * A matrix [rows, k] as 4-bit (e2m1) or 8-bit (e4m3) elements with one power-of-two scale per
+ * block of 32 along k. No counterpart in the reference (its kernels take float* only).
+ *  - codes: [l][rows][ceil(k/32)*32*bits/8] bytes, two 4-bit elements per byte with the lower k
+ *    in the low half; elements behind k are zero.
+ *  - scales: [l][ceil(rows/128)][ceil(k/128)][512] bytes; in a group of 128 rows x 4 blocks, row r
+ *    and block b at byte (r % 32) * 16 + (r / 32) * 4 + b. A byte E stands for 2^(E - 127); bytes of
+ *    rows and blocks that do not exist are 0. 255 marks a block that held an infinity or a NaN:
+ *    all of its elements read as NaN.
+ *  - The scale of a block with largest magnitude a: 4 bits 2^(floor(log2 a) - 2), elements above
+ *    6 * scale saturate; 8 bits the least power of two that keeps a <= 448 * scale, bounded so that
+ *    every element * scale is a finite value of the source's type. Elements are rounded to
+ *    nearest, ties to even.
+ * Bases 16-byte aligned; batch strides in bytes, multiples of 16, 0 = one matrix for every batch. */
+size_t fbmm_mx_codes_bytes(int l, int rows, int k, int bits);
+size_t fbmm_mx_scales_bytes(int l, int rows, int k);
+/* X is [l][rows][k] (layout 'n', k contiguous) or [l][k][rows] (layout 't', rows contiguous), pitch
+ * ldx and batch stride in elements, any alignment of its type. codes and scales are written completely. */
+int fbmm_mx_quantize(void* stream, const void* X, int dtype, int layout, long long ldx, long long stride_x, int bits,
+                     unsigned char* codes, unsigned char* scales, int l, int rows, int k);
+/* out[l][rows][k] (pitch ldo) = element * scale, rounded once to dtype. */
+int fbmm_mx_dequantize(void* stream, const unsigned char* codes, long long stride_codes, const unsigned char* scales,
+                       long long stride_scales, int bits, void* out, int dtype, long long ldo, long long stride_o,
+                       int l, int rows, int k);
+/* C[l][m][n] = A @ B^T of two 4-bit operands, A [m, k] and B [n, k] (both with their blocks along k):
+ * products and scales exact, fp32 sums, C rounded once to dtype. */
+int fbmm_mx4_bmm(void* stream, const unsigned char* a_codes, long long stride_a, const unsigned char* a_scales,
+                 long long stride_as, const unsigned char* b_codes, long long stride_b, const unsigned char* b_scales,
+                 long long stride_bs, void* C, int dtype, long long ldc, long long stride_c, int l, int m, int n, int k);
 
 #ifdef __cplusplus
 }

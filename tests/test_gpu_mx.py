@@ -1,0 +1,251 @@
+"""Microscaled operators on the GPU against their plain 64-bit forms.
+
+Tolerances count roundings. A result type rounds once: half a step, eps / 2 relative. The fp32 sums
+of a product of K terms are off by at most K * 2^-23 of the sum of the terms' magnitudes (every
+addition may truncate at one step, 2^-23, of a partial sum, which that sum bounds)."""
+import pytest
+import torch
+
+from custom_matmul_kernels_b200 import (BMMCUDA, CheckpointBMMCUDA, MXBMMCUDA, MXDenseBMMCUDA, MXQuantizeCUDA, MXTensor)
+from oracle import mx_semantics as S
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def rnd(shape, seed, dtype=F32, spread=1.5):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=g) * torch.exp(spread * torch.randn(shape[:-1] + (1,), generator=g))
+    return x.to(dtype)
+
+
+def stored(X, bits):
+    """Oracle storage of X [l, rows, k]."""
+    out = [S.pack(*S.quantize(x, bits), bits) for x in X]
+    return torch.stack([o[0] for o in out]), torch.stack([o[1] for o in out])
+
+
+def as_mx(rows, k, bits, seed, dev, l=1, dim=-1, **kw):
+    parts = [S.random_mx(rows, k, bits, seed + i, **kw) for i in range(l)]
+    packed = [S.pack(c, s, bits) for c, s in parts]
+    vals = torch.stack([S.values(c, s, bits) for c, s in parts])
+    t = MXTensor(torch.stack([p[0] for p in packed]).to(dev), torch.stack([p[1] for p in packed]).to(dev), bits=bits, k=k,
+                 dim=dim)
+    return t, vals
+
+
+def assert_sum_close(got, want, magnitude, K, dtype):
+    """|got - want| <= rounding of the type + K * 2^-23 of the sum of magnitudes."""
+    tol = want.abs() * (torch.finfo(dtype).eps / 2) + magnitude * (K * 2.0 ** -23) * (1 + torch.finfo(dtype).eps)
+    tol = tol + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps  # half a step below the normal range
+    err = (got.double().cpu() - want).abs()
+    assert bool((err <= tol).all()), f"off by {float((err / tol).max()):.3g} tolerances"
+
+
+# ---- quantisation -----------------------------------------------------------------------------
+SHAPES = [(1, 1, 1), (1, 1, 31), (2, 3, 33), (1, 128, 128), (1, 129, 160), (3, 77, 257), (1, 200, 96), (2, 5, 1000)]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("l,rows,k", SHAPES)
+def test_quantize_storage(dev, l, rows, k, dtype, bits):
+    X = rnd((l, rows, k), rows * 1000 + k, dtype)
+    if rows > 2:
+        X[0, 1] = 0
+    codes, scales = stored(X, bits)
+    q = MXQuantizeCUDA(bits)(X.to(dev))
+    assert q.shape == (l, rows, k) and q.dim == -1
+    assert torch.equal(q.codes.cpu(), codes) and torch.equal(q.scales.cpu(), scales)
+    # along the other axis: the transposed matrix gives the same storage
+    for Xt in (X.transpose(1, 2).contiguous().to(dev), X.to(dev).transpose(1, 2)):
+        qt = MXQuantizeCUDA(bits)(Xt, dim=-2)
+        assert qt.shape == (l, k, rows)
+        assert torch.equal(qt.codes.cpu(), codes) and torch.equal(qt.scales.cpu(), scales)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_quantize_range_of_the_type(dev, dtype, bits):
+    """Blocks at the ends of the type's range: subnormals, the largest values, signed zeros."""
+    fi = torch.finfo(dtype)
+    tiny = fi.smallest_normal * fi.eps
+    rows = [[0.0] * 32, [-0.0] * 32, [tiny] * 32, [3 * tiny, -tiny] * 16, [fi.smallest_normal] * 32, [fi.max, -fi.max] * 16,
+            [fi.max * (1 - fi.eps), 1.0] * 16, [fi.max / 2, tiny] * 16, [1.75, 448.0] * 16, [1.7500001, 449.0] * 16,
+            [7.99, 6.0, 5.0, 2.5] * 8, [1.0, 0.25, 0.75, -1.25] * 8]
+    X = torch.tensor(rows, dtype=torch.float64).clamp(-fi.max, fi.max).to(dtype)[None]
+    codes, scales = stored(X, bits)
+    q = MXQuantizeCUDA(bits)(X.to(dev))
+    assert torch.equal(q.codes.cpu(), codes) and torch.equal(q.scales.cpu(), scales)
+    want = S.values(*S.quantize(X[0], bits), bits)
+    back = q.dequantize(F32)[0].cpu().double()
+    assert torch.equal(back, want)
+    if bits == 8:  # kept values are values of the source's type
+        assert torch.equal(q.dequantize(dtype)[0].cpu().double(), want)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_quantize_non_finite_blocks(dev, bits):
+    X = torch.ones(4, 96)
+    X[0, 5], X[1, 40], X[2, 70], X[2, 3] = float("nan"), float("inf"), float("-inf"), float("nan")
+    back = MXQuantizeCUDA(bits)(X.to(dev)).dequantize().cpu()
+    want = torch.ones(4, 96)
+    want[0, :32] = want[1, 32:64] = want[2, 64:] = want[2, :32] = float("nan")
+    assert torch.equal(torch.isnan(back), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(back), torch.nan_to_num(want))
+    back = MXQuantizeCUDA(bits)(X.t().to(dev).contiguous(), dim=-2).dequantize().cpu().t()
+    assert torch.equal(torch.isnan(back), torch.isnan(want))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_quantize_strides(dev, dtype, bits):
+    """Pitches, offsets and orders that vector loads cannot take."""
+    base = rnd((3, 150, 301), 5, dtype).to(dev)
+    for X in (base[:, :, 1:], base[:, 3:, :64], base[::2, :, :256], base[:, ::2], base[:, :, ::3], base[0], base[1, 7:8],
+              base[:1].expand(4, -1, -1), base.permute(1, 0, 2), base[:, :, 5:6]):
+        for dim in (-1, -2):
+            q, w = MXQuantizeCUDA(bits)(X, dim=dim), MXQuantizeCUDA(bits)(X.contiguous().clone(), dim=dim)
+            assert torch.equal(q.codes, w.codes) and torch.equal(q.scales, w.scales)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("l,rows,k", [(1, 1, 1), (2, 130, 100), (1, 40, 264)])
+def test_dequantize(dev, l, rows, k, dtype, bits):
+    q, v = as_mx(rows, k, bits, 3, dev, l)
+    assert torch.equal(q.dequantize(dtype).cpu(), v.to(F32).to(dtype))  # the fp32 value is exact
+    assert torch.equal(q.mT.dequantize(dtype).cpu(), v.transpose(1, 2).to(F32).to(dtype))
+
+
+# ---- 4-bit product ------------------------------------------------------------------------------
+PRODUCTS = [(1, 1, 1, 1), (1, 1, 129, 33), (2, 3, 5, 64), (1, 16, 200, 257), (1, 17, 128, 128), (3, 33, 70, 500),
+            (1, 64, 130, 96), (1, 65, 1, 31), (2, 128, 128, 256), (1, 129, 257, 640), (1, 300, 400, 1111), (4, 100, 1, 300)]
+
+
+@pytest.mark.parametrize("l,m,n,k", PRODUCTS)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_product_of_microscaled(dev, l, m, n, k, dtype):
+    A, a = as_mx(m, k, 4, 11, dev, l, lo=121, hi=125)
+    B, b = as_mx(n, k, 4, 977, dev, l, dim=-2, lo=121, hi=125)
+    C = MXBMMCUDA(out_dtype=dtype)(A, B)
+    assert C.shape == (l, m, n) and C.dtype == dtype
+    want = a @ b.transpose(1, 2)
+    assert_sum_close(C, want, a.abs() @ b.abs().transpose(1, 2), k, dtype)
+
+
+@pytest.mark.parametrize("m", [1, 16, 40, 200])
+def test_product_exact_integers(dev, m):
+    """Scales of one: every sum is a multiple of 1/4 below 2^22, so the result is exact."""
+    A, a = as_mx(m, 2000, 4, 1, dev, lo=127, hi=128)
+    B, b = as_mx(300, 2000, 4, 2, dev, dim=-2, lo=127, hi=128)
+    assert torch.equal(MXBMMCUDA()(A, B).cpu().double(), a @ b.transpose(1, 2))
+
+
+@pytest.mark.parametrize("m", [1, 30, 150])
+def test_product_scales_place(dev, m):
+    """One non-zero block per row, with a scale that names row and block: a scale that is
+    read from another place shows."""
+    n, k = 300, 1000
+    nb = (k + 31) // 32
+    ca, sa = torch.zeros((m, k), dtype=torch.int64), torch.zeros((m, nb), dtype=torch.int64)
+    cb, sb = torch.zeros((n, k), dtype=torch.int64), torch.zeros((n, nb), dtype=torch.int64)
+    for r in range(m):
+        b = r % nb
+        ca[r, 32 * b:32 * b + 1] = 2
+        sa[r] = 110 + (torch.arange(nb) * 7 + r) % 17
+    for r in range(n):
+        cb[r] = 2
+        sb[r] = 115 + (torch.arange(nb) * 5 + r * 3) % 13
+    pa, pb = S.pack(ca, sa, 4), S.pack(cb, sb, 4)
+    C = MXBMMCUDA()(MXTensor(pa[0].to(dev), pa[1].to(dev), k=k), MXTensor(pb[0].to(dev), pb[1].to(dev), k=k, dim=-2))
+    assert torch.equal(C.cpu().double(), S.values(ca, sa, 4) @ S.values(cb, sb, 4).t())
+
+
+def test_product_nan_blocks_stay_in_their_rows(dev):
+    for m in (5, 150):
+        ca, sa = S.random_mx(m, 600, 4, 1)
+        cb, sb = S.random_mx(140, 600, 4, 2)
+        sa[2, 18], sb[131, 0] = 255, 255
+        pa, pb = S.pack(ca, sa, 4), S.pack(cb, sb, 4)
+        C = MXBMMCUDA()(MXTensor(pa[0].to(dev), pa[1].to(dev), k=600), MXTensor(pb[0].to(dev), pb[1].to(dev), k=600, dim=-2))
+        want = S.values(ca, sa, 4) @ S.values(cb, sb, 4).t()
+        assert torch.equal(torch.isnan(C.cpu()), torch.isnan(want))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("l,m,n,k", [(1, 1, 300, 260), (1, 16, 130, 512), (2, 40, 140, 333), (1, 200, 260, 700)])
+def test_product_of_a_tensor(dev, l, m, n, k, dtype):
+    X = rnd((l, m, k), 31, dtype)
+    B, b = as_mx(n, k, 4, 9, dev, l, dim=-2, lo=119, hi=123)
+    a = torch.stack([S.values(*S.quantize(x, 4), 4) for x in X])
+    want = a @ b.transpose(1, 2)
+    C = MXBMMCUDA()(X.to(dev), B)
+    assert C.dtype == dtype
+    assert_sum_close(C, want, a.abs() @ b.abs().transpose(1, 2), k, dtype)
+    if l == 1:
+        B2 = MXTensor(B.codes[0], B.scales[0], k=k, dim=-2)
+        assert torch.equal(MXBMMCUDA()(X[0].to(dev), B2), C[0])
+
+
+def test_product_shared_operands(dev):
+    """Batch strides of 0 on either side give what copies give."""
+    for m in (4, 150):
+        A, _ = as_mx(m, 300, 4, 1, dev)
+        B, _ = as_mx(260, 300, 4, 2, dev, 3, dim=-2)
+        A3 = MXTensor(A.codes.expand(3, -1, -1), A.scales.expand(3, -1, -1, -1), k=300)
+        Ac = MXTensor(A.codes.repeat(3, 1, 1), A.scales.repeat(3, 1, 1, 1), k=300)
+        assert A3._strides() == (0, 0)
+        assert torch.equal(MXBMMCUDA()(A3, B), MXBMMCUDA()(Ac, B))
+        assert torch.equal(MXBMMCUDA()(B.mT, A3.mT), MXBMMCUDA()(B.mT, Ac.mT))
+
+
+def test_product_empty(dev):
+    B, _ = as_mx(40, 64, 4, 1, dev, dim=-2)
+    assert MXBMMCUDA()(torch.empty(1, 0, 64, device=dev), B).shape == (1, 0, 40)
+    q = MXQuantizeCUDA(4)(torch.empty(0, 5, 64, device=dev))
+    assert q.shape == (0, 5, 64) and q.dequantize().shape == (0, 5, 64)
+
+
+# ---- gradients -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("l,m,j,c", [(1, 1, 1, 1), (1, 64, 64, 64), (2, 70, 130, 200), (1, 300, 129, 257), (3, 5, 1000, 33),
+                                     (1, 257, 640, 300)])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_dense_product(dev, l, m, j, c, dtype, bits):
+    """P @ Q in both layouts of P."""
+    P = rnd((l, m, j), 3, dtype, 0.3)
+    Q, q = as_mx(j, c, bits, 17, dev, l, lo=120, hi=124)
+    want, mag = P.double() @ q, P.double().abs() @ q.abs()
+    for X in (P.to(dev), P.transpose(1, 2).contiguous().to(dev).transpose(1, 2)):
+        C = MXDenseBMMCUDA()(X, Q)
+        assert C.shape == (l, m, c) and C.dtype == dtype
+        assert_sum_close(C, want, mag, j, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("l,m,n,k", [(1, 5, 40, 64), (2, 130, 200, 300)])
+def test_frozen_weights_gradient(dev, l, m, n, k, dtype):
+    W, w = as_mx(n, k, 4, 5, dev, l, dim=-2, lo=120, hi=124)
+    X = rnd((l, m, k), 8, dtype, 0.5).to(dev).requires_grad_()
+    dC = rnd((l, m, n), 9, dtype, 0.3)
+    C = MXBMMCUDA()(X, W)
+    assert torch.equal(C.detach(), MXBMMCUDA()(X.detach(), W))
+    dX, = torch.autograd.grad(C, X, dC.to(dev))
+    tol_k = n * (1 if dtype != F32 else 8)  # the fp32 product splits each term in three
+    assert_sum_close(dX, dC.double() @ w, dC.double().abs() @ w.abs(), tol_k, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("l,m,n,k", [(1, 1, 1, 1), (1, 64, 96, 128), (2, 77, 130, 33), (1, 300, 257, 200)])
+def test_checkpoint_gradients(dev, l, m, n, k, dtype):
+    A, B, dC = rnd((l, m, k), 1, dtype, 0.5), rnd((l, k, n), 2, dtype, 0.2), rnd((l, m, n), 3, dtype, 0.2)
+    a8 = torch.stack([S.values(*S.quantize(x, 8), 8) for x in A])
+    Ad, Bd = A.to(dev).requires_grad_(), B.to(dev).requires_grad_()
+    C = CheckpointBMMCUDA()(Ad, Bd)
+    assert torch.equal(C.detach(), BMMCUDA()(A.to(dev), B.to(dev)))
+    dA, dB = torch.autograd.grad(C, (Ad, Bd), dC.to(dev))
+    f = 8 if dtype == F32 else 1
+    a, b, d = A.double(), B.double(), dC.double()
+    assert_sum_close(dA, d @ b.transpose(1, 2), d.abs() @ b.abs().transpose(1, 2), f * n, dtype)
+    assert_sum_close(dB, a8.transpose(1, 2) @ d, a8.abs().transpose(1, 2) @ d.abs(), f * m, dtype)
