@@ -6,6 +6,7 @@
 #include "fbmm_host.h"
 #include "fbmm_mx_gemm.cuh"
 #include "fbmm_mx_quant.cuh"
+#include "fbmm_x16_gemm.cuh"
 
 namespace {
 
@@ -98,6 +99,131 @@ int launch_mx_gemm(cudaStream_t stream, int sms, const MxSide& p, const MxSide& 
   FBMM_HOST_CUDA(cudaFuncSetAttribute(mx_gemm_kernel<BN, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
   mx_gemm_kernel<BN, SWAP><<<static_cast<unsigned>(std::min<long long>(units, sms)), kMxThreads, S::kSmem, stream>>>(mp, mq, a);
   FBMM_HOST_CUDA(cudaGetLastError());
+  return FBMM_OK;
+}
+
+// One operand of a 16-bit product: a dense matrix of `rows` x J (J contiguous, or the rows), or a
+// microscaled one stored [J][rows] with its blocks along the rows.
+struct X16Side {
+  int kind;
+  const void* ptr;              // elements or codes
+  long long ld, stride;         // elements (dense); stride in bytes for codes
+  const unsigned char* scales;
+  long long scale_stride;
+  int rows;
+};
+
+int check_x16_side(const char* name, const X16Side& s, int J, int l) {
+  if (s.kind >= kX16Mx4)
+    return check_mx(name, static_cast<const unsigned char*>(s.ptr), s.stride, s.scales, s.scale_stride, l);
+  if (s.ptr == nullptr) return fail(FBMM_ERR_INVALID, "%s is null", name);
+  const int inner = s.kind == kX16K ? J : s.rows;
+  if (s.ld < inner) return fail(FBMM_ERR_INVALID, "%s pitch %lld smaller than its row length %d", name, s.ld, inner);
+  if ((reinterpret_cast<uintptr_t>(s.ptr) & 15u) != 0) return fail(FBMM_ERR_ALIGN, "%s is not 16-byte aligned", name);
+  if ((s.ld & 7) != 0) return fail(FBMM_ERR_ALIGN, "%s pitch %lld is not a multiple of 8 elements", name, s.ld);
+  if (l > 1 && ((s.stride & 7) != 0 || s.stride < 0))
+    return fail(FBMM_ERR_ALIGN, "%s batch stride %lld is not a non-negative multiple of 8 elements", name, s.stride);
+  return FBMM_OK;
+}
+
+int x16_map(CUtensorMap* map, const X16Side& s, int J, int l, int dtype) {
+  const bool one = l == 1 || s.stride == 0;
+  const cuuint64_t batches = one ? 1u : static_cast<cuuint64_t>(l);
+  if (s.kind >= kX16Mx4) {
+    const int bits = s.kind == kX16Mx4 ? 4 : 8;
+    const cuuint64_t pitch = static_cast<cuuint64_t>(mx_pitch(s.rows, bits));
+    const cuuint64_t dims[3] = {pitch, static_cast<cuuint64_t>(J), batches};
+    const cuuint64_t strides[2] = {pitch, one ? pitch * dims[1] : static_cast<cuuint64_t>(s.stride)};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 * bits / 8), kX16J, 1};
+    return fbmm_host::tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, s.ptr, dims, strides, box, false);
+  }
+  const bool kmajor = s.kind == kX16K;
+  const cuuint64_t pitch = static_cast<cuuint64_t>(s.ld) * 2u;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(kmajor ? J : s.rows), static_cast<cuuint64_t>(kmajor ? s.rows : J), batches};
+  const cuuint64_t strides[2] = {pitch, one ? pitch * dims[1] : static_cast<cuuint64_t>(s.stride) * 2u};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(kmajor ? 128 : kX16J), 1};
+  return fbmm_host::tensor_map_3d(map, dtype == FBMM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                                  s.ptr, dims, strides, box, true);
+}
+
+template <int XK, int YK, bool PAIR>
+int launch_x16(cudaStream_t stream, int sms, const CUtensorMap& mx, const CUtensorMap& my, X16Args a) {
+  using S = X16Shape<XK, YK>;
+  constexpr int kTile = PAIR ? 256 : 128;
+  a.x_tiles = (a.x.rows + kTile - 1) / kTile;
+  a.y_tiles = (a.y.rows + kTile - 1) / kTile;
+  const long long units = static_cast<long long>(a.x_tiles) * a.y_tiles * a.l;
+  FBMM_HOST_CUDA(cudaFuncSetAttribute(x16_gemm_kernel<XK, YK, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(PAIR ? 2 * std::min<long long>(units, sms / 2) : std::min<long long>(units, sms)));
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+  if (PAIR) { cfg.attrs = &attr; cfg.numAttrs = 1; }
+  FBMM_HOST_CUDA(cudaLaunchKernelEx(&cfg, x16_gemm_kernel<XK, YK, PAIR>, mx, my, a));
+  return FBMM_OK;
+}
+
+template <int XK, int YK>
+int launch_x16_any(cudaStream_t stream, int sms, const CUtensorMap& mx, const CUtensorMap& my, const X16Args& a) {
+  // 256 x 256 tiles on pairs unless they leave SMs idle: a wave of pair tiles takes about twice a wave of
+  // 128 x 128 tiles (four times the work at twice the rate)
+  auto waves = [&](int tile, long long workers) {
+    const long long units = static_cast<long long>((a.x.rows + tile - 1) / tile) * ((a.y.rows + tile - 1) / tile) * a.l;
+    return (units + workers - 1) / workers;
+  };
+  if (2 * waves(256, sms / 2) <= waves(128, sms)) return launch_x16<XK, YK, true>(stream, sms, mx, my, a);
+  return launch_x16<XK, YK, false>(stream, sms, mx, my, a);
+}
+
+int x16_product(cudaStream_t stream, const X16Side& x, const X16Side& y, int dtype, void* C, long long ldc,
+                long long stride_c, int l, int J, const char* xn, const char* yn) {
+  int rc, sms;
+  if (l <= 0 || x.rows <= 0 || y.rows <= 0 || J <= 0)
+    return fail(FBMM_ERR_INVALID, "all extents must be positive, got %d %d %d %d", l, x.rows, y.rows, J);
+  if (dtype != FBMM_F16 && dtype != FBMM_BF16)
+    return fail(FBMM_ERR_INVALID, "dtype must be FBMM_F16 (1) or FBMM_BF16 (2), got %d", dtype);
+  if ((rc = check_x16_side(xn, x, J, l)) != FBMM_OK) return rc;
+  if ((rc = check_x16_side(yn, y, J, l)) != FBMM_OK) return rc;
+  if (C == nullptr) return fail(FBMM_ERR_INVALID, "C is null");
+  if ((reinterpret_cast<uintptr_t>(C) & 1u) != 0) return fail(FBMM_ERR_ALIGN, "C is not 2-byte aligned");
+  if (ldc < y.rows) return fail(FBMM_ERR_INVALID, "ldc %lld smaller than a row of C (%d)", ldc, y.rows);
+  if (l > 1 && stride_c < static_cast<long long>(x.rows - 1) * ldc + y.rows)
+    return fail(FBMM_ERR_INVALID, "batches of C overlap (stride %lld)", stride_c);
+  if (static_cast<long long>((x.rows + 127) / 128) * ((y.rows + 127) / 128) > 0x3fffffffLL)
+    return fail(FBMM_ERR_INVALID, "product of %d x %d is too large", x.rows, y.rows);
+  if ((rc = fbmm_host::device_sms(&sms)) != FBMM_OK) return rc;
+  CUtensorMap mx, my;
+  if ((rc = x16_map(&mx, x, J, l, dtype)) != FBMM_OK) return rc;
+  if ((rc = x16_map(&my, y, J, l, dtype)) != FBMM_OK) return rc;
+  X16Args a{};
+  a.x = X16Operand{x.scales, l > 1 ? x.scale_stride : 0, x.rows, l > 1 && x.stride == 0};
+  a.y = X16Operand{y.scales, l > 1 ? y.scale_stride : 0, y.rows, l > 1 && y.stride == 0};
+  a.C = C; a.ldc = ldc; a.stride_c = l > 1 ? stride_c : 0;
+  a.l = l; a.J = J; a.dtype = dtype;
+  a.vec_ok = ((reinterpret_cast<uintptr_t>(C) | (ldc * 2) | (a.stride_c * 2)) & 15) == 0;
+#define FBMM_X16(XK, YK) \
+  if (x.kind == XK && y.kind == YK) return launch_x16_any<XK, YK>(stream, sms, mx, my, a)
+  FBMM_X16(kX16K, kX16K);
+  FBMM_X16(kX16K, kX16MN);
+  FBMM_X16(kX16MN, kX16K);
+  FBMM_X16(kX16MN, kX16MN);
+  FBMM_X16(kX16K, kX16Mx4);
+  FBMM_X16(kX16MN, kX16Mx4);
+  FBMM_X16(kX16K, kX16Mx8);
+  FBMM_X16(kX16MN, kX16Mx8);
+  FBMM_X16(kX16Mx4, kX16MN);
+  FBMM_X16(kX16Mx8, kX16MN);
+#undef FBMM_X16
+  return fail(FBMM_ERR_INVALID, "internal: no kernel for kinds %d and %d", x.kind, y.kind);
+}
+
+int layout_kind(const char* name, int letter, int k_major_letter, int* kind) {
+  if (letter != 'n' && letter != 't') return fail(FBMM_ERR_INVALID, "%s layout must be 'n' or 't', got %d", name, letter);
+  *kind = letter == k_major_letter ? kX16K : kX16MN;
   return FBMM_OK;
 }
 
@@ -207,6 +333,59 @@ int fbmm_mx4_bmm(void* stream_, const unsigned char* a_codes, long long stride_a
   if (m <= 16) return launch_mx_gemm<16, true>(stream, sms, B, A, a);
   if (m <= 64) return launch_mx_gemm<64, true>(stream, sms, B, A, a);
   return launch_mx_gemm<128, false>(stream, sms, A, B, a);
+}
+
+size_t fbmm_mx4_bmm_tensor_workspace_bytes(int l, int m, int k) {
+  const size_t codes = fbmm_mx_codes_bytes(l, m, k, 4);
+  return (codes + 255) / 256 * 256 + fbmm_mx_scales_bytes(l, m, k);
+}
+
+int fbmm_mx4_bmm_tensor(void* stream, const void* A, int a_dtype, int a_layout, long long lda, long long stride_a,
+                        const unsigned char* b_codes, long long stride_b, const unsigned char* b_scales,
+                        long long stride_bs, void* C, int dtype, long long ldc, long long stride_c, int l, int m, int n,
+                        int k, void* workspace, size_t workspace_bytes) {
+  const size_t need = fbmm_mx4_bmm_tensor_workspace_bytes(l, m, k);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(FBMM_ERR_WORKSPACE, "fbmm_mx4_bmm_tensor needs %zu workspace bytes, got %zu", need,
+                workspace == nullptr ? static_cast<size_t>(0) : workspace_bytes);
+  unsigned char* codes = static_cast<unsigned char*>(workspace);
+  unsigned char* scales = codes + (need - fbmm_mx_scales_bytes(l, m, k));
+  const int rc = fbmm_mx_quantize(stream, A, a_dtype, a_layout, lda, stride_a, 4, codes, scales, l, m, k);
+  if (rc != FBMM_OK) return rc;
+  return fbmm_mx4_bmm(stream, codes, static_cast<long long>(m) * mx_pitch(k, 4), scales, mx_scale_bytes(m, k), b_codes,
+                      stride_b, b_scales, stride_bs, C, dtype, ldc, stride_c, l, m, n, k);
+}
+
+int fbmm_dense_bmm_x16(void* stream, const void* A, int a_layout, long long lda, long long stride_a, const void* B,
+                       int b_layout, long long ldb, long long stride_b, int dtype, void* C, long long ldc,
+                       long long stride_c, int l, int m, int n, int k) {
+  X16Side x{0, A, lda, stride_a, nullptr, 0, m}, y{0, B, ldb, stride_b, nullptr, 0, n};
+  int rc;
+  if ((rc = layout_kind("A", a_layout, 'n', &x.kind)) != FBMM_OK) return rc;
+  if ((rc = layout_kind("B", b_layout, 't', &y.kind)) != FBMM_OK) return rc;
+  return x16_product(static_cast<cudaStream_t>(stream), x, y, dtype, C, ldc, stride_c, l, k, "A", "B");
+}
+
+int fbmm_dense_mx_bmm_x16(void* stream, const void* A, int a_layout, long long lda, long long stride_a, int dtype,
+                          const unsigned char* b_codes, long long stride_b, const unsigned char* b_scales,
+                          long long stride_bs, int bits, void* C, long long ldc, long long stride_c, int l, int m, int n,
+                          int k) {
+  int rc;
+  if ((rc = check_bits(bits)) != FBMM_OK) return rc;
+  X16Side x{0, A, lda, stride_a, nullptr, 0, m};
+  const X16Side y{bits == 4 ? kX16Mx4 : kX16Mx8, b_codes, 0, stride_b, b_scales, stride_bs, n};
+  if ((rc = layout_kind("A", a_layout, 'n', &x.kind)) != FBMM_OK) return rc;
+  return x16_product(static_cast<cudaStream_t>(stream), x, y, dtype, C, ldc, stride_c, l, k, "A", "B");
+}
+
+int fbmm_mx_dense_bmm_x16(void* stream, const unsigned char* a_codes, long long stride_a, const unsigned char* a_scales,
+                          long long stride_as, int bits, const void* B, long long ldb, long long stride_b, int dtype,
+                          void* C, long long ldc, long long stride_c, int l, int m, int n, int k) {
+  int rc;
+  if ((rc = check_bits(bits)) != FBMM_OK) return rc;
+  const X16Side x{bits == 4 ? kX16Mx4 : kX16Mx8, a_codes, 0, stride_a, a_scales, stride_as, m};
+  const X16Side y{kX16MN, B, ldb, stride_b, nullptr, 0, n};
+  return x16_product(static_cast<cudaStream_t>(stream), x, y, dtype, C, ldc, stride_c, l, k, "A", "B");
 }
 
 }  // extern "C"

@@ -1,0 +1,337 @@
+// 16-bit products for training: D[b][x][y] = sum_j X[b][x][j] * Y[b][y][j] with fp32 sums, each
+// operand fp16 / bf16 in either storage order, or one of them microscaled (fbmm_mx_quant.cuh) with
+// its blocks along its own output axis. The forward pass, the gradient of the activations
+// and the gradient of the weights from 8-bit activations are this one product in three layouts:
+//   C  = A B        X = A [m][k]        j contiguous     Y = B [k][n]   y contiguous (or B^T stored: j)
+//   dA = dC B^T     X = dC [m][n]       j contiguous     Y = B [k][n]   j contiguous
+//   dB = A8^T dC    X = A8 [m][k]       microscaled      Y = dC [m][n]  y contiguous
+//   dA = dC W4      X = dC              j contiguous     Y = W4 [n][k]  microscaled
+//
+// tcgen05.mma.kind::f16 takes both K-major and MN-major tiles, so no operand is transposed in memory.
+// Microscaled codes arrive raw by TMA (8 KB or 4 KB per stage, half or a quarter of what the
+// 16-bit values would take out of L2) with their 512-byte group of scales; four warps turn them into
+// 16-bit values (code * 2^(E-127), rounded to the type: exact for bf16) in the MN-major
+// swizzled tile that the MMA reads. A dequantised copy of the operand never exists in memory.
+//
+// PAIR: two CTAs (cta_group::2) share a 256 x 256 tile, each supplying 128 rows of X and 128 of Y
+// from its own shared memory, so per 64 elements of j a CTA fetches 32 KB for 512 cycles of MMA;
+// without it a CTA does a 128 x 128 tile (the same 32 KB for 256 cycles), for products with few tiles.
+//
+// Roles of a CTA: warp 0 copies, warp 1 (the even CTA's) MMAs, four warps for codes where an operand
+// is microscaled, four warps for the epilogue. Two accumulator stages, persistent.
+#pragma once
+#include "fbmm_mx_gemm.cuh"
+
+namespace fbmm {
+
+enum X16Kind { kX16K = 0, kX16MN = 1, kX16Mx4 = 2, kX16Mx8 = 3 };
+
+constexpr int kX16J = 64;                   // j per stage: 128 bytes of a K-major row
+constexpr int kX16Part = 128 * kX16J * 2;   // 16 KB: 128 rows of one operand
+constexpr int kX16Stages = 5;
+constexpr int kX16Chunk = 64 * kX16J * 2;   // MN-major: 64 rows x 64 j
+
+struct X16Operand {
+  const uint8_t* scales;   // microscaled: groups [j / 128][rows / 128][512]
+  long long scale_stride;  // bytes, 0 = shared
+  int rows;
+  int shared;
+};
+
+struct X16Args {
+  X16Operand x, y;
+  void* C;
+  long long ldc, stride_c;
+  int l, J;
+  int dtype;     // 1 fp16, 2 bf16
+  int x_tiles, y_tiles;
+  int vec_ok;
+};
+
+template <int XK, int YK>
+struct X16Shape {
+  static constexpr bool kMx = XK >= kX16Mx4 || YK >= kX16Mx4;
+  static constexpr int kBits = (XK == kX16Mx4 || YK == kX16Mx4) ? 4 : 8;
+  static constexpr int kRaw = kMx ? kX16J * 128 * kBits / 8 + kMxGroupBytes : 0;
+  static constexpr int kStageBytes = 2 * kX16Part + (kMx ? (kRaw + 1023) / 1024 * 1024 : 0);
+  static constexpr int kSmem = 1024 + kX16Stages * kStageBytes + kMxEpiBytes + 256;
+  static constexpr int kThreads = kMx ? 320 : 192;
+  static constexpr int kEpiWarp = kMx ? 6 : 2;
+};
+
+struct X16Barriers {
+  uint64_t full[kX16Stages], raw[kX16Stages], empty[kX16Stages], acc_full[2], acc_empty[2];
+  uint32_t tmem_base, abort_flag;
+};
+static_assert(sizeof(X16Barriers) <= 256, "barrier block");
+
+__device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
+      "}\n"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Shared-memory descriptor of a 128-row part with the 128-byte swizzle. K-major: 8-row groups 1024
+// bytes apart, an MMA step (16 j) is 32 bytes. MN-major: chunks of 64 rows kX16Chunk apart, 8-j groups 1024 bytes
+// apart, an MMA step is 2048 bytes.
+__device__ __forceinline__ uint64_t x16_desc(uint32_t smem_addr, bool mn_major) {
+  const uint64_t lbo = mn_major ? kX16Chunk : 16;
+  return static_cast<uint64_t>((smem_addr >> 4) & 0x3fffu) | ((lbo >> 4) << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) |
+         (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+
+// A stage's raw codes -> 16-bit values in MN-major order; 128 threads, 16 codes at a time (half a
+// block, so one scale). Lanes of the second 64 rows write their two 16-byte pieces in the other order, which
+// keeps the eight lanes of a row on different banks.
+template <int BITS, bool BF16>
+__device__ __forceinline__ void x16_expand(const uint8_t* raw, uint8_t* dst, int j0, int j_end, int tid) {
+  const uint8_t* sc = raw + kX16J * 128 * BITS / 8;
+#pragma unroll
+  for (int it = 0; it < 4; ++it) {
+    const int i = it * 128 + tid;
+    const int j = i >> 3, u = i & 7;
+    uint32_t h[8];
+    if (BITS == 8) {
+      const uint4 c = *reinterpret_cast<const uint4*>(raw + j * 128 + u * 16);
+      mx_unpack8(c.x, h[0], h[1]);
+      mx_unpack8(c.y, h[2], h[3]);
+      mx_unpack8(c.z, h[4], h[5]);
+      mx_unpack8(c.w, h[6], h[7]);
+    } else {
+      const uint2 c = *reinterpret_cast<const uint2*>(raw + j * 64 + u * 8);
+      uint32_t a[4], b[4];
+      mx_unpack4(c.x, a);
+      mx_unpack4(c.y, b);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) { h[q] = a[q]; h[q + 4] = b[q]; }
+    }
+    // rows behind the last j are zero codes, but their scale bytes may be anything
+    const float s = j0 + j < j_end ? mx_scale_value(sc[mx_scale_at((j0 + j) & 127, u >> 1)]) : 0.f;
+    uint32_t w[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float2 f = mx_half2_floats(h[q]);
+      w[q] = mx_pack_out(BF16 ? 2 : 1, f.x * s, f.y * s);
+    }
+    uint8_t* row = dst + (u >> 2) * kX16Chunk + j * 128;
+    const int first = u >> 2;  // 0 or 1
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {
+      const int p = o ^ first;
+      const int unit = ((u & 3) * 2 + p) ^ (j & 7);
+      *reinterpret_cast<uint4*>(row + unit * 16) =
+          p ? make_uint4(w[4], w[5], w[6], w[7]) : make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// Tiles in bands of 8 along x, so that the tiles in flight share few rows of either operand.
+__device__ __forceinline__ void x16_decode(long long u, int x_tiles, int y_tiles, int& b, int& xt, int& yt) {
+  const long long per_batch = static_cast<long long>(x_tiles) * y_tiles;
+  b = static_cast<int>(u / per_batch);
+  const int r = static_cast<int>(u - b * per_batch);
+  const int band = r / (8 * y_tiles);
+  const int in = r - band * 8 * y_tiles;
+  const int height = min(8, x_tiles - band * 8);
+  yt = in / height;
+  xt = band * 8 + in - yt * height;
+}
+
+template <int XK, int YK, bool PAIR>
+__global__ void __launch_bounds__(X16Shape<XK, YK>::kThreads, 1)
+x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y, const X16Args a) {
+  using S = X16Shape<XK, YK>;
+  constexpr int kCtas = PAIR ? 2 : 1;
+  constexpr int kTile = 128 * kCtas;
+  constexpr uint32_t kDense = (XK < kX16Mx4 ? kX16Part : 0) + (YK < kX16Mx4 ? kX16Part : 0);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* epi = smem + kX16Stages * S::kStageBytes;
+  X16Barriers* bars = reinterpret_cast<X16Barriers*>(epi + kMxEpiBytes);
+  volatile uint32_t* abort_flag = &bars->abort_flag;
+  const uint32_t warp = threadIdx.x >> 5, lane = lane_id();
+  const uint32_t rank = PAIR ? cluster_cta_rank() : 0u;
+  if (threadIdx.x == 0) {
+    bars->abort_flag = 0;
+    for (int s = 0; s < kX16Stages; ++s) {
+      mbar_init(&bars->full[s], 1 + (S::kMx ? 4 * kCtas : 0));
+      mbar_init(&bars->raw[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) { mbar_init(&bars->acc_full[s], 1); mbar_init(&bars->acc_empty[s], 4 * kCtas); }
+    fence_barrier_init();
+    tma_prefetch_desc(&map_x);
+    tma_prefetch_desc(&map_y);
+  }
+  if (warp == 1) {
+    if (PAIR) { tmem_alloc_pair(&bars->tmem_base, 512); tmem_relinquish_alloc_permit_pair(); }
+    else { tmem_alloc(&bars->tmem_base, 512); tmem_relinquish_alloc_permit(); }
+  }
+  tcgen05_fence_before_sync();
+  if (PAIR) cluster_sync_all(); else __syncthreads();
+  tcgen05_fence_after_sync();
+  const uint32_t tmem = bars->tmem_base;
+  const uint32_t bars0 = PAIR ? map_to_cta(smem_u32(bars), 0) : smem_u32(bars);
+  const uint32_t bars1 = PAIR ? map_to_cta(smem_u32(bars), 1) : smem_u32(bars);
+  auto off = [&](const uint64_t* b) -> uint32_t { return smem_u32(b) - smem_u32(bars); };
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    return PAIR ? mbar_wait_cluster(bar, parity, abort_flag) : mbar_wait(bar, parity, abort_flag);
+  };
+  auto commit = [&](uint64_t* bar) {
+    if (PAIR) { umma_commit_pair(bars0 + off(bar)); umma_commit_pair(bars1 + off(bar)); }
+    else umma_commit(bar);
+  };
+  auto arrive_leader = [&](uint64_t* bar) {  // one arrival per warp
+    __syncwarp();
+    if (lane == 0) {
+      if (PAIR && rank != 0) mbar_arrive_cluster(bars0 + off(bar)); else mbar_arrive(bar);
+    }
+  };
+
+  const int jblocks = (a.J + kX16J - 1) / kX16J;
+  const long long units = static_cast<long long>(a.x_tiles) * a.y_tiles * a.l;
+  const long long u0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, du = PAIR ? gridDim.x >> 1 : gridDim.x;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      // 128 rows of one operand, from row r0: to the part's place, or its raw codes
+      auto load = [&](const CUtensorMap* map, int kind, uint8_t* part, uint8_t* raw, int j0, int r0, int b,
+                      const X16Operand& op) {
+        if (op.shared) b = 0;
+        uint64_t* full = &bars->full[stage];
+        if (kind == kX16K) {
+          if (PAIR) tma_load_3d_pair(part, map, bars0 + off(full), j0, r0, b, kL2EvictLast);
+          else tma_load_3d(part, map, full, j0, r0, b, kL2EvictLast);
+        } else if (kind == kX16MN) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            if (PAIR) tma_load_3d_pair(part + c * kX16Chunk, map, bars0 + off(full), r0 + c * 64, j0, b, kL2EvictLast);
+            else tma_load_3d(part + c * kX16Chunk, map, full, r0 + c * 64, j0, b, kL2EvictLast);
+          }
+        } else {
+          const int bytes = kX16J * 128 * S::kBits / 8;
+          const int groups = (op.rows + 127) / 128;
+          const bool exists = r0 < op.rows;
+          mbar_arrive_expect_tx(&bars->raw[stage], bytes + (exists ? kMxGroupBytes : 0));
+          tma_load_3d(raw, map, &bars->raw[stage], r0 * S::kBits / 8, j0, b, kL2EvictLast);
+          if (exists)
+            mx_bulk_load(raw + bytes,
+                         op.scales + b * op.scale_stride +
+                             (static_cast<long long>(j0 / 128) * groups + r0 / 128) * kMxGroupBytes,
+                         kMxGroupBytes, &bars->raw[stage]);
+        }
+      };
+      for (long long u = u0; u < units && ok; u += du) {
+        int b, xt, yt;
+        x16_decode(u, a.x_tiles, a.y_tiles, b, xt, yt);
+        const int xr = xt * kTile + static_cast<int>(rank) * 128, yr = yt * kTile + static_cast<int>(rank) * 128;
+        for (int jb = 0; jb < jblocks; ++jb) {
+          ok = wait(&bars->empty[stage], phase ^ 1u);
+          if (!ok) break;
+          uint8_t* st = smem + stage * S::kStageBytes;
+          if (rank == 0) mbar_arrive_expect_tx(&bars->full[stage], kDense * kCtas);
+          load(&map_x, XK, st, st + 2 * kX16Part, jb * kX16J, xr, b, a.x);
+          load(&map_y, YK, st + kX16Part, st + 2 * kX16Part, jb * kX16J, yr, b, a.y);
+          if (++stage == kX16Stages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (!ok) {  // copies in flight land before the CTA leaves
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) {}
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      bool ok = true;
+      constexpr bool kXmn = XK != kX16K, kYmn = YK != kX16K;
+      const uint32_t idesc = make_idesc_f16(kTile, kTile, a.dtype == 2) | (kXmn ? 1u << 15 : 0u) | (kYmn ? 1u << 16 : 0u);
+      for (long long u = u0; u < units && ok; u += du) {
+        ok = wait(&bars->acc_empty[acc], acc_phase ^ 1u);
+        if (!ok) break;
+        tcgen05_fence_after_sync();
+        const uint32_t d = tmem + acc * 256;
+        for (int jb = 0; jb < jblocks; ++jb) {
+          ok = wait(&bars->full[stage], phase);
+          if (!ok) break;
+          tcgen05_fence_after_sync();
+          const uint32_t st = smem_u32(smem + stage * S::kStageBytes);
+          const uint64_t xd = x16_desc(st, kXmn), yd = x16_desc(st + kX16Part, kYmn);
+#pragma unroll
+          for (int q = 0; q < kX16J / 16; ++q) {
+            const uint64_t xs = xd + q * ((kXmn ? 2048 : 32) >> 4), ys = yd + q * ((kYmn ? 2048 : 32) >> 4);
+            if (PAIR) umma_f16_pair(d, xs, ys, idesc, (jb | q) != 0 ? 1u : 0u);
+            else umma_f16(d, xs, ys, idesc, (jb | q) != 0 ? 1u : 0u);
+          }
+          commit(&bars->empty[stage]);
+          if (++stage == kX16Stages) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        commit(&bars->acc_full[acc]);
+        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      }
+    }
+  } else if (S::kMx && warp < S::kEpiWarp) {
+    uint32_t stage = 0, phase = 0;
+    bool ok = true;
+    const int tid = static_cast<int>(threadIdx.x) - 64;
+    for (long long u = u0; u < units && ok; u += du)
+      for (int jb = 0; jb < jblocks; ++jb) {
+        ok = mbar_wait(&bars->raw[stage], phase, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        uint8_t* st = smem + stage * S::kStageBytes;
+        uint8_t* dst = st + (XK >= kX16Mx4 ? 0 : kX16Part);
+        if (a.dtype == 2) x16_expand<S::kBits, true>(st + 2 * kX16Part, dst, jb * kX16J, a.J, tid);
+        else x16_expand<S::kBits, false>(st + 2 * kX16Part, dst, jb * kX16J, a.J, tid);
+        fence_proxy_async_smem();
+        arrive_leader(&bars->full[stage]);
+        if (++stage == kX16Stages) { stage = 0; phase ^= 1u; }
+      }
+  } else {
+    const uint32_t quarter = warp & 3u;
+    uint8_t* stage_mem = epi + (warp - S::kEpiWarp) * 4096;
+    uint32_t acc = 0, acc_phase = 0;
+    bool ok = true;
+    for (long long u = u0; u < units && ok; u += du) {
+      int b, xt, yt;
+      x16_decode(u, a.x_tiles, a.y_tiles, b, xt, yt);
+      ok = wait(&bars->acc_full[acc], acc_phase);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tcgen05_fence_after_sync();
+      const uint32_t t = tmem + acc * 256 + ((quarter * 32u) << 16);
+      const int x0 = xt * kTile + static_cast<int>(rank) * 128 + static_cast<int>(quarter) * 32;
+#pragma unroll 1
+      for (int c = 0; c < kTile; c += 32) {
+        const int y0 = yt * kTile + c;
+        if (y0 >= a.y.rows || x0 >= a.x.rows) break;  // warp-uniform
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(t + c, v);
+        tmem_ld_wait();
+        mx_store_rows(stage_mem, v, a.C, b * a.stride_c + static_cast<long long>(x0) * a.ldc + y0, a.ldc, a.dtype,
+                      a.x.rows - x0, min(32, a.y.rows - y0), a.vec_ok != 0);
+      }
+      tcgen05_fence_before_sync();
+      arrive_leader(&bars->acc_empty[acc]);
+      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+    }
+  }
+  tcgen05_fence_before_sync();
+  if (PAIR) cluster_sync_all(); else __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag != 0) atomicOr(&g_mx_status[0], 1u);
+  if (warp == 1) {
+    tcgen05_fence_after_sync();
+    if (PAIR) tmem_dealloc_pair(tmem, 512); else tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace fbmm

@@ -10,10 +10,11 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .bmm import BMMCUDA
-from .custom_kernel import FBMM_BF16, FBMM_F16, FBMM_F32, CustomKernel, check
+from .custom_kernel import FBMM_BF16, FBMM_F16, FBMM_F32, CustomKernel, check, load_library
 
 _DTYPES = {torch.float32: FBMM_F32, torch.float16: FBMM_F16, torch.bfloat16: FBMM_BF16}
 _X16 = (torch.float16, torch.bfloat16)
+_N, _T = ord("n"), ord("t")
 BLOCK = 32
 
 
@@ -24,6 +25,45 @@ def _code(dtype: torch.dtype) -> int:
     return code
 
 
+def _call(name: str, device: torch.device, *args) -> None:
+    """One library call on the stream that is current on `device`; the device is only switched when
+    it is not the current one (the switch costs more than the call)."""
+    fn = getattr(load_library(), name)
+    if torch.cuda.current_device() == device.index:
+        check(fn(torch.cuda.current_stream(device).cuda_stream, *args))
+    else:
+        with torch.cuda.device(device):
+            check(fn(torch.cuda.current_stream(device).cuda_stream, *args))
+
+
+def _dense_layout(X: torch.Tensor):
+    """(tensor, layout letter, pitch, batch stride) of a [l, r, c] tensor whose last ('n') or middle
+    ('t') axis is contiguous; any other order is copied."""
+    l, r, c = X.shape
+    sl, sr, sc = X.stride()
+    if (sc == 1 or c == 1) and (sr >= c or r == 1):
+        return X, _N, max(sr, c), sl
+    if (sr == 1 or r == 1) and (sc >= r or c == 1):
+        return X, _T, max(sc, r), sl
+    return X.contiguous(), _N, c, r * c
+
+
+def _aligned_layout(X: torch.Tensor):
+    """The same for the 16-bit products, whose copies need 16-byte aligned bases, pitches and batch
+    strides: other storage is copied to rows padded to 8 elements."""
+    X, letter, ld, sl = _dense_layout(X)
+    l, r, c = X.shape
+    if X.data_ptr() % 16 == 0 and ld % 8 == 0 and (l == 1 or (sl % 8 == 0 and sl >= 0)):
+        return X, letter, ld, sl
+    if letter == _T:
+        r, c = c, r
+        X = X.transpose(1, 2)
+    cp = (c + 7) // 8 * 8
+    buf = torch.empty((l, r, cp), dtype=X.dtype, device=X.device)
+    buf[:, :, :c] = X  # the padding is behind the extents that the kernels are given, never read
+    return buf, letter, cp, r * cp
+
+
 class MXTensor:
     """A [l, r, c] (or [r, c]) matrix held as microscaled elements.
 
@@ -31,7 +71,8 @@ class MXTensor:
     [l, ceil(rows / 128), ceil(k / 128), 512] as ``include/fbmm.h`` lays them out; k is the extent
     of the axis the blocks run along, ``dim``: -1 (the matrix is [l, rows, k]) or -2 (it is
     [l, k, rows], held k-contiguous all the same). A batch stride of 0 (an expanded tensor)
-    serves every batch with one matrix. 2-D codes with 3-D scales make a 2-D matrix."""
+    serves every batch with one matrix. 2-D codes with 3-D scales make a 2-D matrix. The codes
+    behind k must be zero, as ``MXQuantizeCUDA`` leaves them."""
 
     __slots__ = ("codes", "scales", "bits", "k", "dim", "two_d")
 
@@ -55,19 +96,21 @@ class MXTensor:
         blocks = (k + BLOCK - 1) // BLOCK
         if k <= 0 or pitch != blocks * (4 * bits):
             raise ValueError(f"codes have {pitch} bytes per row, which is not what k = {k} takes at {bits} bits")
-        want = (l, (rows + 127) // 128, (blocks + 3) // 4, 512)
-        if tuple(scales.shape) != want:
-            raise ValueError(f"scales have shape {tuple(scales.shape)}, expected {want}")
-        self.codes = self._addressable(codes)
-        self.scales = self._addressable(scales)
+        groups = (rows + 127) // 128, (blocks + 3) // 4
+        if scales.shape != (l, *groups, 512):
+            raise ValueError(f"scales have shape {tuple(scales.shape)}, expected {(l, *groups, 512)}")
+        self.codes = self._addressable(codes, rows * pitch)
+        self.scales = self._addressable(scales, groups[0] * groups[1] * 512)
         self.bits, self.k, self.dim, self.two_d = bits, k, dim, two_d
 
     @staticmethod
-    def _addressable(t: torch.Tensor) -> torch.Tensor:
-        # dense within a batch, batches a multiple of 16 bytes apart (or one for all), 16-byte base
-        if t.numel() == 0:
+    def _addressable(t: torch.Tensor, per_batch: int) -> torch.Tensor:
+        """t itself where its batches are dense, lie 16 bytes apart (or are one) and start aligned."""
+        if t.is_contiguous() and t.data_ptr() % 16 == 0:
             return t
-        if t[0].is_contiguous() and t.data_ptr() % 16 == 0 and (t.shape[0] == 1 or t.stride(0) % 16 == 0):
+        step = t.stride(0)
+        if (t.numel() and t[0].is_contiguous() and t.data_ptr() % 16 == 0
+                and (t.shape[0] == 1 or step == 0 or (step >= per_batch and step % 16 == 0))):
             return t
         return t.clone(memory_format=torch.contiguous_format)
 
@@ -81,28 +124,38 @@ class MXTensor:
 
     @property
     def shape(self) -> tuple:
-        l, rows = self.codes.shape[:2]
+        l, rows, _ = self.codes.shape
         s = (rows, self.k) if self.dim == -1 else (self.k, rows)
         return s if self.two_d else (l,) + s
 
     @property
     def mT(self) -> "MXTensor":
         """The transposed matrix: the same storage with the blocks along the other axis."""
-        return self._with(-3 - self.dim)
+        return self._of(self.codes, self.scales, self.bits, self.k, -3 - self.dim, self.two_d)
 
-    def _with(self, dim: int) -> "MXTensor":
-        t = object.__new__(MXTensor)
-        t.codes, t.scales, t.bits, t.k, t.dim, t.two_d = self.codes, self.scales, self.bits, self.k, dim, self.two_d
+    @classmethod
+    def _of(cls, codes, scales, bits, k, dim, two_d) -> "MXTensor":
+        t = object.__new__(cls)
+        t.codes, t.scales, t.bits, t.k, t.dim, t.two_d = codes, scales, bits, k, dim, two_d
         return t
 
-    def _strides(self):
-        """Batch strides of codes and scales in bytes (0: one matrix for every batch)."""
-        return self.codes.stride(0), self.scales.stride(0)
+    def _arguments(self):
+        """codes, their batch stride, scales, their batch stride (bytes; 0: one matrix for all)."""
+        return self.codes.data_ptr(), self.codes.stride(0), self.scales.data_ptr(), self.scales.stride(0)
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """Element times scale, rounded once to `dtype`; with dim=-2 a transposed view of
         k-contiguous storage."""
-        return MXQuantizeCUDA(self.bits).dequantize(self, dtype)
+        code = _code(dtype)
+        l, rows, _ = self.codes.shape
+        out = torch.empty((l, rows, self.k), dtype=dtype, device=self.device)
+        if out.numel():
+            codes, sc, scales, ss = self._arguments()
+            _call("fbmm_mx_dequantize", self.device, codes, sc, scales, ss, self.bits, out.data_ptr(), code, self.k,
+                  rows * self.k, l, rows, self.k)
+        if self.dim == -2:
+            out = out.transpose(1, 2)
+        return out[0] if self.two_d else out
 
     def __repr__(self) -> str:
         return f"MXTensor(shape={self.shape}, bits={self.bits}, dim={self.dim}, device={self.device})"
@@ -141,114 +194,131 @@ class MXQuantizeCUDA(CustomKernel):
         l, rows, k = X3.shape
         if k == 0:
             raise ValueError("the axis the blocks run along is empty")
-        pitch = (k + BLOCK - 1) // BLOCK * (4 * self.bits)
-        q = object.__new__(MXTensor)
-        q.codes = torch.empty((l, rows, pitch), dtype=torch.uint8, device=X.device)
-        q.scales = torch.empty((l, (rows + 127) // 128, (k + 127) // 128, 512), dtype=torch.uint8, device=X.device)
-        q.bits, q.k, q.dim, q.two_d = self.bits, k, dim, two_d
-        if l == 0 or rows == 0:
-            return q
-        sl, sr, sk = X3.stride()
-        if sk == 1 and (sr >= k or rows == 1):
-            layout, ld = ord("n"), max(sr, k)
-        elif sr == 1 and (sk >= rows or k == 1):
-            layout, ld = ord("t"), max(sk, rows)
-        else:
-            X3 = X3.contiguous()
-            sl, layout, ld = rows * k, ord("n"), k
-        with torch.cuda.device(X.device):
-            check(self.lib.fbmm_mx_quantize(self.stream_ptr(X.device), X3.data_ptr(), dtype, layout, ld, sl, self.bits,
-                                            q.codes.data_ptr(), q.scales.data_ptr(), l, rows, k))
-        return q
-
-    def dequantize(self, q: MXTensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-        code = _code(dtype)
-        l, rows = q.codes.shape[:2]
-        out = torch.empty((l, rows, q.k), dtype=dtype, device=q.device)
-        if out.numel():
-            sc, ss = q._strides()
-            with torch.cuda.device(q.device):
-                check(self.lib.fbmm_mx_dequantize(self.stream_ptr(q.device), q.codes.data_ptr(), sc, q.scales.data_ptr(),
-                                                  ss, q.bits, out.data_ptr(), code, q.k, rows * q.k, l, rows, q.k))
-        if q.dim == -2:
-            out = out.transpose(1, 2)
-        return out[0] if q.two_d else out
+        codes = torch.empty((l, rows, (k + BLOCK - 1) // BLOCK * (4 * self.bits)), dtype=torch.uint8, device=X.device)
+        scales = torch.empty((l, (rows + 127) // 128, (k + 127) // 128, 512), dtype=torch.uint8, device=X.device)
+        if l and rows:
+            X3, layout, ld, step = _dense_layout(X3)
+            _call("fbmm_mx_quantize", X.device, X3.data_ptr(), dtype, layout, ld, step, self.bits, codes.data_ptr(),
+                  scales.data_ptr(), l, rows, k)
+        return MXTensor._of(codes, scales, self.bits, k, dim, two_d)
 
 
-def _check_product(a_shape, b_shape, a_device, b_device):
-    if len(a_shape) != len(b_shape):
+def _check_product(A, B) -> bool:
+    """Shapes and devices of a product with a microscaled operand; True for 2-D operands."""
+    a, b = A.shape, B.shape
+    if len(a) != len(b):
         raise ValueError("A and B need the same number of dimensions")
-    if len(a_shape) == 3 and a_shape[0] != b_shape[0]:
-        raise ValueError(f"batch sizes differ: {a_shape[0]} vs {b_shape[0]}")
-    if a_shape[-1] != b_shape[-2]:
-        raise ValueError(f"inner dimensions differ: A {tuple(a_shape)} B {tuple(b_shape)}")
-    if a_device != b_device:
+    if len(a) not in (2, 3):
+        raise ValueError("A and B need to be 2d or 3d")
+    if len(a) == 3 and a[0] != b[0]:
+        raise ValueError(f"batch sizes differ: {a[0]} vs {b[0]}")
+    if a[-1] != b[-2]:
+        raise ValueError(f"inner dimensions differ: A {tuple(a)} B {tuple(b)}")
+    if A.device.type != "cuda":
+        raise ValueError("A and B must be CUDA tensors")
+    if A.device != B.device:
         raise ValueError("A and B must be on the same device")
+    return len(a) == 2
+
+
+def _dense_bmm(A: torch.Tensor, B: torch.Tensor) -> torch.Tensor:
+    """16-bit [l, m, k] @ [l, k, n] in any storage order, k > 0."""
+    l, m, k = A.shape
+    n = B.shape[2]
+    C = torch.empty((l, m, n), dtype=A.dtype, device=A.device)
+    if C.numel():
+        a, la, lda, sa = _aligned_layout(A)
+        b, lb, ldb, sb = _aligned_layout(B)
+        _call("fbmm_dense_bmm_x16", A.device, a.data_ptr(), la, lda, sa, b.data_ptr(), lb, ldb, sb, _DTYPES[A.dtype],
+              C.data_ptr(), n, m * n, l, m, n, k)
+    return C
 
 
 class MXDenseBMMCUDA(CustomKernel):
-    """``MXDenseBMMCUDA()(P, Q) -> C``: fp16 / bf16 P [l, m, j] times a microscaled Q [l, j, c] whose
-    blocks run along c (``dim=-1``), C in P's type. Q's elements times their scales enter as values of
-    P's type, which is exact for bf16 and, for fp16, wherever they are fp16 values. This is the
-    product of both backward passes below: the gradient of activations through 4-bit weights, and
-    of weights from activations kept in 8 bits."""
+    """``MXDenseBMMCUDA()(A, B) -> C``: A [l, m, k] @ B [l, k, n] with one fp16 / bf16 tensor and
+    one ``MXTensor`` (4 or 8 bits) whose blocks run along its own axis of C (``dim=-2`` for A,
+    ``dim=-1`` for B); C in the tensor's type, fp32 sums. The microscaled elements times their
+    scales enter as values of that type: exact for bf16, and for fp16 wherever they are fp16
+    values. These are the products of the backward passes below: activations' gradient through
+    4-bit weights, weights' gradient from activations kept in 8 bits. No gradient flows through."""
 
-    def __call__(self, P: torch.Tensor, Q: MXTensor) -> torch.Tensor:
-        if not isinstance(Q, MXTensor):
-            raise TypeError("Q must be an MXTensor")
-        if P.dtype not in _X16:
-            raise TypeError(f"dtype {P.dtype} is not one of float16, bfloat16")
-        if P.dim() not in (2, 3):
-            raise ValueError("P needs to be 2d or 3d")
-        if P.device.type != "cuda":
-            raise ValueError("P must be a CUDA tensor")
-        _check_product(P.shape, Q.shape, P.device, Q.device)
-        if Q.dim != -1:
-            raise ValueError("Q's blocks must run along its last axis (dim=-1)")
-        return BMMCUDA()(P, Q.dequantize(P.dtype))
+    def __call__(self, A, B) -> torch.Tensor:
+        if isinstance(A, MXTensor) == isinstance(B, MXTensor):
+            raise TypeError("one of A and B must be an MXTensor, the other a tensor")
+        two_d = _check_product(A, B)
+        mx, dense = (A, B) if isinstance(A, MXTensor) else (B, A)
+        if dense.dtype not in _X16:
+            raise TypeError(f"dtype {dense.dtype} is not one of float16, bfloat16")
+        if mx.dim != (-2 if mx is A else -1):
+            raise ValueError("the blocks must run along the operand's own axis of C (dim=-2 for A, dim=-1 for B)")
+        D = dense[None] if two_d else dense
+        l, m, n = D.shape[0], A.shape[-2], B.shape[-1]
+        k = A.shape[-1]
+        C = torch.empty((l, m, n), dtype=D.dtype, device=D.device)
+        if C.numel() == 0 or k == 0:
+            C.zero_()
+        elif mx is B:
+            d, letter, ld, step = _aligned_layout(D)
+            _call("fbmm_dense_mx_bmm_x16", D.device, d.data_ptr(), letter, ld, step, _DTYPES[D.dtype], *mx._arguments(),
+                  mx.bits, C.data_ptr(), n, m * n, l, m, n, k)
+        else:
+            d, letter, ld, step = _aligned_layout(D)
+            if letter != _N:
+                d, letter, ld, step = _aligned_layout(D.contiguous())
+            _call("fbmm_mx_dense_bmm_x16", D.device, *mx._arguments(), mx.bits, d.data_ptr(), ld, step, _DTYPES[D.dtype],
+                  C.data_ptr(), n, m * n, l, m, n, k)
+        return C[0] if two_d else C
 
 
-class _MXProduct(torch.autograd.Function):
-    """C = Q4(A) @ W, differentiable in A: straight through the rounding, dA = dC @ W^T."""
+def _mx4_product(A, B: MXTensor, out_dtype: torch.dtype) -> torch.Tensor:
+    two_d = B.two_d
+    n, k = B.rows, B.k
+    if isinstance(A, MXTensor):
+        l, m, _ = A.codes.shape
+        C = torch.empty((l, m, n), dtype=out_dtype, device=B.device)
+        if C.numel():
+            _call("fbmm_mx4_bmm", B.device, *A._arguments(), *B._arguments(), C.data_ptr(), _code(out_dtype), n, m * n, l, m,
+                  n, k)
+    else:
+        A3 = A[None] if two_d else A
+        l, m, _ = A3.shape
+        C = torch.empty((l, m, n), dtype=out_dtype, device=B.device)
+        if C.numel():
+            A3, layout, ld, step = _dense_layout(A3)
+            need = load_library().fbmm_mx4_bmm_tensor_workspace_bytes(l, m, k)
+            ws = torch.empty(need, dtype=torch.uint8, device=B.device)
+            _call("fbmm_mx4_bmm_tensor", B.device, A3.data_ptr(), _DTYPES[A.dtype], layout, ld, step, *B._arguments(),
+                  C.data_ptr(), _code(out_dtype), n, m * n, l, m, n, k, ws.data_ptr(), need)
+    return C[0] if two_d else C
+
+
+class _MX4Product(torch.autograd.Function):
+    """C = Q4(A) @ B, differentiable in A: straight through the rounding, dA = dC @ B^T."""
 
     @staticmethod
-    def forward(ctx, A, W, out_dtype):
-        ctx.W, ctx.dtype = W, A.dtype
-        ctx.save_for_backward(W.codes, W.scales)
-        return _mx_product(MXQuantizeCUDA(4)(A), W, out_dtype)
+    def forward(ctx, A, B, out_dtype):
+        ctx.B, ctx.dtype = B, A.dtype
+        ctx.save_for_backward(B.codes, B.scales)
+        return _mx4_product(A, B, out_dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dC):
         ctx.saved_tensors  # raises if the weights were written to since the forward pass
-        W = ctx.W.mT
+        dC, BT = dC.to(ctx.dtype), ctx.B.mT
         if ctx.dtype in _X16:
-            return MXDenseBMMCUDA()(dC.to(ctx.dtype), W), None, None
-        return BMMCUDA()(dC.to(ctx.dtype), W.dequantize(ctx.dtype)), None, None
-
-
-def _mx_product(A: MXTensor, B: MXTensor, out_dtype: torch.dtype) -> torch.Tensor:
-    kernel = CustomKernel()
-    l, m, _ = A.codes.shape
-    n = B.rows
-    C = torch.empty((l, m, n), dtype=out_dtype, device=A.device)
-    if C.numel():
-        sa, sas = A._strides()
-        sb, sbs = B._strides()
-        with torch.cuda.device(A.device):
-            check(kernel.lib.fbmm_mx4_bmm(
-                kernel.stream_ptr(A.device), A.codes.data_ptr(), sa, A.scales.data_ptr(), sas, B.codes.data_ptr(), sb,
-                B.scales.data_ptr(), sbs, C.data_ptr(), _code(out_dtype), n, m * n, l, m, n, A.k))
-    return C[0] if A.two_d else C
+            return MXDenseBMMCUDA()(dC, BT), None, None
+        return BMMCUDA()(dC, BT.dequantize(ctx.dtype)), None, None
 
 
 class MXBMMCUDA(CustomKernel):
     """``MXBMMCUDA(out_dtype)(A, B) -> C``: A [l, m, k] times B [l, k, n], both with 4-bit elements
     (``MXTensor``, blocks along k: ``dim=-1`` for A, ``dim=-2`` for B). A may be a fp32 / fp16 /
-    bf16 tensor, which is quantised first; C then has its type unless `out_dtype` says
+    bf16 tensor, which is quantised on the way; C then has its type unless `out_dtype` says
     otherwise, and is differentiable in A (the gradient passes straight through A's rounding:
-    dA = dC @ B^T with B's values). With a microscaled A, C is fp32 unless `out_dtype` says
-    otherwise. Products and scales are exact, sums are kept in fp32, C is rounded once."""
+    dA = dC @ B^T with B's values, computed in A's type). With a microscaled A, C is fp32 unless
+    `out_dtype` says otherwise. Products and scales are exact, sums are kept in fp32, C is rounded
+    once."""
 
     def __init__(self, out_dtype: torch.dtype | None = None):
         super().__init__()
@@ -259,48 +329,49 @@ class MXBMMCUDA(CustomKernel):
     def __call__(self, A, B: MXTensor) -> torch.Tensor:
         if not isinstance(B, MXTensor):
             raise TypeError("B must be an MXTensor")
-        _check_product(A.shape, B.shape, A.device, B.device)
+        _check_product(A, B)
         if B.bits != 4 or B.dim != -2:
             raise ValueError("B must hold 4-bit elements with their blocks along k (dim=-2)")
         if isinstance(A, MXTensor):
             if A.bits != 4 or A.dim != -1:
                 raise ValueError("A must hold 4-bit elements with their blocks along k (dim=-1)")
-            return _mx_product(A, B, self.out_dtype or torch.float32)
+            return _mx4_product(A, B, self.out_dtype or torch.float32)
         _code(A.dtype)
         out_dtype = self.out_dtype or A.dtype
         if A.requires_grad and torch.is_grad_enabled():
-            return _MXProduct.apply(A, B, out_dtype)
-        return _mx_product(MXQuantizeCUDA(4)(A), B, out_dtype)
+            return _MX4Product.apply(A, B, out_dtype)
+        return _mx4_product(A, B, out_dtype)
 
 
 class _CheckpointProduct(torch.autograd.Function):
+    """Operands are 3-D with every extent positive."""
+
     @staticmethod
     def forward(ctx, A, B):
-        C = BMMCUDA()(A, B)
-        ctx.a_shape, ctx.dtype = A.shape, A.dtype
-        ctx.q = None
-        if ctx.needs_input_grad[1] and A.shape[2] != 0:
-            ctx.q = MXQuantizeCUDA(8)(A)
-        if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(B)
+        x16 = A.dtype in _X16
+        C = _dense_bmm(A, B) if x16 else BMMCUDA()(A, B)
+        need_a, need_b = ctx.needs_input_grad
+        ctx.q = MXQuantizeCUDA(8)(A) if need_b else None
+        ctx.b_transposed = B.stride(2) != 1 and B.stride(1) == 1
+        ctx.save_for_backward(B if need_a else None)
         return C
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dC):
+        need_a, need_b = ctx.needs_input_grad
+        x16 = dC.dtype in _X16
         dA = dB = None
-        l, m, k = ctx.a_shape
-        n = dC.shape[2]
-        if ctx.needs_input_grad[0]:
-            B, = ctx.saved_tensors
-            dA = BMMCUDA()(dC, B.transpose(1, 2))
-        if ctx.needs_input_grad[1]:
-            if ctx.q is None or m == 0 or n == 0 or l == 0:
-                dB = torch.zeros((l, k, n), dtype=ctx.dtype, device=dC.device)
-            elif ctx.dtype in _X16:
+        if need_a:
+            BT = ctx.saved_tensors[0].transpose(1, 2)
+            dA = _dense_bmm(dC, BT) if x16 else BMMCUDA()(dC, BT)
+        if need_b:
+            if not x16:
+                dB = BMMCUDA()(ctx.q.mT.dequantize(dC.dtype), dC)
+            elif ctx.b_transposed:  # in B's own storage order
                 dB = MXDenseBMMCUDA()(dC.transpose(1, 2), ctx.q).transpose(1, 2)
             else:
-                dB = BMMCUDA()(ctx.q.dequantize(ctx.dtype).transpose(1, 2), dC)
+                dB = MXDenseBMMCUDA()(ctx.q.mT, dC)
         return dA, dB
 
 
@@ -310,11 +381,15 @@ class CheckpointBMMCUDA(BMMCUDA):
     along k: 1.03 bytes per element) instead of their own type. C and dA = dC @ B^T are what the full
     A gives; dB = A8^T @ dC uses the kept values, each within 2^-4 of its own size or, where it is
     far below its block's largest, within half of the block's finest step. A itself is not
-    kept; B is. Differentiable once."""
+    kept; B is. Differentiable once. Without a gradient to compute it is ``BMMCUDA``."""
 
     def __call__(self, A: torch.Tensor, B: torch.Tensor) -> torch.Tensor:
         if not (torch.is_grad_enabled() and (A.requires_grad or B.requires_grad)):
             return super().__call__(A, B)
         A3, B3, two_d = self.check_inputs(A, B, (torch.float32,) + _X16)
-        C = _CheckpointProduct.apply(A3, B3)
+        l, m, k = A3.shape
+        if min(l, m, k, B3.shape[2]) == 0:
+            C = torch.bmm(A3, B3)  # nothing to compute or to keep: empty, or zeros with zero gradients
+        else:
+            C = _CheckpointProduct.apply(A3, B3)
         return C[0] if two_d else C

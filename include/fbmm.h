@@ -317,6 +317,34 @@ int fbmm_mx_dequantize(void* stream, const unsigned char* codes, long long strid
 int fbmm_mx4_bmm(void* stream, const unsigned char* a_codes, long long stride_a, const unsigned char* a_scales,
                  long long stride_as, const unsigned char* b_codes, long long stride_b, const unsigned char* b_scales,
                  long long stride_bs, void* C, int dtype, long long ldc, long long stride_c, int l, int m, int n, int k);
+/* The same product with A a dense matrix of any FBMM_* element type and layout ('n' [l][m][k] or 't'
+ * [l][k][m]), quantised on the way (fbmm_mx_quantize's rules at 4 bits). The workspace is always needed. */
+size_t fbmm_mx4_bmm_tensor_workspace_bytes(int l, int m, int k);
+int fbmm_mx4_bmm_tensor(void* stream, const void* A, int a_dtype, int a_layout, long long lda, long long stride_a,
+                        const unsigned char* b_codes, long long stride_b, const unsigned char* b_scales,
+                        long long stride_bs, void* C, int dtype, long long ldc, long long stride_c, int l, int m, int n,
+                        int k, void* workspace, size_t workspace_bytes);
+
+/* 16-bit products (dtype FBMM_F16 / FBMM_BF16, fp32 sums, C [l][m][n] in the same type) in the layouts
+ * that a training step meets, without a transposed copy of any operand. Dense operands: either
+ * layout letter, bases 16-byte aligned, pitches and batch strides (elements) multiples of 8.
+ *  - fbmm_dense_bmm_x16: A [m, k] @ B [k, n].
+ *  - fbmm_dense_mx_bmm_x16: B is microscaled, stored [k][n] with its blocks along n (what
+ *    fbmm_mx_quantize makes of rows = k, k = n).
+ *  - fbmm_mx_dense_bmm_x16: A is microscaled, stored [k][m] with its blocks along m; B stored
+ *    [k][n], n contiguous.
+ * A microscaled element enters as element * scale rounded to dtype: exact for bf16, and for fp16
+ * wherever it is an fp16 value (always, if it was quantised from fp16 at 8 bits). */
+int fbmm_dense_bmm_x16(void* stream, const void* A, int a_layout, long long lda, long long stride_a, const void* B,
+                       int b_layout, long long ldb, long long stride_b, int dtype, void* C, long long ldc,
+                       long long stride_c, int l, int m, int n, int k);
+int fbmm_dense_mx_bmm_x16(void* stream, const void* A, int a_layout, long long lda, long long stride_a, int dtype,
+                          const unsigned char* b_codes, long long stride_b, const unsigned char* b_scales,
+                          long long stride_bs, int bits, void* C, long long ldc, long long stride_c,
+                          int l, int m, int n, int k);
+int fbmm_mx_dense_bmm_x16(void* stream, const unsigned char* a_codes, long long stride_a, const unsigned char* a_scales,
+                          long long stride_as, int bits, const void* B, long long ldb, long long stride_b, int dtype,
+                          void* C, long long ldc, long long stride_c, int l, int m, int n, int k);
 
 #ifdef __cplusplus
 }

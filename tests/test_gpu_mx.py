@@ -195,7 +195,7 @@ def test_product_shared_operands(dev):
         B, _ = as_mx(260, 300, 4, 2, dev, 3, dim=-2)
         A3 = MXTensor(A.codes.expand(3, -1, -1), A.scales.expand(3, -1, -1, -1), k=300)
         Ac = MXTensor(A.codes.repeat(3, 1, 1), A.scales.repeat(3, 1, 1, 1), k=300)
-        assert A3._strides() == (0, 0)
+        assert A3.codes.stride(0) == 0
         assert torch.equal(MXBMMCUDA()(A3, B), MXBMMCUDA()(Ac, B))
         assert torch.equal(MXBMMCUDA()(B.mT, A3.mT), MXBMMCUDA()(B.mT, Ac.mT))
 
@@ -210,17 +210,47 @@ def test_product_empty(dev):
 # ---- gradients -----------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("l,m,j,c", [(1, 1, 1, 1), (1, 64, 64, 64), (2, 70, 130, 200), (1, 300, 129, 257), (3, 5, 1000, 33),
-                                     (1, 257, 640, 300)])
+                                     (1, 257, 640, 300), (2, 1000, 200, 2600)])
 @pytest.mark.parametrize("bits", [4, 8])
 def test_dense_product(dev, l, m, j, c, dtype, bits):
-    """P @ Q in both layouts of P."""
-    P = rnd((l, m, j), 3, dtype, 0.3)
+    """One microscaled operand on either side, both layouts of the other."""
+    P = rnd((l, m, j), 3, dtype, 0.3)  # a [l, m, j] tensor
     Q, q = as_mx(j, c, bits, 17, dev, l, lo=120, hi=124)
     want, mag = P.double() @ q, P.double().abs() @ q.abs()
     for X in (P.to(dev), P.transpose(1, 2).contiguous().to(dev).transpose(1, 2)):
         C = MXDenseBMMCUDA()(X, Q)
         assert C.shape == (l, m, c) and C.dtype == dtype
         assert_sum_close(C, want, mag, j, dtype)
+        D = MXDenseBMMCUDA()(Q.mT, X.transpose(1, 2))
+        assert D.shape == (l, c, m)
+        assert_sum_close(D, want.transpose(1, 2), mag.transpose(1, 2), j, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_dense_product_many_tiles(dev, dtype, bits):
+    """Enough tiles for CTA pairs (256 x 256 tiles); the plain form runs in float64 on the GPU."""
+    m, j, c = 2000, 200, 2300
+    P = rnd((1, m, j), 3, dtype, 0.3).to(dev)
+    Q, q = as_mx(j, c, bits, 17, dev, 1, lo=120, hi=124)
+    q = q.to(dev)
+    want, mag = P.double() @ q, P.double().abs() @ q.abs()
+    for X in (P, P.transpose(1, 2).contiguous().transpose(1, 2)):
+        assert_sum_close(MXDenseBMMCUDA()(X, Q), want.cpu(), mag.cpu(), j, dtype)
+        assert_sum_close(MXDenseBMMCUDA()(Q.mT, X.transpose(1, 2)), want.transpose(1, 2).cpu(), mag.transpose(1, 2).cpu(),
+                         j, dtype)
+    if bits == 8:  # the dense products of a training step, in its three layouts
+        for transposed in (False, True):
+            A = rnd((1, 2100, 2050), 5, dtype, 0.3).to(dev).requires_grad_()
+            B = rnd((1, 2050, 2310), 6, dtype, 0.3).to(dev)
+            B = (B.transpose(1, 2).contiguous().transpose(1, 2) if transposed else B).detach().requires_grad_()
+            dC = rnd((1, 2100, 2310), 7, dtype, 0.3).to(dev)
+            C = CheckpointBMMCUDA()(A, B)
+            dA, dB = torch.autograd.grad(C, (A, B), dC)
+            a, b, d = A.detach().double(), B.detach().double(), dC.double()
+            a8 = MXQuantizeCUDA(8)(A.detach()).dequantize().double()
+            for got, x, y in ((C, a, b), (dA, d, b.transpose(1, 2)), (dB, a8.transpose(1, 2), d)):
+                assert_sum_close(got.detach(), (x @ y).cpu(), (x.abs() @ y.abs()).cpu(), x.shape[2], dtype)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
@@ -237,15 +267,22 @@ def test_frozen_weights_gradient(dev, l, m, n, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("l,m,n,k", [(1, 1, 1, 1), (1, 64, 96, 128), (2, 77, 130, 33), (1, 300, 257, 200)])
+@pytest.mark.parametrize("l,m,n,k", [(1, 1, 1, 1), (1, 64, 96, 128), (2, 77, 130, 33), (1, 300, 257, 200), (1, 700, 530, 600)])
 def test_checkpoint_gradients(dev, l, m, n, k, dtype):
     A, B, dC = rnd((l, m, k), 1, dtype, 0.5), rnd((l, k, n), 2, dtype, 0.2), rnd((l, m, n), 3, dtype, 0.2)
     a8 = torch.stack([S.values(*S.quantize(x, 8), 8) for x in A])
     Ad, Bd = A.to(dev).requires_grad_(), B.to(dev).requires_grad_()
     C = CheckpointBMMCUDA()(Ad, Bd)
-    assert torch.equal(C.detach(), BMMCUDA()(A.to(dev), B.to(dev)))
     dA, dB = torch.autograd.grad(C, (Ad, Bd), dC.to(dev))
-    f = 8 if dtype == F32 else 1
+    f = 8 if dtype == F32 else 1  # the fp32 product splits each term in three
     a, b, d = A.double(), B.double(), dC.double()
+    assert_sum_close(C.detach(), a @ b, a.abs() @ b.abs(), f * k, dtype)
     assert_sum_close(dA, d @ b.transpose(1, 2), d.abs() @ b.abs().transpose(1, 2), f * n, dtype)
     assert_sum_close(dB, a8.transpose(1, 2) @ d, a8.abs().transpose(1, 2) @ d.abs(), f * m, dtype)
+    # B stored transposed (a weight [n, k] used as its own transpose)
+    Wd = B.transpose(1, 2).contiguous().to(dev).requires_grad_()
+    Ct = CheckpointBMMCUDA()(Ad, Wd.transpose(1, 2))
+    dA2, dW = torch.autograd.grad(Ct, (Ad, Wd), dC.to(dev))
+    assert_sum_close(Ct.detach(), a @ b, a.abs() @ b.abs(), f * k, dtype)
+    assert_sum_close(dA2, d @ b.transpose(1, 2), d.abs() @ b.abs().transpose(1, 2), f * n, dtype)
+    assert_sum_close(dW, d.transpose(1, 2) @ a8, d.abs().transpose(1, 2) @ a8.abs(), f * m, dtype)
