@@ -29,6 +29,7 @@ enum X16Kind { kX16K = 0, kX16MN = 1, kX16Mx4 = 2, kX16Mx8 = 3 };
 constexpr int kX16J = 64;                   // j per stage: 128 bytes of a K-major row
 constexpr int kX16Part = 128 * kX16J * 2;   // 16 KB: 128 rows of one operand
 constexpr int kX16Stages = 5;
+constexpr int kX16Expanders = 3;            // groups of four warps that expand codes, each its own stages
 constexpr int kX16Chunk = 64 * kX16J * 2;   // MN-major: 64 rows x 64 j
 
 struct X16Operand {
@@ -55,8 +56,8 @@ struct X16Shape {
   static constexpr int kRaw = kMx ? kX16J * 128 * kBits / 8 + kMxGroupBytes : 0;
   static constexpr int kStageBytes = 2 * kX16Part + (kMx ? (kRaw + 1023) / 1024 * 1024 : 0);
   static constexpr int kSmem = 1024 + kX16Stages * kStageBytes + kMxEpiBytes + 256;
-  static constexpr int kThreads = kMx ? 320 : 192;
-  static constexpr int kEpiWarp = kMx ? 6 : 2;
+  static constexpr int kEpiWarp = kMx ? 2 + 4 * kX16Expanders : 2;
+  static constexpr int kThreads = (kEpiWarp + 4) * 32;
 };
 
 struct X16Barriers {
@@ -86,49 +87,132 @@ __device__ __forceinline__ uint64_t x16_desc(uint32_t smem_addr, bool mn_major) 
          (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
 
-// A stage's raw codes -> 16-bit values in MN-major order; 128 threads, 16 codes at a time (half a
-// block, so one scale). Lanes of the second 64 rows write their two 16-byte pieces in the other order, which
-// keeps the eight lanes of a row on different banks.
+// Reports to the pair's issuing CTA that this warp's values lie in THIS CTA's shared memory, behind its
+// proxy fence, where only this CTA's tensor core reads them. So the release covers this CTA; with
+// one at cluster scope the arrival itself took about 1400 cycles beside 16 writing warps, twice the expansion
+// (8-bit gradient of weights at 4096^3: 145 us with it, 115 us without).
+__device__ __forceinline__ void mbar_arrive_values(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// 16 codes (half a block) of a row as eight packed pairs of 16-bit values, scaled by 2^(E - 127).
+//
+// The fast form moves the code's fields to where the 16-bit type has them (sign to bit 15, exponent
+// and mantissa as one piece, zero and subnormal codes included), which gives the value times a
+// power of two (bf16: 2^-120 for e4m3 and 2^-126 for e2m1; fp16: 2^-8 and 2^-14), and multiplies
+// packed pairs by the power of two that is left: four or five integer instructions and one multiplication per
+// pair, where converting through fp16 and fp32 takes one slow conversion and five more instructions
+// (dA at 8192 x 4096 x 4096: 264 us that way). It rounds once, in that multiplication. Scales whose remaining power the type
+// cannot hold as a normal number, and the NaN scale, take the general form.
 template <int BITS, bool BF16>
-__device__ __forceinline__ void x16_expand(const uint8_t* raw, uint8_t* dst, int j0, int j_end, int tid) {
-  const uint8_t* sc = raw + kX16J * 128 * BITS / 8;
+struct X16Fast {
+  static constexpr int kBias = BF16 ? (BITS == 8 ? 120 : 126) : (BITS == 8 ? -104 : -98);  // E + kBias = exponent field
+  static constexpr int kTop = BF16 ? 254 : 30;
+  __device__ static __forceinline__ bool in_range(uint32_t E) {
+    const int f = static_cast<int>(E) + kBias;
+    return f >= 1 && f <= kTop;
+  }
+  __device__ static __forceinline__ uint32_t scale(uint32_t E) {  // both halves
+    return ((E + static_cast<uint32_t>(kBias)) << (BF16 ? 7 : 10)) * 0x10001u;
+  }
+};
+template <bool BF16>
+__device__ __forceinline__ uint32_t x16_mul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <int BITS, bool BF16>
+__device__ __forceinline__ void x16_values(const uint32_t (&c)[BITS / 2], uint32_t E, bool fast, uint32_t (&w)[8]) {
+  if (fast) {
+    const uint32_t s = X16Fast<BITS, BF16>::scale(E);
+    if (BITS == 8) {
+      constexpr int kShift = BF16 ? 4 : 1;
+      constexpr uint32_t kMag = BF16 ? 0x07f007f0u : 0x3f803f80u;
 #pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    const int i = it * 128 + tid;
-    const int j = i >> 3, u = i & 7;
+      for (int q = 0; q < 8; ++q) {
+        const uint32_t t = __byte_perm(c[q >> 1], 0, (q & 1) ? 0x3424 : 0x1404);  // two codes, each in a high byte
+        w[q] = x16_mul2<BF16>(((t >> kShift) & kMag) | (t & 0x80008000u), s);
+      }
+    } else {
+      constexpr int kShift = BF16 ? 6 : 9;
+      constexpr uint32_t kMag = 7u * 0x10001u << kShift;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t y[4];  // elements i and i + 4 of the word
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t m = 4 * i <= kShift ? c[h] << (kShift - 4 * i) : c[h] >> (4 * i - kShift);
+          y[i] = x16_mul2<BF16>((m & kMag) | ((c[h] << (12 - 4 * i)) & 0x80008000u), s);
+        }
+        w[h * 4 + 0] = __byte_perm(y[0], y[1], 0x5410);
+        w[h * 4 + 1] = __byte_perm(y[2], y[3], 0x5410);
+        w[h * 4 + 2] = __byte_perm(y[0], y[1], 0x7632);
+        w[h * 4 + 3] = __byte_perm(y[2], y[3], 0x7632);
+      }
+    }
+  } else {
+    const float s = mx_scale_value(E);
     uint32_t h[8];
     if (BITS == 8) {
-      const uint4 c = *reinterpret_cast<const uint4*>(raw + j * 128 + u * 16);
-      mx_unpack8(c.x, h[0], h[1]);
-      mx_unpack8(c.y, h[2], h[3]);
-      mx_unpack8(c.z, h[4], h[5]);
-      mx_unpack8(c.w, h[6], h[7]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) mx_unpack8(c[q & (BITS / 2 - 1)], h[2 * q], h[2 * q + 1]);
     } else {
-      const uint2 c = *reinterpret_cast<const uint2*>(raw + j * 64 + u * 8);
       uint32_t a[4], b[4];
-      mx_unpack4(c.x, a);
-      mx_unpack4(c.y, b);
+      mx_unpack4(c[0], a);
+      mx_unpack4(c[1], b);
 #pragma unroll
       for (int q = 0; q < 4; ++q) { h[q] = a[q]; h[q + 4] = b[q]; }
     }
-    // rows behind the last j are zero codes, but their scale bytes may be anything
-    const float s = j0 + j < j_end ? mx_scale_value(sc[mx_scale_at((j0 + j) & 127, u >> 1)]) : 0.f;
-    uint32_t w[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       const float2 f = mx_half2_floats(h[q]);
       w[q] = mx_pack_out(BF16 ? 2 : 1, f.x * s, f.y * s);
     }
-    uint8_t* row = dst + (u >> 2) * kX16Chunk + j * 128;
-    const int first = u >> 2;  // 0 or 1
-#pragma unroll
-    for (int o = 0; o < 2; ++o) {
-      const int p = o ^ first;
-      const int unit = ((u & 3) * 2 + p) ^ (j & 7);
-      *reinterpret_cast<uint4*>(row + unit * 16) =
-          p ? make_uint4(w[4], w[5], w[6], w[7]) : make_uint4(w[0], w[1], w[2], w[3]);
-    }
   }
+}
+
+// A stage's raw codes -> 16-bit values in MN-major order; 128 threads, 16 codes of a row of 128 at a time.
+// Eight neighbouring lanes take 64 codes of rows j and j ^ 5: with the 128-byte swizzle on the raw
+// 8-bit rows (4-bit rows are 64 bytes and need none) and on the values, neither their reads nor
+// their writes share a bank. Rows behind the last j are zero codes whose scale bytes may be anything.
+template <int BITS, bool BF16>
+__device__ __forceinline__ void x16_expand(const uint8_t* raw, uint8_t* dst, int j0, int j_end, int tid) {
+  const uint8_t* sc = raw + kX16J * 128 * BITS / 8;
+  const int half = (tid >> 3) & 1;             // which 64 of the row
+  const int u = half * 4 + (tid & 3);          // 16-code piece of the row
+  const int base = (tid >> 4) & 3, flip = (tid & 4) ? 5 : 0;
+  uint32_t c[4][BITS / 2], E[4];
+  bool in_range = true;
+#pragma unroll
+  for (int it = 0; it < 4; ++it) {
+    const int j = (((tid >> 6) * 4 + it) << 3) | (base ^ flip);
+    if (BITS == 8) {
+      const uint4 v = *reinterpret_cast<const uint4*>(raw + j * 128 + ((u ^ (j & 7)) << 4));
+      c[it][0] = v.x; c[it][1] = v.y; c[it][BITS / 2 - 2] = v.z; c[it][BITS / 2 - 1] = v.w;
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2*>(raw + j * 64 + u * 8);
+      c[it][0] = v.x; c[it][1] = v.y;
+    }
+    E[it] = sc[mx_scale_at((j0 + j) & 127, u >> 1)];
+    if (j0 + j >= j_end) E[it] = 127;
+    in_range = in_range && X16Fast<BITS, BF16>::in_range(E[it]);
+  }
+  const bool fast = __all_sync(0xffffffffu, in_range);
+  auto expand = [&](bool quick) {
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      const int j = (((tid >> 6) * 4 + it) << 3) | (base ^ flip);
+      uint32_t w[8];
+      x16_values<BITS, BF16>(c[it], E[it], quick, w);
+      uint8_t* row = dst + half * kX16Chunk + j * 128;
+      const int unit = ((u & 3) * 2) ^ (j & 7);
+      *reinterpret_cast<uint4*>(row + unit * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(row + (unit ^ 1) * 16) = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+  };
+  if (fast) expand(true); else expand(false);
 }
 
 // Tiles in bands of 8 along x, so that the tiles in flight share few rows of either operand.
@@ -160,7 +244,7 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   if (threadIdx.x == 0) {
     bars->abort_flag = 0;
     for (int s = 0; s < kX16Stages; ++s) {
-      mbar_init(&bars->full[s], 1 + (S::kMx ? 4 * kCtas : 0));
+      mbar_init(&bars->full[s], 1 + (S::kMx ? 4 * kCtas : 0));  // the copies, and the expanders' warps
       mbar_init(&bars->raw[s], 1);
       mbar_init(&bars->empty[s], 1);
     }
@@ -282,9 +366,16 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   } else if (S::kMx && warp < S::kEpiWarp) {
     uint32_t stage = 0, phase = 0;
     bool ok = true;
-    const int tid = static_cast<int>(threadIdx.x) - 64;
+    const int tid = static_cast<int>(threadIdx.x - 64) & 127;
+    int turn = static_cast<int>(warp - 2) >> 2;  // stages until this group's next one
     for (long long u = u0; u < units && ok; u += du)
       for (int jb = 0; jb < jblocks; ++jb) {
+        if (turn != 0) {
+          --turn;
+          if (++stage == kX16Stages) { stage = 0; phase ^= 1u; }
+          continue;
+        }
+        turn = kX16Expanders - 1;
         ok = mbar_wait(&bars->raw[stage], phase, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -293,7 +384,8 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         if (a.dtype == 2) x16_expand<S::kBits, true>(st + 2 * kX16Part, dst, jb * kX16J, a.J, tid);
         else x16_expand<S::kBits, false>(st + 2 * kX16Part, dst, jb * kX16J, a.J, tid);
         fence_proxy_async_smem();
-        arrive_leader(&bars->full[stage]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive_values(bars0 + off(&bars->full[stage]));
         if (++stage == kX16Stages) { stage = 0; phase ^= 1u; }
       }
   } else {
