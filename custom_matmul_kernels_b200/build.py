@@ -22,6 +22,7 @@ UNITS = {
                                         os.path.join(CSRC, "fbmm_l1_kernel.cuh")] + _SHARED,
     os.path.join(CSRC, "fbmm_mx_api.cu"): [os.path.join(CSRC, "fbmm_mx_quant.cuh"),
                                            os.path.join(CSRC, "fbmm_mx_gemm.cuh"),
+                                           os.path.join(CSRC, "fbmm_mx_pair.cuh"),
                                            os.path.join(CSRC, "fbmm_x16_gemm.cuh")] + _SHARED,
 }
 SOURCES = list(UNITS)

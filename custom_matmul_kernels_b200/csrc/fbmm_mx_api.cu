@@ -6,6 +6,7 @@
 #include "fbmm_host.h"
 #include "fbmm_mx_gemm.cuh"
 #include "fbmm_mx_quant.cuh"
+#include "fbmm_mx_pair.cuh"
 #include "fbmm_x16_gemm.cuh"
 
 namespace {
@@ -98,6 +99,40 @@ int launch_mx_gemm(cudaStream_t stream, int sms, const MxSide& p, const MxSide& 
   using S = MxShape<BN, SWAP>;
   FBMM_HOST_CUDA(cudaFuncSetAttribute(mx_gemm_kernel<BN, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
   mx_gemm_kernel<BN, SWAP><<<static_cast<unsigned>(std::min<long long>(units, sms)), kMxThreads, S::kSmem, stream>>>(mp, mq, a);
+  FBMM_HOST_CUDA(cudaGetLastError());
+  return FBMM_OK;
+}
+
+// Tensor map over scales [l][row groups][k groups][512]: boxes of two k groups x row_groups.
+int scales_map(CUtensorMap* map, const unsigned char* scales, long long stride, int l, int rows, int k, int row_groups) {
+  const cuuint64_t pitch = static_cast<cuuint64_t>((k + kMxGroupK - 1) / kMxGroupK) * kMxGroupBytes;
+  const cuuint64_t groups = static_cast<cuuint64_t>((rows + kMxGroupRows - 1) / kMxGroupRows);
+  const bool one = l == 1 || stride == 0;
+  const cuuint64_t dims[3] = {pitch / 4, groups, one ? 1u : static_cast<cuuint64_t>(l)};
+  const cuuint64_t strides[2] = {pitch, one ? pitch * groups : static_cast<cuuint64_t>(stride)};
+  const cuuint32_t box[3] = {kMxScaleStage / 4, static_cast<cuuint32_t>(row_groups), 1};
+  return fbmm_host::tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, scales, dims, strides, box, false);
+}
+
+int launch_mx_pair(cudaStream_t stream, int sms, const MxSide& A, const MxSide& B, const MxGemmArgs& g) {
+  CUtensorMap ma, mb, msa, msb;
+  int rc;
+  if ((rc = codes_map(&ma, A.codes, A.stride, g.l, A.rows, g.k, 128)) != FBMM_OK) return rc;
+  if ((rc = codes_map(&mb, B.codes, B.stride, g.l, B.rows, g.k, 128)) != FBMM_OK) return rc;
+  if ((rc = scales_map(&msa, A.scales, A.scale_stride, g.l, A.rows, g.k, 1)) != FBMM_OK) return rc;
+  if ((rc = scales_map(&msb, B.scales, B.scale_stride, g.l, B.rows, g.k, 2)) != FBMM_OK) return rc;
+  MxPairArgs a{};
+  a.C = g.C; a.ldc = g.ldc; a.stride_c = g.stride_c;
+  a.l = g.l; a.m = A.rows; a.n = B.rows; a.k = g.k;
+  a.a_shared = A.stride == 0; a.b_shared = B.stride == 0;
+  a.as_shared = A.scale_stride == 0; a.bs_shared = B.scale_stride == 0;
+  a.out_type = g.out_type; a.vec_ok = g.vec_ok;
+  a.m_tiles = (a.m + 255) / 256;
+  a.n_tiles = (a.n + 255) / 256;
+  const long long units = static_cast<long long>(a.m_tiles) * a.n_tiles * a.l;
+  FBMM_HOST_CUDA(cudaFuncSetAttribute(mx_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMxPairSmem));
+  mx_gemm_pair_kernel<<<static_cast<unsigned>(2 * std::min<long long>(units, sms / 2)), kMxPairThreads, kMxPairSmem, stream>>>(
+      ma, mb, msa, msb, a);
   FBMM_HOST_CUDA(cudaGetLastError());
   return FBMM_OK;
 }
@@ -332,6 +367,10 @@ int fbmm_mx4_bmm(void* stream_, const unsigned char* a_codes, long long stride_a
   const MxSide A{a_codes, stride_a, a_scales, stride_as, m}, B{b_codes, stride_b, b_scales, stride_bs, n};
   if (m <= 16) return launch_mx_gemm<16, true>(stream, sms, B, A, a);
   if (m <= 64) return launch_mx_gemm<64, true>(stream, sms, B, A, a);
+  const long long pairs = static_cast<long long>((m + 255) / 256) * ((n + 255) / 256) * l;
+  const long long singles = static_cast<long long>((m + 127) / 128) * ((n + 127) / 128) * l;
+  const long long pair_waves = (pairs + sms / 2 - 1) / (sms / 2), single_waves = (singles + sms - 1) / sms;
+  if (5 * pair_waves <= 4 * single_waves) return launch_mx_pair(stream, sms, A, B, a);
   return launch_mx_gemm<128, false>(stream, sms, A, B, a);
 }
 

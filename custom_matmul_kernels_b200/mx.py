@@ -25,15 +25,25 @@ def _code(dtype: torch.dtype) -> int:
     return code
 
 
+try:  # the stream's handle without a Stream object around it (2 us less per call)
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
+
 def _call(name: str, device: torch.device, *args) -> None:
     """One library call on the stream that is current on `device`; the device is only switched when
     it is not the current one (the switch costs more than the call)."""
     fn = getattr(load_library(), name)
-    if torch.cuda.current_device() == device.index:
-        check(fn(torch.cuda.current_stream(device).cuda_stream, *args))
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(_raw_stream(index), *args)
     else:
         with torch.cuda.device(device):
-            check(fn(torch.cuda.current_stream(device).cuda_stream, *args))
+            rc = fn(_raw_stream(index), *args)
+    if rc:
+        check(rc)
 
 
 def _dense_layout(X: torch.Tensor):
@@ -148,8 +158,8 @@ class MXTensor:
         k-contiguous storage."""
         code = _code(dtype)
         l, rows, _ = self.codes.shape
-        out = torch.empty((l, rows, self.k), dtype=dtype, device=self.device)
-        if out.numel():
+        out = self.codes.new_empty((l, rows, self.k), dtype=dtype)
+        if l and rows:
             codes, sc, scales, ss = self._arguments()
             _call("fbmm_mx_dequantize", self.device, codes, sc, scales, ss, self.bits, out.data_ptr(), code, self.k,
                   rows * self.k, l, rows, self.k)
@@ -194,8 +204,8 @@ class MXQuantizeCUDA(CustomKernel):
         l, rows, k = X3.shape
         if k == 0:
             raise ValueError("the axis the blocks run along is empty")
-        codes = torch.empty((l, rows, (k + BLOCK - 1) // BLOCK * (4 * self.bits)), dtype=torch.uint8, device=X.device)
-        scales = torch.empty((l, (rows + 127) // 128, (k + 127) // 128, 512), dtype=torch.uint8, device=X.device)
+        codes = X.new_empty((l, rows, (k + BLOCK - 1) // BLOCK * (4 * self.bits)), dtype=torch.uint8)
+        scales = X.new_empty((l, (rows + 127) // 128, (k + 127) // 128, 512), dtype=torch.uint8)
         if l and rows:
             X3, layout, ld, step = _dense_layout(X3)
             _call("fbmm_mx_quantize", X.device, X3.data_ptr(), dtype, layout, ld, step, self.bits, codes.data_ptr(),
@@ -225,8 +235,8 @@ def _dense_bmm(A: torch.Tensor, B: torch.Tensor) -> torch.Tensor:
     """16-bit [l, m, k] @ [l, k, n] in any storage order, k > 0."""
     l, m, k = A.shape
     n = B.shape[2]
-    C = torch.empty((l, m, n), dtype=A.dtype, device=A.device)
-    if C.numel():
+    C = A.new_empty((l, m, n))
+    if l and m and n:
         a, la, lda, sa = _aligned_layout(A)
         b, lb, ldb, sb = _aligned_layout(B)
         _call("fbmm_dense_bmm_x16", A.device, a.data_ptr(), la, lda, sa, b.data_ptr(), lb, ldb, sb, _DTYPES[A.dtype],
@@ -254,7 +264,7 @@ class MXDenseBMMCUDA(CustomKernel):
         D = dense[None] if two_d else dense
         l, m, n = D.shape[0], A.shape[-2], B.shape[-1]
         k = A.shape[-1]
-        C = torch.empty((l, m, n), dtype=D.dtype, device=D.device)
+        C = D.new_empty((l, m, n))
         if C.numel() == 0 or k == 0:
             C.zero_()
         elif mx is B:
@@ -275,21 +285,31 @@ def _mx4_product(A, B: MXTensor, out_dtype: torch.dtype) -> torch.Tensor:
     n, k = B.rows, B.k
     if isinstance(A, MXTensor):
         l, m, _ = A.codes.shape
-        C = torch.empty((l, m, n), dtype=out_dtype, device=B.device)
+        C = A.codes.new_empty((l, m, n), dtype=out_dtype)
         if C.numel():
             _call("fbmm_mx4_bmm", B.device, *A._arguments(), *B._arguments(), C.data_ptr(), _code(out_dtype), n, m * n, l, m,
                   n, k)
     else:
         A3 = A[None] if two_d else A
         l, m, _ = A3.shape
-        C = torch.empty((l, m, n), dtype=out_dtype, device=B.device)
+        C = A.new_empty((l, m, n), dtype=out_dtype)
         if C.numel():
             A3, layout, ld, step = _dense_layout(A3)
             need = load_library().fbmm_mx4_bmm_tensor_workspace_bytes(l, m, k)
-            ws = torch.empty(need, dtype=torch.uint8, device=B.device)
+            ws = A.new_empty(need, dtype=torch.uint8)
             _call("fbmm_mx4_bmm_tensor", B.device, A3.data_ptr(), _DTYPES[A.dtype], layout, ld, step, *B._arguments(),
                   C.data_ptr(), _code(out_dtype), n, m * n, l, m, n, k, ws.data_ptr(), need)
     return C[0] if two_d else C
+
+
+def _once(backward):
+    """A backward pass that can itself not be differentiated. The wrapper that says so to a graph
+    of higher order (10 us a call) is only entered where such a graph is being made."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, dC):
+        return guarded(ctx, dC) if torch.is_grad_enabled() else backward(ctx, dC)
+    return run
 
 
 class _MX4Product(torch.autograd.Function):
@@ -302,7 +322,7 @@ class _MX4Product(torch.autograd.Function):
         return _mx4_product(A, B, out_dtype)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dC):
         ctx.saved_tensors  # raises if the weights were written to since the forward pass
         dC, BT = dC.to(ctx.dtype), ctx.B.mT
@@ -357,7 +377,7 @@ class _CheckpointProduct(torch.autograd.Function):
         return C
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dC):
         need_a, need_b = ctx.needs_input_grad
         x16 = dC.dtype in _X16

@@ -134,6 +134,25 @@ def test_product_of_microscaled(dev, l, m, n, k, dtype):
     assert_sum_close(C, want, a.abs() @ b.abs().transpose(1, 2), k, dtype)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("l,m,n,k", [(1, 2300, 2500, 700), (2, 2048, 1536, 1280), (9, 1100, 300, 130)])
+def test_product_many_tiles(dev, l, m, n, k, dtype):
+    """Enough tiles for CTA pairs (256 x 256 tiles); the plain form runs in float64 on the GPU."""
+    A, a = as_mx(m, k, 4, 11, dev, l, lo=121, hi=125)
+    B, b = as_mx(n, k, 4, 977, dev, l, dim=-2, lo=121, hi=125)
+    a, b = a.to(dev), b.to(dev)
+    C = MXBMMCUDA(out_dtype=dtype)(A, B)
+    assert_sum_close(C, (a @ b.transpose(1, 2)).cpu(), (a.abs() @ b.abs().transpose(1, 2)).cpu(), k, dtype)
+    if l == 1:  # shared across batches, and a scale and a NaN block in every corner
+        A3 = MXTensor(A.codes.expand(2, -1, -1), A.scales.expand(2, -1, -1, -1), k=k)
+        B3 = MXTensor(B.codes.repeat(2, 1, 1), B.scales.repeat(2, 1, 1, 1), k=k, dim=-2)
+        assert torch.equal(MXBMMCUDA(out_dtype=dtype)(A3, B3), C.expand(2, -1, -1))
+        S2 = A.scales.clone()
+        S2.view(-1)[-512 + (m - 1) % 32 * 16 + (m - 1) % 128 // 32 * 4] = 255
+        C2 = MXBMMCUDA(out_dtype=dtype)(MXTensor(A.codes, S2, k=k), B)
+        assert bool(torch.isnan(C2[0, -1]).all()) and torch.equal(C2[0, :-1], C[0, :-1])
+
+
 @pytest.mark.parametrize("m", [1, 16, 40, 200])
 def test_product_exact_integers(dev, m):
     """Scales of one: every sum is a multiple of 1/4 below 2^22, so the result is exact."""
