@@ -95,84 +95,6 @@ __device__ __forceinline__ void mbar_arrive_values(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-// 16 codes (half a block) of a row as eight packed pairs of 16-bit values, scaled by 2^(E - 127).
-//
-// The fast form moves the code's fields to where the 16-bit type has them (sign to bit 15, exponent
-// and mantissa as one piece, zero and subnormal codes included), which gives the value times a
-// power of two (bf16: 2^-120 for e4m3 and 2^-126 for e2m1; fp16: 2^-8 and 2^-14), and multiplies
-// packed pairs by the power of two that is left: four or five integer instructions and one multiplication per
-// pair, where converting through fp16 and fp32 takes one slow conversion and five more instructions
-// (dA at 8192 x 4096 x 4096: 264 us that way). It rounds once, in that multiplication. Scales whose remaining power the type
-// cannot hold as a normal number, and the NaN scale, take the general form.
-template <int BITS, bool BF16>
-struct X16Fast {
-  static constexpr int kBias = BF16 ? (BITS == 8 ? 120 : 126) : (BITS == 8 ? -104 : -98);  // E + kBias = exponent field
-  static constexpr int kTop = BF16 ? 254 : 30;
-  __device__ static __forceinline__ bool in_range(uint32_t E) {
-    const int f = static_cast<int>(E) + kBias;
-    return f >= 1 && f <= kTop;
-  }
-  __device__ static __forceinline__ uint32_t scale(uint32_t E) {  // both halves
-    return ((E + static_cast<uint32_t>(kBias)) << (BF16 ? 7 : 10)) * 0x10001u;
-  }
-};
-template <bool BF16>
-__device__ __forceinline__ uint32_t x16_mul2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  if (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-template <int BITS, bool BF16>
-__device__ __forceinline__ void x16_values(const uint32_t (&c)[BITS / 2], uint32_t E, bool fast, uint32_t (&w)[8]) {
-  if (fast) {
-    const uint32_t s = X16Fast<BITS, BF16>::scale(E);
-    if (BITS == 8) {
-      constexpr int kShift = BF16 ? 4 : 1;
-      constexpr uint32_t kMag = BF16 ? 0x07f007f0u : 0x3f803f80u;
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const uint32_t t = __byte_perm(c[q >> 1], 0, (q & 1) ? 0x3424 : 0x1404);  // two codes, each in a high byte
-        w[q] = x16_mul2<BF16>(((t >> kShift) & kMag) | (t & 0x80008000u), s);
-      }
-    } else {
-      constexpr int kShift = BF16 ? 6 : 9;
-      constexpr uint32_t kMag = 7u * 0x10001u << kShift;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t y[4];  // elements i and i + 4 of the word
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t m = 4 * i <= kShift ? c[h] << (kShift - 4 * i) : c[h] >> (4 * i - kShift);
-          y[i] = x16_mul2<BF16>((m & kMag) | ((c[h] << (12 - 4 * i)) & 0x80008000u), s);
-        }
-        w[h * 4 + 0] = __byte_perm(y[0], y[1], 0x5410);
-        w[h * 4 + 1] = __byte_perm(y[2], y[3], 0x5410);
-        w[h * 4 + 2] = __byte_perm(y[0], y[1], 0x7632);
-        w[h * 4 + 3] = __byte_perm(y[2], y[3], 0x7632);
-      }
-    }
-  } else {
-    const float s = mx_scale_value(E);
-    uint32_t h[8];
-    if (BITS == 8) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) mx_unpack8(c[q & (BITS / 2 - 1)], h[2 * q], h[2 * q + 1]);
-    } else {
-      uint32_t a[4], b[4];
-      mx_unpack4(c[0], a);
-      mx_unpack4(c[1], b);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) { h[q] = a[q]; h[q + 4] = b[q]; }
-    }
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const float2 f = mx_half2_floats(h[q]);
-      w[q] = mx_pack_out(BF16 ? 2 : 1, f.x * s, f.y * s);
-    }
-  }
-}
-
 // A stage's raw codes -> 16-bit values in MN-major order; 128 threads, 16 codes of a row of 128 at a time.
 // Eight neighbouring lanes take 64 codes of rows j and j ^ 5: with the 128-byte swizzle on the raw
 // 8-bit rows (4-bit rows are 64 bytes and need none) and on the values, neither their reads nor
@@ -197,7 +119,7 @@ __device__ __forceinline__ void x16_expand(const uint8_t* raw, uint8_t* dst, int
     }
     E[it] = sc[mx_scale_at((j0 + j) & 127, u >> 1)];
     if (j0 + j >= j_end) E[it] = 127;
-    in_range = in_range && X16Fast<BITS, BF16>::in_range(E[it]);
+    in_range = in_range && MxFast<BITS, BF16>::in_range(E[it]);
   }
   const bool fast = __all_sync(0xffffffffu, in_range);
   auto expand = [&](bool quick) {
@@ -205,7 +127,7 @@ __device__ __forceinline__ void x16_expand(const uint8_t* raw, uint8_t* dst, int
     for (int it = 0; it < 4; ++it) {
       const int j = (((tid >> 6) * 4 + it) << 3) | (base ^ flip);
       uint32_t w[8];
-      x16_values<BITS, BF16>(c[it], E[it], quick, w);
+      mx_values16<BITS, BF16>(c[it], E[it], quick, w);
       uint8_t* row = dst + half * kX16Chunk + j * 128;
       const int unit = ((u & 3) * 2) ^ (j & 7);
       *reinterpret_cast<uint4*>(row + unit * 16) = make_uint4(w[0], w[1], w[2], w[3]);
