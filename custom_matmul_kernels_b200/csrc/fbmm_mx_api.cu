@@ -85,23 +85,6 @@ struct MxSide {
   int rows;
 };
 
-template <int BN, bool SWAP>
-int launch_mx_gemm(cudaStream_t stream, int sms, const MxSide& p, const MxSide& q, MxGemmArgs a) {
-  CUtensorMap mp, mq;
-  int rc;
-  if ((rc = codes_map(&mp, p.codes, p.stride, a.l, p.rows, a.k, kMxM)) != FBMM_OK) return rc;
-  if ((rc = codes_map(&mq, q.codes, q.stride, a.l, q.rows, a.k, BN)) != FBMM_OK) return rc;
-  a.p = MxOperand{p.scales, a.l > 1 ? p.scale_stride : 0, p.rows, a.l > 1 && p.stride == 0};
-  a.q = MxOperand{q.scales, a.l > 1 ? q.scale_stride : 0, q.rows, a.l > 1 && q.stride == 0};
-  a.p_tiles = (p.rows + kMxM - 1) / kMxM;
-  a.q_tiles = (q.rows + BN - 1) / BN;
-  const long long units = static_cast<long long>(a.p_tiles) * a.q_tiles * a.l;
-  using S = MxShape<BN, SWAP>;
-  FBMM_HOST_CUDA(cudaFuncSetAttribute(mx_gemm_kernel<BN, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-  mx_gemm_kernel<BN, SWAP><<<static_cast<unsigned>(std::min<long long>(units, sms)), kMxThreads, S::kSmem, stream>>>(mp, mq, a);
-  FBMM_HOST_CUDA(cudaGetLastError());
-  return FBMM_OK;
-}
 
 // Tensor map over scales [l][row groups][k groups][512]: boxes of two k groups x row_groups.
 int scales_map(CUtensorMap* map, const unsigned char* scales, long long stride, int l, int rows, int k, int row_groups) {
@@ -112,6 +95,27 @@ int scales_map(CUtensorMap* map, const unsigned char* scales, long long stride, 
   const cuuint64_t strides[2] = {pitch, one ? pitch * groups : static_cast<cuuint64_t>(stride)};
   const cuuint32_t box[3] = {kMxScaleStage / 4, static_cast<cuuint32_t>(row_groups), 1};
   return fbmm_host::tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, scales, dims, strides, box, false);
+}
+
+template <int BN, bool SWAP>
+int launch_mx_gemm(cudaStream_t stream, int sms, const MxSide& p, const MxSide& q, MxGemmArgs a) {
+  CUtensorMap mp, mq, msp, msq;
+  int rc;
+  if ((rc = codes_map(&mp, p.codes, p.stride, a.l, p.rows, a.k, kMxM)) != FBMM_OK) return rc;
+  if ((rc = codes_map(&mq, q.codes, q.stride, a.l, q.rows, a.k, BN)) != FBMM_OK) return rc;
+  if ((rc = scales_map(&msp, p.scales, p.scale_stride, a.l, p.rows, a.k, 1)) != FBMM_OK) return rc;
+  if ((rc = scales_map(&msq, q.scales, q.scale_stride, a.l, q.rows, a.k, 1)) != FBMM_OK) return rc;
+  a.p_rows = p.rows; a.q_rows = q.rows;
+  a.p_shared = p.stride == 0; a.q_shared = q.stride == 0;
+  a.sp_shared = p.scale_stride == 0; a.sq_shared = q.scale_stride == 0;
+  a.p_tiles = (p.rows + kMxM - 1) / kMxM;
+  a.q_tiles = (q.rows + BN - 1) / BN;
+  const long long units = static_cast<long long>(a.p_tiles) * a.q_tiles * a.l;
+  using S = MxShape<BN>;
+  FBMM_HOST_CUDA(cudaFuncSetAttribute(mx_gemm_kernel<BN, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  mx_gemm_kernel<BN, SWAP><<<static_cast<unsigned>(std::min<long long>(units, sms)), kMxThreads, S::kSmem, stream>>>(mp, mq, msp, msq, a);
+  FBMM_HOST_CUDA(cudaGetLastError());
+  return FBMM_OK;
 }
 
 int launch_mx_pair(cudaStream_t stream, int sms, const MxSide& A, const MxSide& B, const MxGemmArgs& g) {

@@ -7,12 +7,11 @@
 // two 512-byte groups of scales per 128 rows, which tcgen05.cp moves from shared to tensor memory
 // in the order they are stored in (fbmm_mx_quant.cuh). The tensor-memory columns of the scales
 // belong to the ring stage, so they are rewritten only after the commit that frees the stage.
-// Elements behind k are zero by the tensor maps' fill, but a group of scales behind the last one
-// does not exist and holds whatever the stage held before (255 would be NaN): the MMAs of such
-// groups are not issued.
+// Elements behind k and groups of scales that do not exist are zero by the tensor maps' fill: they add
+// nothing (a zero scale byte is 2^-127).
 //
-// Roles of a CTA: warp 0 (one lane) issues the copies, warp 1 (one lane) the scale copies and MMAs,
-// warps 2-5 move accumulators to global memory. Persistent, one CTA per SM.
+// Roles of a CTA: warp 0 issues the copies, warp 1 the scale copies and MMAs, warps 2-5 move
+// accumulators to global memory. Two accumulator stages, persistent, one CTA per SM.
 #pragma once
 #include "fbmm_mx_quant.cuh"
 #include "sm100_primitives.cuh"
@@ -30,38 +29,27 @@ constexpr int kMxMaxStages = 8;
 constexpr int kMxThreads = 192;
 constexpr int kMxEpiBytes = 4 * 4096;  // staging, 4 KB per epilogue warp
 
-// One operand seen as rows x k.
-struct MxOperand {
-  const uint8_t* scales;
-  long long scale_stride;  // bytes between batches, 0 = shared
-  int rows;
-  int shared;              // codes are one matrix for every batch
-};
-
+// p supplies the 128-row operand of the MMA, q the other one.
 struct MxGemmArgs {
-  MxOperand p, q;  // p supplies the 128-row operand of the MMA, q the other one
   void* C;
   long long ldc, stride_c;  // elements
-  int l, k;
+  int l, k, p_rows, q_rows;
+  int p_shared, q_shared, sp_shared, sq_shared;  // one matrix of codes / scales for every batch
   int out_type;  // 0 fp32, 1 fp16, 2 bf16
   int p_tiles, q_tiles;
   int vec_ok;    // C's rows are 16-byte aligned
 };
 
-template <int BN, bool SWAP>
+template <int BN>
 struct MxShape {
-  static constexpr int kQGroups = (BN + 127) / 128;
   static constexpr int kPBytes = kMxM * kMxRowBytes, kQBytes = BN * kMxRowBytes;
-  static constexpr int kSfCols = 8 + 8 * kQGroups;  // tensor-memory columns of a stage's scales
-  static constexpr int kStageBytes = kPBytes + kQBytes + kMxScaleStage * (1 + kQGroups);
-  static constexpr int kAccStages = BN > 128 ? 1 : 2;
-  static constexpr int kSfBase = BN * kAccStages;
-  static constexpr int kStagesFit = static_cast<int>((kMxSmemLimit - 1024 - 256 - kMxEpiBytes) / kStageBytes);
-  static constexpr int kStagesTmem = (512 - kSfBase) / kSfCols;
-  static constexpr int kStages0 = kStagesFit < kStagesTmem ? kStagesFit : kStagesTmem;
-  static constexpr int kStages = kStages0 < kMxMaxStages ? kStages0 : kMxMaxStages;
+  static constexpr int kSfCols = 16;  // tensor-memory columns of a stage's scales
+  static constexpr int kStageBytes = kPBytes + kQBytes + 2 * kMxScaleStage;
+  static constexpr int kSfBase = 2 * BN;
+  static constexpr int kFit = static_cast<int>((kMxSmemLimit - 1024 - 256 - kMxEpiBytes) / kStageBytes);
+  static constexpr int kStages = kFit < kMxMaxStages ? kFit : kMxMaxStages;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kMxEpiBytes + 256;
-  static constexpr uint32_t kTmemCols = 512;
+  static_assert(BN <= 128 && kSfBase + kStages * kSfCols <= 512, "tensor memory");
 };
 
 struct MxBarriers {
@@ -101,13 +89,22 @@ __device__ __forceinline__ void mx_umma(uint32_t d_tmem, uint64_t a_desc, uint64
 __device__ __forceinline__ void mx_copy_scales(uint32_t tmem, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
-// Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) into shared memory.
-__device__ __forceinline__ void mx_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
+// One lane of the (converged) warp, always the same one. The loops that issue copies and MMAs run on the whole
+// warp, so that descriptors and addresses stay in uniform registers, and only the issuing instructions are
+// under this predicate: with the loop itself on one lane every tcgen05 instruction took about 100
+// cycles to issue (its operands moved to uniform registers one by one), which bound all three kernels.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n"
+      ".reg .pred P;\n"
+      "elect.sync _|P, 0xffffffff;\n"
+      "selp.u32 %0, 1, 0, P;\n"
+      "}\n"
+      : "=r"(p));
+  return p != 0;
 }
+__device__ __forceinline__ uint32_t warp_index() { return __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0); }
 
 __device__ __forceinline__ uint32_t mx_pack_out(int out_type, float a, float b) {
   if (out_type == 2) {
@@ -184,14 +181,15 @@ __device__ __forceinline__ void mx_store_rows(uint8_t* stage, const uint32_t (&v
 // of A: the weights fill the 128-row side of the MMA), lanes are columns of C.
 template <int BN, bool SWAP>
 __global__ void __launch_bounds__(kMxThreads, 1)
-mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const MxGemmArgs a) {
-  using S = MxShape<BN, SWAP>;
+mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+               const __grid_constant__ CUtensorMap map_sp, const __grid_constant__ CUtensorMap map_sq, const MxGemmArgs a) {
+  using S = MxShape<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* epi = smem + S::kStages * S::kStageBytes;
   MxBarriers* bars = reinterpret_cast<MxBarriers*>(epi + kMxEpiBytes);
   volatile uint32_t* abort_flag = &bars->abort_flag;
-  const uint32_t warp = threadIdx.x >> 5, lane = lane_id();
+  const uint32_t warp = warp_index(), lane = lane_id();
   if (threadIdx.x == 0) {
     bars->abort_flag = 0;
     for (int s = 0; s < S::kStages; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
@@ -199,9 +197,11 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant_
     fence_barrier_init();
     tma_prefetch_desc(&map_p);
     tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_sp);
+    tma_prefetch_desc(&map_sq);
   }
   if (warp == 1) {
-    tmem_alloc(&bars->tmem_base, S::kTmemCols);
+    tmem_alloc(&bars->tmem_base, 512);
     tmem_relinquish_alloc_permit();
   }
   tcgen05_fence_before_sync();
@@ -210,7 +210,6 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant_
   const uint32_t tmem = bars->tmem_base;
 
   const int kblocks = (a.k + kMxStageK - 1) / kMxStageK;
-  const int kgroups = (a.k + kMxGroupK - 1) / kMxGroupK;
   const long long per_batch = static_cast<long long>(a.p_tiles) * a.q_tiles;
   const long long units = per_batch * a.l;
   auto decode = [&](long long u, int& b, int& pt, int& qt) {
@@ -221,80 +220,64 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant_
   };
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t stage = 0, phase = 0;
-      bool ok = true;
-      for (long long u = blockIdx.x; u < units && ok; u += gridDim.x) {
-        int b, pt, qt;
-        decode(u, b, pt, qt);
-        const uint8_t* sp = a.p.scales + b * a.p.scale_stride + static_cast<long long>(pt) * kgroups * kMxGroupBytes;
-        const int q_group = qt * BN / 128;  // first group of 128 rows of the q tile
-        const int q_groups = min(S::kQGroups, (a.q.rows + 127) / 128 - q_group);
-        const uint8_t* sq = a.q.scales + b * a.q.scale_stride + static_cast<long long>(q_group) * kgroups * kMxGroupBytes;
-        for (int kb = 0; kb < kblocks; ++kb) {
-          ok = mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag);
-          if (!ok) break;
-          uint8_t* st = smem + stage * S::kStageBytes;
-          uint8_t* sf = st + S::kPBytes + S::kQBytes;
-          const uint32_t sf_bytes = static_cast<uint32_t>(min(2, kgroups - 2 * kb)) * kMxGroupBytes;
-          mbar_arrive_expect_tx(&bars->full[stage],
-                                S::kPBytes + S::kQBytes + sf_bytes * static_cast<uint32_t>(1 + q_groups));
-          tma_load_3d(st, &map_p, &bars->full[stage], kb * kMxRowBytes, pt * kMxM, a.p.shared ? 0 : b,
-                      SWAP ? kL2EvictFirst : kL2EvictLast);
-          tma_load_3d(st + S::kPBytes, &map_q, &bars->full[stage], kb * kMxRowBytes, qt * BN, a.q.shared ? 0 : b,
+    uint32_t stage = 0, phase = 0;
+    bool ok = true;
+    for (long long u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      int b, pt, qt;
+      decode(u, b, pt, qt);
+      for (int kb = 0; kb < kblocks; ++kb) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag));
+        if (!ok) break;
+        uint8_t* st = smem + stage * S::kStageBytes;
+        uint8_t* sf = st + S::kPBytes + S::kQBytes;
+        uint64_t* full = &bars->full[stage];
+        if (elect_one()) {
+          mbar_arrive_expect_tx(full, S::kStageBytes);
+          tma_load_3d(st, &map_p, full, kb * kMxRowBytes, pt * kMxM, a.p_shared ? 0 : b, kL2EvictLast);
+          tma_load_3d(st + S::kPBytes, &map_q, full, kb * kMxRowBytes, qt * BN, a.q_shared ? 0 : b, kL2EvictLast);
+          tma_load_3d(sf, &map_sp, full, kb * (kMxScaleStage / 4), pt, a.sp_shared ? 0 : b, kL2EvictLast);
+          tma_load_3d(sf + kMxScaleStage, &map_sq, full, kb * (kMxScaleStage / 4), qt * BN / 128, a.sq_shared ? 0 : b,
                       kL2EvictLast);
-          mx_bulk_load(sf, sp + static_cast<long long>(kb) * kMxScaleStage, sf_bytes, &bars->full[stage]);
-          for (int g = 0; g < q_groups; ++g)
-            mx_bulk_load(sf + kMxScaleStage * (1 + g),
-                         sq + (static_cast<long long>(g) * kgroups + 2 * kb) * kMxGroupBytes, sf_bytes, &bars->full[stage]);
-          if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
         }
-      }
-      if (!ok) {  // copies in flight land before the CTA leaves
-        const long long t0 = clock64();
-        while (clock64() - t0 < 2000000LL) {}
+        __syncwarp();
+        if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
       }
     }
+    if (!ok) {  // copies in flight land before the CTA leaves
+      const long long t0 = clock64();
+      while (clock64() - t0 < 2000000LL) {}
+    }
   } else if (warp == 1) {
-    if (lane == 0) {
-      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
-      bool ok = true;
-      for (long long u = blockIdx.x; u < units && ok; u += gridDim.x) {
-        ok = mbar_wait(&bars->acc_empty[acc], acc_phase ^ 1u, abort_flag);
+    uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+    bool ok = true;
+    for (long long u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->acc_empty[acc], acc_phase ^ 1u, abort_flag));
+      if (!ok) break;
+      const uint32_t d = tmem + acc * BN;
+      for (int kb = 0; kb < kblocks; ++kb) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->full[stage], phase, abort_flag));
         if (!ok) break;
         tcgen05_fence_after_sync();
-        const uint32_t d = tmem + acc * BN;
-        for (int kb = 0; kb < kblocks; ++kb) {
-          ok = mbar_wait(&bars->full[stage], phase, abort_flag);
-          if (!ok) break;
-          tcgen05_fence_after_sync();
-          const uint32_t st = smem_u32(smem + stage * S::kStageBytes);
-          const uint32_t sf = st + S::kPBytes + S::kQBytes;
-          const uint32_t t_sf = tmem + S::kSfBase + stage * S::kSfCols;
-          const int groups = min(2, kgroups - 2 * kb);
-          // columns of a stage: p's two groups, then for each group of k all of q's rows side by side
-          for (int g = 0; g < groups; ++g) {
-            mx_copy_scales(t_sf + g * 4, mx_desc_scales(sf + g * kMxGroupBytes));
+        const uint32_t st = smem_u32(smem + stage * S::kStageBytes);
+        const uint32_t sf = st + S::kPBytes + S::kQBytes;
+        const uint32_t t_sf = tmem + S::kSfBase + stage * S::kSfCols;  // per group of k: 4 columns of p, then q's
+        const uint64_t pd = mx_desc_codes(st), qd = mx_desc_codes(st + S::kPBytes);
+        if (elect_one()) {
 #pragma unroll
-            for (int r = 0; r < S::kQGroups; ++r)
-              mx_copy_scales(t_sf + 8 + g * 4 * S::kQGroups + r * 4,
-                             mx_desc_scales(sf + kMxScaleStage * (1 + r) + g * kMxGroupBytes));
-          }
-          const uint64_t pd = mx_desc_codes(st), qd = mx_desc_codes(st + S::kPBytes);
-          for (int g = 0; g < groups; ++g)
+          for (int g = 0; g < 2; ++g)
+            mx_copy_scales(t_sf + g * 8, mx_desc_scales(sf + g * kMxGroupBytes)),
+            mx_copy_scales(t_sf + g * 8 + 4, mx_desc_scales(sf + kMxScaleStage + g * kMxGroupBytes));
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint32_t step = static_cast<uint32_t>(g * 2 + j) * 2;  // 32 bytes of codes, in units of 16
-              mx_umma(d, pd + step, qd + step, mx_idesc(kMxM, BN, j * 2), t_sf + g * 4, t_sf + 8 + g * 4 * S::kQGroups,
-                      (kb | g | j) != 0 ? 1u : 0u);
-            }
+          for (int q = 0; q < 4; ++q)
+            mx_umma(d, pd + q * 2, qd + q * 2, mx_idesc(kMxM, BN, (q & 1) * 2), t_sf + (q >> 1) * 8, t_sf + (q >> 1) * 8 + 4,
+                    (kb | q) != 0 ? 1u : 0u);
           umma_commit(&bars->empty[stage]);
-          if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
+          if (kb == kblocks - 1) umma_commit(&bars->acc_full[acc]);
         }
-        if (!ok) break;
-        umma_commit(&bars->acc_full[acc]);
-        if (++acc == S::kAccStages) { acc = 0; acc_phase ^= 1u; }
+        __syncwarp();
+        if (++stage == S::kStages) { stage = 0; phase ^= 1u; }
       }
+      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
   } else {
     const uint32_t quarter = warp & 3u;
@@ -318,21 +301,21 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant_
         const int q0 = qt * BN + c;
         if (SWAP) {
           const int n = p0 + static_cast<int>(lane);
-          if (n < a.p.rows) {
+          if (n < a.p_rows) {
             const long long at = b * a.stride_c + static_cast<long long>(q0) * a.ldc + n;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (c + j < BN && q0 + j < a.q.rows) mx_store_one(a.C, a.out_type, at + j * a.ldc, __uint_as_float(v[j]));
+              if (c + j < BN && q0 + j < a.q_rows) mx_store_one(a.C, a.out_type, at + j * a.ldc, __uint_as_float(v[j]));
           }
         } else {
           mx_store_rows(stage_mem, v, a.C, b * a.stride_c + static_cast<long long>(p0) * a.ldc + q0, a.ldc, a.out_type,
-                        a.p.rows - p0, min(32, a.q.rows - q0), a.vec_ok != 0);
+                        a.p_rows - p0, min(32, a.q_rows - q0), a.vec_ok != 0);
         }
       }
       tcgen05_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->acc_empty[acc]);
-      if (++acc == S::kAccStages) { acc = 0; acc_phase ^= 1u; }
+      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
   }
   tcgen05_fence_before_sync();
@@ -340,7 +323,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant_
   if (threadIdx.x == 0 && *abort_flag != 0) atomicOr(&g_mx_status[0], 1u);
   if (warp == 1) {
     tcgen05_fence_after_sync();
-    tmem_dealloc(tmem, S::kTmemCols);
+    tmem_dealloc(tmem, 512);
   }
 }
 

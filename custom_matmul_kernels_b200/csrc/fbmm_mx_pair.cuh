@@ -65,7 +65,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   uint8_t* epi = smem + kMxPairStages * kMxPairStage;
   MxPairBarriers* bars = reinterpret_cast<MxPairBarriers*>(epi + kMxPairEpiBytes);
   volatile uint32_t* abort_flag = &bars->abort_flag;
-  const uint32_t warp = threadIdx.x >> 5, lane = lane_id();
+  const uint32_t warp = warp_index(), lane = lane_id();
   const uint32_t rank = cluster_cta_rank();
   if (threadIdx.x == 0) {
     bars->abort_flag = 0;
@@ -97,7 +97,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   const long long u0 = blockIdx.x >> 1, du = gridDim.x >> 1;
 
   if (warp == 0) {
-    if (lane == 0) {
+    {
       uint32_t stage = 0, phase = 0;
       bool ok = true;
       for (long long u = u0; u < units && ok; u += du) {
@@ -105,16 +105,19 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         x16_decode(u, a.m_tiles, a.n_tiles, b, mt, nt);
         const int mr = mt * 256 + static_cast<int>(rank) * 128, nr = nt * 256 + static_cast<int>(rank) * 128;
         for (int kb = 0; kb < kblocks; ++kb) {
-          ok = mbar_wait_cluster(&bars->empty[stage], phase ^ 1u, abort_flag);
+          ok = __all_sync(0xffffffffu, mbar_wait_cluster(&bars->empty[stage], phase ^ 1u, abort_flag));
           if (!ok) break;
           uint8_t* st = smem + stage * kMxPairStage;
           uint8_t* sf = st + 2 * kMxPairPart;
           const uint32_t full = bars0 + off(&bars->full[stage]);
-          if (rank == 0) mbar_arrive_expect_tx(&bars->full[stage], 2 * kMxPairStage);
-          tma_load_3d_pair(st, &map_a, full, kb * kMxRowBytes, mr, a.a_shared ? 0 : b, kL2EvictLast);
-          tma_load_3d_pair(st + kMxPairPart, &map_b, full, kb * kMxRowBytes, nr, a.b_shared ? 0 : b, kL2EvictLast);
-          tma_load_3d_pair(sf, &map_sa, full, kb * (kMxScaleStage / 4), mr / 128, a.as_shared ? 0 : b, kL2EvictLast);
-          tma_load_3d_pair(sf + kMxScaleStage, &map_sb, full, kb * (kMxScaleStage / 4), nt * 2, a.bs_shared ? 0 : b, kL2EvictLast);
+          if (elect_one()) {
+            if (rank == 0) mbar_arrive_expect_tx(&bars->full[stage], 2 * kMxPairStage);
+            tma_load_3d_pair(st, &map_a, full, kb * kMxRowBytes, mr, a.a_shared ? 0 : b, kL2EvictLast);
+            tma_load_3d_pair(st + kMxPairPart, &map_b, full, kb * kMxRowBytes, nr, a.b_shared ? 0 : b, kL2EvictLast);
+            tma_load_3d_pair(sf, &map_sa, full, kb * (kMxScaleStage / 4), mr / 128, a.as_shared ? 0 : b, kL2EvictLast);
+            tma_load_3d_pair(sf + kMxScaleStage, &map_sb, full, kb * (kMxScaleStage / 4), nt * 2, a.bs_shared ? 0 : b, kL2EvictLast);
+          }
+          __syncwarp();
           if (++stage == kMxPairStages) { stage = 0; phase ^= 1u; }
         }
       }
@@ -124,36 +127,37 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       uint32_t stage = 0, phase = 0, acc_phase = 0;
       bool ok = true;
       for (long long u = u0; u < units && ok; u += du) {
-        ok = mbar_wait_cluster(&bars->acc_empty, acc_phase ^ 1u, abort_flag);
+        ok = __all_sync(0xffffffffu, mbar_wait_cluster(&bars->acc_empty, acc_phase ^ 1u, abort_flag));
         if (!ok) break;
-        tcgen05_fence_after_sync();
         for (int kb = 0; kb < kblocks; ++kb) {
-          ok = mbar_wait_cluster(&bars->full[stage], phase, abort_flag);
+          ok = __all_sync(0xffffffffu, mbar_wait_cluster(&bars->full[stage], phase, abort_flag));
           if (!ok) break;
           tcgen05_fence_after_sync();
           const uint32_t st = smem_u32(smem + stage * kMxPairStage);
           const uint32_t sf = st + 2 * kMxPairPart;
           const uint32_t t_sf = tmem + 256 + stage * kMxPairSfCols;  // per group of k: 4 columns of A, 8 of B
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            mx_copy_scales_pair(t_sf + g * 12, mx_desc_scales(sf + g * kMxGroupBytes));
-            mx_copy_scales_pair(t_sf + g * 12 + 4, mx_desc_scales(sf + kMxScaleStage + g * kMxGroupBytes));
-            mx_copy_scales_pair(t_sf + g * 12 + 8, mx_desc_scales(sf + 2 * kMxScaleStage + g * kMxGroupBytes));
-          }
           const uint64_t ad = mx_desc_codes(st), bd = mx_desc_codes(st + kMxPairPart);
+          if (elect_one()) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            mx_umma_pair(tmem, ad + q * 2, bd + q * 2, mx_idesc(256, 256, (q & 1) * 2), t_sf + (q >> 1) * 12,
-                         t_sf + (q >> 1) * 12 + 4, (kb | q) != 0 ? 1u : 0u);
-          commit(&bars->empty[stage]);
+            for (int g = 0; g < 2; ++g) {
+              mx_copy_scales_pair(t_sf + g * 12, mx_desc_scales(sf + g * kMxGroupBytes));
+              mx_copy_scales_pair(t_sf + g * 12 + 4, mx_desc_scales(sf + kMxScaleStage + g * kMxGroupBytes));
+              mx_copy_scales_pair(t_sf + g * 12 + 8, mx_desc_scales(sf + 2 * kMxScaleStage + g * kMxGroupBytes));
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              mx_umma_pair(tmem, ad + q * 2, bd + q * 2, mx_idesc(256, 256, (q & 1) * 2), t_sf + (q >> 1) * 12,
+                           t_sf + (q >> 1) * 12 + 4, (kb | q) != 0 ? 1u : 0u);
+            commit(&bars->empty[stage]);
+            if (kb == kblocks - 1) commit(&bars->acc_full);
+          }
+          __syncwarp();
           if (++stage == kMxPairStages) { stage = 0; phase ^= 1u; }
         }
-        if (!ok) break;
-        commit(&bars->acc_full);
         acc_phase ^= 1u;
       }
     }

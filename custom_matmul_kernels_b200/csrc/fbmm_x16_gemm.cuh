@@ -78,6 +78,14 @@ __device__ __forceinline__ void umma_f16_pair(uint32_t d_tmem, uint64_t a_desc, 
       : "memory");
 }
 
+// Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) into shared memory.
+__device__ __forceinline__ void mx_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
 // Shared-memory descriptor of a 128-row part with the 128-byte swizzle. K-major: 8-row groups 1024
 // bytes apart, an MMA step (16 j) is 32 bytes. MN-major: chunks of 64 rows kX16Chunk apart, 8-j groups 1024 bytes
 // apart, an MMA step is 2048 bytes.
@@ -161,7 +169,7 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   uint8_t* epi = smem + kX16Stages * S::kStageBytes;
   X16Barriers* bars = reinterpret_cast<X16Barriers*>(epi + kMxEpiBytes);
   volatile uint32_t* abort_flag = &bars->abort_flag;
-  const uint32_t warp = threadIdx.x >> 5, lane = lane_id();
+  const uint32_t warp = warp_index(), lane = lane_id();
   const uint32_t rank = PAIR ? cluster_cta_rank() : 0u;
   if (threadIdx.x == 0) {
     bars->abort_flag = 0;
@@ -205,7 +213,7 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   const long long u0 = PAIR ? blockIdx.x >> 1 : blockIdx.x, du = PAIR ? gridDim.x >> 1 : gridDim.x;
 
   if (warp == 0) {
-    if (lane == 0) {
+    {
       uint32_t stage = 0, phase = 0;
       bool ok = true;
       // 128 rows of one operand, from row r0: to the part's place, or its raw codes
@@ -240,12 +248,15 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         x16_decode(u, a.x_tiles, a.y_tiles, b, xt, yt);
         const int xr = xt * kTile + static_cast<int>(rank) * 128, yr = yt * kTile + static_cast<int>(rank) * 128;
         for (int jb = 0; jb < jblocks; ++jb) {
-          ok = wait(&bars->empty[stage], phase ^ 1u);
+          ok = __all_sync(0xffffffffu, wait(&bars->empty[stage], phase ^ 1u));
           if (!ok) break;
           uint8_t* st = smem + stage * S::kStageBytes;
-          if (rank == 0) mbar_arrive_expect_tx(&bars->full[stage], kDense * kCtas);
-          load(&map_x, XK, st, st + 2 * kX16Part, jb * kX16J, xr, b, a.x);
-          load(&map_y, YK, st + kX16Part, st + 2 * kX16Part, jb * kX16J, yr, b, a.y);
+          if (elect_one()) {
+            if (rank == 0) mbar_arrive_expect_tx(&bars->full[stage], kDense * kCtas);
+            load(&map_x, XK, st, st + 2 * kX16Part, jb * kX16J, xr, b, a.x);
+            load(&map_y, YK, st + kX16Part, st + 2 * kX16Part, jb * kX16J, yr, b, a.y);
+          }
+          __syncwarp();
           if (++stage == kX16Stages) { stage = 0; phase ^= 1u; }
         }
       }
@@ -255,33 +266,34 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
       bool ok = true;
       constexpr bool kXmn = XK != kX16K, kYmn = YK != kX16K;
       const uint32_t idesc = make_idesc_f16(kTile, kTile, a.dtype == 2) | (kXmn ? 1u << 15 : 0u) | (kYmn ? 1u << 16 : 0u);
       for (long long u = u0; u < units && ok; u += du) {
-        ok = wait(&bars->acc_empty[acc], acc_phase ^ 1u);
+        ok = __all_sync(0xffffffffu, wait(&bars->acc_empty[acc], acc_phase ^ 1u));
         if (!ok) break;
-        tcgen05_fence_after_sync();
         const uint32_t d = tmem + acc * 256;
         for (int jb = 0; jb < jblocks; ++jb) {
-          ok = wait(&bars->full[stage], phase);
+          ok = __all_sync(0xffffffffu, wait(&bars->full[stage], phase));
           if (!ok) break;
           tcgen05_fence_after_sync();
           const uint32_t st = smem_u32(smem + stage * S::kStageBytes);
           const uint64_t xd = x16_desc(st, kXmn), yd = x16_desc(st + kX16Part, kYmn);
+          if (elect_one()) {
 #pragma unroll
-          for (int q = 0; q < kX16J / 16; ++q) {
-            const uint64_t xs = xd + q * ((kXmn ? 2048 : 32) >> 4), ys = yd + q * ((kYmn ? 2048 : 32) >> 4);
-            if (PAIR) umma_f16_pair(d, xs, ys, idesc, (jb | q) != 0 ? 1u : 0u);
-            else umma_f16(d, xs, ys, idesc, (jb | q) != 0 ? 1u : 0u);
+            for (int q = 0; q < kX16J / 16; ++q) {
+              const uint64_t xs = xd + q * ((kXmn ? 2048 : 32) >> 4), ys = yd + q * ((kYmn ? 2048 : 32) >> 4);
+              if (PAIR) umma_f16_pair(d, xs, ys, idesc, (jb | q) != 0 ? 1u : 0u);
+              else umma_f16(d, xs, ys, idesc, (jb | q) != 0 ? 1u : 0u);
+            }
+            commit(&bars->empty[stage]);
+            if (jb == jblocks - 1) commit(&bars->acc_full[acc]);
           }
-          commit(&bars->empty[stage]);
+          __syncwarp();
           if (++stage == kX16Stages) { stage = 0; phase ^= 1u; }
         }
-        if (!ok) break;
-        commit(&bars->acc_full[acc]);
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
     }
