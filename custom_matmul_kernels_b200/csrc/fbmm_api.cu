@@ -197,6 +197,17 @@ void tensor_map_remember(const TensorMapKey& key, const CUtensorMap& map) {
   if (g_tm_cache.used < kTensorMapCacheSize) ++g_tm_cache.used;
 }
 
+// cuTensorMapEncodeTiled is a driver call and wants a current context, which a thread that has made no
+// runtime call yet (the thread of a backward pass, for one) does not have: naming its device gives it one.
+template <typename... Args>
+CUresult encode_tiled(Args... args) {
+  CUresult r = g_encode(args...);
+  int dev = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+    r = g_encode(args...);
+  return r;
+}
+
 int encode_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base, const cuuint64_t dims[3],
               const cuuint64_t strides[2], const cuuint32_t box[3], bool swizzle128) {
   const TensorMapKey key{base, static_cast<long long>(strides[0]), static_cast<long long>(strides[1]),
@@ -205,7 +216,7 @@ int encode_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base, cons
                          16 + static_cast<int>(type) * 1024 + static_cast<int>(box[0]) * 2 + (swizzle128 ? 1 : 0)};
   if (tensor_map_lookup(key, map)) return FBMM_OK;
   cuuint32_t elem_strides[3] = {1, 1, 1};
-  const CUresult r = g_encode(map, type, 3, const_cast<void*>(base), dims, strides, box, elem_strides,
+  const CUresult r = encode_tiled(map, type, 3, const_cast<void*>(base), dims, strides, box, elem_strides,
                               CU_TENSOR_MAP_INTERLEAVE_NONE,
                               swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -234,7 +245,7 @@ int make_tensor_map(CUtensorMap* map, const Operand& op, int k, int l, int box_r
   const cuuint64_t pitch_bytes = static_cast<cuuint64_t>(op.ld) * 4u;
   cuuint64_t strides[2] = {pitch_bytes, one_batch ? pitch_bytes * dims[1] : static_cast<cuuint64_t>(op.stride) * 4u};
   cuuint32_t elem_strides[3] = {1, 1, 1};
-  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(op.ptr), dims, strides,
+  const CUresult r = encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(op.ptr), dims, strides,
                               box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               op.mn_major ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -254,7 +265,7 @@ int make_mask_map(CUtensorMap* map, const unsigned char* ptr, int rows, int cols
   cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows) * static_cast<cuuint64_t>(cols)};
   cuuint32_t elem_strides[3] = {1, 1, 1};
-  const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<unsigned char*>(ptr), dims, strides, box,
+  const CUresult r = encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<unsigned char*>(ptr), dims, strides, box,
                               elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(FBMM_ERR_CUDA, "cuTensorMapEncodeTiled (mask) failed with CUresult %d", static_cast<int>(r));
@@ -1279,7 +1290,7 @@ int make_tensor_map_x16(CUtensorMap* map, const Operand& op, int k, int l, int b
   const cuuint64_t pitch_bytes = static_cast<cuuint64_t>(op.ld) * 2u;
   cuuint64_t strides[2] = {pitch_bytes, one_batch ? pitch_bytes * dims[1] : static_cast<cuuint64_t>(op.stride) * 2u};
   cuuint32_t elem_strides[3] = {1, 1, 1};
-  const CUresult r = g_encode(map, dtype == FBMM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+  const CUresult r = encode_tiled(map, dtype == FBMM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                               3, const_cast<float*>(op.ptr), dims, strides, box, elem_strides,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

@@ -120,60 +120,60 @@ __device__ __forceinline__ void mx_store_one(void* C, int out_type, long long at
   else static_cast<__nv_bfloat16*>(C)[at] = __float2bfloat16_rn(v);
 }
 
-// 32 rows x 32 columns of a warp (lane = row, v = its columns) -> row-major C. The lanes' 16-byte
-// pieces cross the warp's staging area (chunk index xor row, free of bank conflicts) so that a store
-// instruction covers whole 64- or 128-byte row pieces. `C0`: element (row 0, column 0) of the block.
-__device__ __forceinline__ void mx_store_rows(uint8_t* stage, const uint32_t (&v)[32], void* C, long long c0, long long ldc,
-                                              int out_type, int rows, int cols, bool vec) {
+// 32 rows of a warp's accumulators (lane = row) -> row-major C, 128 bytes of every row at a time: 64 columns
+// (v0, v1) of a 16-bit type, or 32 columns of fp32 in two calls. The lanes' 16-byte pieces cross the
+// warp's staging area (piece index xor row, free of bank conflicts) so that every store instruction covers
+// four whole 128-byte lines; with 64-byte pieces of rows 16-bit results left at 2.0 TB/s (8192 x 8192 with
+// k = 256: 68 us, xxx with whole lines). `c0`: element (row 0, column 0) of the block.
+template <typename Word>
+__device__ __forceinline__ void mx_store_lines(uint8_t* stage, Word word, void* C, long long c0, long long ldc, int size,
+                                               int rows, int cols, bool vec) {
   const int lane = static_cast<int>(lane_id());
   uint4* st = reinterpret_cast<uint4*>(stage);
   __syncwarp();
-  if (out_type == 0) {
 #pragma unroll
-    for (int c = 0; c < 8; ++c) st[lane * 8 + (c ^ (lane & 7))] = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-    __syncwarp();
-    float* out = static_cast<float*>(C) + c0;
+  for (int c = 0; c < 8; ++c) st[lane * 8 + (c ^ (lane & 7))] = word(c);
+  __syncwarp();
+  const int per = 16 / size;  // elements of a piece
+  const int c = lane & 7;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = i * 4 + (lane >> 3), c = lane & 7;
-      const uint4 x = st[r * 8 + (c ^ (r & 7))];
-      if (r < rows) {
-        float* at = out + r * ldc + c * 4;
-        if (vec && c * 4 + 4 <= cols) {
-          *reinterpret_cast<uint4*>(at) = x;
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3);
+    const uint4 x = st[r * 8 + (c ^ (r & 7))];
+    if (r < rows) {
+      uint8_t* at = static_cast<uint8_t*>(C) + (c0 + r * ldc) * size + c * 16;
+      if (vec && (c + 1) * per <= cols) {
+        *reinterpret_cast<uint4*>(at) = x;
+      } else {
+        const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+        if (size == 4) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) if (c * 4 + j < cols) reinterpret_cast<uint32_t*>(at)[j] = e[j];
         } else {
-          const uint32_t e[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) if (c * 4 + j < cols) at[j] = __uint_as_float(e[j]);
+          for (int j = 0; j < 8; ++j)
+            if (c * 8 + j < cols) reinterpret_cast<uint16_t*>(at)[j] = static_cast<uint16_t>(e[j >> 1] >> (16 * (j & 1)));
         }
       }
     }
+  }
+}
+__device__ __forceinline__ void mx_store_rows(uint8_t* stage, const uint32_t (&v0)[32], const uint32_t (&v1)[32], void* C,
+                                              long long c0, long long ldc, int out_type, int rows, int cols, bool vec) {
+  if (out_type == 0) {
+    mx_store_lines(stage, [&](int c) { return make_uint4(v0[4 * c], v0[4 * c + 1], v0[4 * c + 2], v0[4 * c + 3]); }, C, c0,
+                   ldc, 4, rows, cols, vec);
+    mx_store_lines(stage, [&](int c) { return make_uint4(v1[4 * c], v1[4 * c + 1], v1[4 * c + 2], v1[4 * c + 3]); }, C,
+                   c0 + 32, ldc, 4, rows, cols - 32, vec);
   } else {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    mx_store_lines(stage, [&](int c) {
+      const uint32_t (&v)[32] = c < 4 ? v0 : v1;
       uint32_t p[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        p[j] = mx_pack_out(out_type, __uint_as_float(v[8 * c + 2 * j]), __uint_as_float(v[8 * c + 2 * j + 1]));
-      st[lane * 4 + (c ^ ((lane >> 1) & 3))] = make_uint4(p[0], p[1], p[2], p[3]);
-    }
-    __syncwarp();
-    uint16_t* out = static_cast<uint16_t*>(C) + c0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = i * 8 + (lane >> 2), c = lane & 3;
-      const uint4 x = st[r * 4 + (c ^ ((r >> 1) & 3))];
-      if (r < rows) {
-        uint16_t* at = out + r * ldc + c * 8;
-        if (vec && c * 8 + 8 <= cols) {
-          *reinterpret_cast<uint4*>(at) = x;
-        } else {
-          const uint32_t e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int j = 0; j < 8; ++j) if (c * 8 + j < cols) at[j] = static_cast<uint16_t>(e[j >> 1] >> (16 * (j & 1)));
-        }
-      }
-    }
+        p[j] = mx_pack_out(out_type, __uint_as_float(v[8 * (c & 3) + 2 * j]), __uint_as_float(v[8 * (c & 3) + 2 * j + 1]));
+      return make_uint4(p[0], p[1], p[2], p[3]);
+    }, C, c0, ldc, 2, rows, cols, vec);
   }
 }
 
@@ -293,13 +293,13 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant_
       tcgen05_fence_after_sync();
       const uint32_t t = tmem + acc * BN + ((quarter * 32u) << 16);
       const int p0 = pt * kMxM + static_cast<int>(quarter) * 32;
+      if (SWAP) {
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(t + c, v);
-        tmem_ld_wait();
-        const int q0 = qt * BN + c;
-        if (SWAP) {
+        for (int c = 0; c < BN; c += 32) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(t + c, v);
+          tmem_ld_wait();
+          const int q0 = qt * BN + c;
           const int n = p0 + static_cast<int>(lane);
           if (n < a.p_rows) {
             const long long at = b * a.stride_c + static_cast<long long>(q0) * a.ldc + n;
@@ -307,9 +307,18 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant_
             for (int j = 0; j < 32; ++j)
               if (c + j < BN && q0 + j < a.q_rows) mx_store_one(a.C, a.out_type, at + j * a.ldc, __uint_as_float(v[j]));
           }
-        } else {
-          mx_store_rows(stage_mem, v, a.C, b * a.stride_c + static_cast<long long>(p0) * a.ldc + q0, a.ldc, a.out_type,
-                        a.p_rows - p0, min(32, a.q_rows - q0), a.vec_ok != 0);
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < BN; c += 64) {
+          const int q0 = qt * BN + c;
+          if (q0 >= a.q_rows || p0 >= a.p_rows) break;  // warp-uniform
+          uint32_t v0[32], v1[32];
+          tmem_ld_32x32b_x32(t + c, v0);
+          tmem_ld_32x32b_x32(t + c + 32, v1);
+          tmem_ld_wait();
+          mx_store_rows(stage_mem, v0, v1, a.C, b * a.stride_c + static_cast<long long>(p0) * a.ldc + q0, a.ldc, a.out_type,
+                        a.p_rows - p0, a.q_rows - q0, a.vec_ok != 0);
         }
       }
       tcgen05_fence_before_sync();

@@ -185,11 +185,11 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
       acc_phase ^= 1u;
       const int m0 = mt * 256 + static_cast<int>(rank) * 128 + static_cast<int>(quarter) * 32;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 4; c += 2) {
         const int n0 = nt * 256 + half * 128 + c * 32;
         if (n0 < a.n && m0 < a.m)
-          mx_store_rows(stage_mem, v[c], a.C, b * a.stride_c + static_cast<long long>(m0) * a.ldc + n0, a.ldc, a.out_type,
-                        a.m - m0, min(32, a.n - n0), a.vec_ok != 0);
+          mx_store_rows(stage_mem, v[c], v[c + 1], a.C, b * a.stride_c + static_cast<long long>(m0) * a.ldc + n0, a.ldc,
+                        a.out_type, a.m - m0, a.n - n0, a.vec_ok != 0);
       }
     }
   }

@@ -337,14 +337,22 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       const uint32_t t = tmem + acc * 256 + ((quarter * 32u) << 16);
       const int x0 = xt * kTile + static_cast<int>(rank) * 128 + static_cast<int>(quarter) * 32;
 #pragma unroll 1
-      for (int c = 0; c < kTile; c += 32) {
+      for (int c = 0; c < kTile; c += 64) {
         const int y0 = yt * kTile + c;
         if (y0 >= a.y.rows || x0 >= a.x.rows) break;  // warp-uniform
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(t + c, v);
+        uint32_t v0[32], v1[32];
+        tmem_ld_32x32b_x32(t + c, v0);
+        tmem_ld_32x32b_x32(t + c + 32, v1);
         tmem_ld_wait();
-        mx_store_rows(stage_mem, v, a.C, b * a.stride_c + static_cast<long long>(x0) * a.ldc + y0, a.ldc, a.dtype,
-                      a.x.rows - x0, min(32, a.y.rows - y0), a.vec_ok != 0);
+        mx_store_lines(stage_mem, [&](int i) {
+          const uint32_t (&v)[32] = i < 4 ? v0 : v1;
+          uint32_t p[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            p[j] = mx_pack_out(a.dtype, __uint_as_float(v[8 * (i & 3) + 2 * j]), __uint_as_float(v[8 * (i & 3) + 2 * j + 1]));
+          return make_uint4(p[0], p[1], p[2], p[3]);
+        }, a.C, b * a.stride_c + static_cast<long long>(x0) * a.ldc + y0, a.ldc, 2, a.x.rows - x0, a.y.rows - y0,
+                       a.vec_ok != 0);
       }
       tcgen05_fence_before_sync();
       arrive_leader(&bars->acc_empty[acc]);

@@ -219,6 +219,26 @@ def test_product_shared_operands(dev):
         assert torch.equal(MXBMMCUDA()(B.mT, A3.mT), MXBMMCUDA()(B.mT, Ac.mT))
 
 
+def test_first_call_of_a_thread(dev):
+    """A thread that has made no CUDA call yet (as the one of a backward pass) has no context for
+    the tensor maps; shapes of its own, so that no cached map serves it."""
+    import threading
+    got = {}
+
+    def work():
+        W, w = as_mx(173, 231, 4, 5, dev, dim=-2, lo=120, hi=124)
+        X = torch.ones(1, 19, 231, device=dev)
+        got["mx"] = MXBMMCUDA()(X, W), torch.ones(1, 19, 231).double() @ w.transpose(1, 2)
+        got["f32"] = BMMCUDA()(torch.ones(1, 37, 44, device=dev), torch.ones(1, 44, 76, device=dev)), torch.full((1, 37, 76), 44.0)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    for g, w in got.values():
+        assert torch.allclose(g.cpu().double(), w.double(), rtol=1e-4, atol=1e-4)
+    assert len(got) == 2
+
+
 def test_product_empty(dev):
     B, _ = as_mx(40, 64, 4, 1, dev, dim=-2)
     assert MXBMMCUDA()(torch.empty(1, 0, 64, device=dev), B).shape == (1, 0, 40)
