@@ -23,6 +23,7 @@ UNITS = {
     os.path.join(CSRC, "fbmm_mx_api.cu"): [os.path.join(CSRC, "fbmm_mx_quant.cuh"),
                                            os.path.join(CSRC, "fbmm_mx_gemm.cuh"),
                                            os.path.join(CSRC, "fbmm_mx_pair.cuh"),
+                                           os.path.join(CSRC, "fbmm_mx_rows.cuh"),
                                            os.path.join(CSRC, "fbmm_x16_gemm.cuh")] + _SHARED,
 }
 SOURCES = list(UNITS)

@@ -1389,6 +1389,7 @@ int device_sms(int* sms) {
   if (rc == FBMM_OK) *sms = st->sms;
   return rc;
 }
+int sms_or_default() { return sm_count_or_default(); }
 int tensor_map_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base, const cuuint64_t dims[3],
                   const cuuint64_t strides[2], const cuuint32_t box[3], bool swizzle128) {
   return encode_3d(map, type, base, dims, strides, box, swizzle128);

@@ -12,6 +12,10 @@ int fail(int code, const char* fmt, ...);
 // FBMM_OK and the SM count when the current device is one this library runs on.
 int device_sms(int* sms);
 
+// SM count of the current device, or the B200's where no device can be asked (the workspace queries work on
+// a machine without one).
+int sms_or_default();
+
 // 3-D tiled tensor map (dims, strides in bytes of dims 1 and 2, box), 128-byte or no swizzle, from
 // the cache of recent maps where it is there.
 int tensor_map_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base, const cuuint64_t dims[3],

@@ -6,6 +6,7 @@
 #include "fbmm_host.h"
 #include "fbmm_mx_gemm.cuh"
 #include "fbmm_mx_quant.cuh"
+#include "fbmm_mx_rows.cuh"
 #include "fbmm_mx_pair.cuh"
 #include "fbmm_x16_gemm.cuh"
 
@@ -44,6 +45,33 @@ int check_mx(const char* name, const unsigned char* codes, long long stride_code
   if (l > 1 && (stride_codes < 0 || stride_scales < 0 || (stride_codes & 15) != 0 || (stride_scales & 15) != 0))
     return fail(FBMM_ERR_ALIGN, "%s batch strides %lld and %lld are not non-negative multiples of 16 bytes", name,
                 stride_codes, stride_scales);
+  return FBMM_OK;
+}
+
+int check_quantize_source(const void* X, int dtype, int layout, long long ldx, long long stride_x, int l, int rows, int k) {
+  int rc;
+  if ((rc = check_shape(l, rows, k)) != FBMM_OK) return rc;
+  if ((rc = check_type(dtype)) != FBMM_OK) return rc;
+  if (layout != 'n' && layout != 't') return fail(FBMM_ERR_INVALID, "layout must be 'n' or 't', got %d", layout);
+  if (X == nullptr) return fail(FBMM_ERR_INVALID, "the source is null");
+  if ((reinterpret_cast<uintptr_t>(X) & static_cast<uintptr_t>(elem_size(dtype) - 1)) != 0)
+    return fail(FBMM_ERR_ALIGN, "the source is not aligned to its element type");
+  if (ldx < (layout == 'n' ? k : rows)) return fail(FBMM_ERR_INVALID, "source pitch %lld smaller than its row length", ldx);
+  if (l > 1 && stride_x < 0) return fail(FBMM_ERR_INVALID, "source batch stride is negative");
+  return FBMM_OK;
+}
+
+int check_result(const void* C, int dtype, long long ldc, long long stride_c, int l, int m, int n) {
+  int rc;
+  if ((rc = check_type(dtype)) != FBMM_OK) return rc;
+  if (C == nullptr) return fail(FBMM_ERR_INVALID, "C is null");
+  if ((reinterpret_cast<uintptr_t>(C) & static_cast<uintptr_t>(elem_size(dtype) - 1)) != 0)
+    return fail(FBMM_ERR_ALIGN, "C is not aligned to its element type");
+  if (ldc < n) return fail(FBMM_ERR_INVALID, "ldc %lld smaller than a row of C (%d)", ldc, n);
+  if (l > 1 && stride_c < static_cast<long long>(m - 1) * ldc + n)
+    return fail(FBMM_ERR_INVALID, "batches of C overlap (stride %lld)", stride_c);
+  if (static_cast<long long>((m + 127) / 128) * ((n + 127) / 128) > 0x3fffffffLL)
+    return fail(FBMM_ERR_INVALID, "product of %d x %d is too large", m, n);
   return FBMM_OK;
 }
 
@@ -97,23 +125,22 @@ int scales_map(CUtensorMap* map, const unsigned char* scales, long long stride, 
   return fbmm_host::tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, scales, dims, strides, box, false);
 }
 
-template <int BN, bool SWAP>
 int launch_mx_gemm(cudaStream_t stream, int sms, const MxSide& p, const MxSide& q, MxGemmArgs a) {
   CUtensorMap mp, mq, msp, msq;
   int rc;
   if ((rc = codes_map(&mp, p.codes, p.stride, a.l, p.rows, a.k, kMxM)) != FBMM_OK) return rc;
-  if ((rc = codes_map(&mq, q.codes, q.stride, a.l, q.rows, a.k, BN)) != FBMM_OK) return rc;
+  if ((rc = codes_map(&mq, q.codes, q.stride, a.l, q.rows, a.k, MxShape::BN)) != FBMM_OK) return rc;
   if ((rc = scales_map(&msp, p.scales, p.scale_stride, a.l, p.rows, a.k, 1)) != FBMM_OK) return rc;
   if ((rc = scales_map(&msq, q.scales, q.scale_stride, a.l, q.rows, a.k, 1)) != FBMM_OK) return rc;
   a.p_rows = p.rows; a.q_rows = q.rows;
   a.p_shared = p.stride == 0; a.q_shared = q.stride == 0;
   a.sp_shared = p.scale_stride == 0; a.sq_shared = q.scale_stride == 0;
   a.p_tiles = (p.rows + kMxM - 1) / kMxM;
-  a.q_tiles = (q.rows + BN - 1) / BN;
+  a.q_tiles = (q.rows + MxShape::BN - 1) / MxShape::BN;
   const long long units = static_cast<long long>(a.p_tiles) * a.q_tiles * a.l;
-  using S = MxShape<BN>;
-  FBMM_HOST_CUDA(cudaFuncSetAttribute(mx_gemm_kernel<BN, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-  mx_gemm_kernel<BN, SWAP><<<static_cast<unsigned>(std::min<long long>(units, sms)), kMxThreads, S::kSmem, stream>>>(mp, mq, msp, msq, a);
+  using S = MxShape;
+  FBMM_HOST_CUDA(cudaFuncSetAttribute(mx_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+  mx_gemm_kernel<<<static_cast<unsigned>(std::min<long long>(units, sms)), kMxThreads, S::kSmem, stream>>>(mp, mq, msp, msq, a);
   FBMM_HOST_CUDA(cudaGetLastError());
   return FBMM_OK;
 }
@@ -139,6 +166,87 @@ int launch_mx_pair(cudaStream_t stream, int sms, const MxSide& A, const MxSide& 
       ma, mb, msa, msb, a);
   FBMM_HOST_CUDA(cudaGetLastError());
   return FBMM_OK;
+}
+
+constexpr int kMxFewRows = 64;  // rows of A up to which the weights take the 128-row side of the MMA
+
+// How many CTAs share the k of a tile in the few-row kernel. A CTA takes about 0.25 us per 256 k (one
+// stage's latency over the depth of the ring), joining the sums 0.7 us, and a second CTA on an SM starts 0.7 us
+// late; two fit an SM. The least sum of these decides (measured: n = 4096, k = 4096 on 128 CTAs; n = 16384, k = 8192
+// 11.0 us on 256 against 12.4 on 128; n = 1024, k = 8192 4.9 us on 64 against 11.2 on 8).
+void rows_splits(int sms, int l, int n, int k, int* splits, int* blocks) {
+  const int kblocks = (k + kMxStageK - 1) / kMxStageK;
+  const long long base = static_cast<long long>((n + kMxM - 1) / kMxM) * l;
+  long long best = 0;
+  for (int s = 1; s <= 8 && (s == 1 || s <= kblocks); s *= 2) {
+    const long long ctas = base * s, per = (kblocks + s - 1) / s;
+    const long long cost = (s > 1 ? 700 : 0) + 250 * per * ((ctas + 2 * sms - 1) / (2 * sms)) + 700 * ((ctas - 1) / sms);
+    if (s == 1 || cost < best) {
+      best = cost;
+      *splits = s;
+      *blocks = static_cast<int>(per);
+    }
+  }
+}
+
+// Whether the kernel quantises A itself. Every CTA quantises its range of k of all rows: up to 1024 blocks
+// of 32 (four a thread) that hides behind the first weights; beyond, a pass of its own is faster
+// (16 rows: 8.6 against 9.8 us at 4096 x 4096, 512 blocks; 16.6 against 14.4 us at n = 16384, k = 8192, 2048 blocks).
+// The quantised rows also have to fit beside the ring.
+bool few_rows_fused(int sms, int l, int m, int n, int k, int layout) {
+  if (m > kMxFewRows || layout != 'n') return false;
+  int splits, blocks;
+  rows_splits(sms, l, n, k, &splits, &blocks);
+  const int stages = std::min(4, blocks);
+  const int smem = m <= 16 ? MxRowsShape<16, float>::smem(stages, blocks) : MxRowsShape<64, float>::smem(stages, blocks);
+  return static_cast<long long>(m) * blocks * (kMxStageK / kMxBlock) <= 1024 && smem <= static_cast<int>(kMxSmemLimit);
+}
+
+template <int NT, typename T>
+int launch_mx_rows(cudaStream_t stream, int sms, const MxSide& W, const MxSide* A, MxRowsArgs a) {
+  using S = MxRowsShape<NT, T>;
+  CUtensorMap mw, msw, ma, msa;
+  int rc;
+  if ((rc = codes_map(&mw, W.codes, W.stride, a.l, W.rows, a.k, kMxM)) != FBMM_OK) return rc;
+  if ((rc = scales_map(&msw, W.scales, W.scale_stride, a.l, W.rows, a.k, 1)) != FBMM_OK) return rc;
+  a.w_shared = W.stride == 0; a.sw_shared = W.scale_stride == 0;
+  if (S::kCodes) {
+    if ((rc = codes_map(&ma, A->codes, A->stride, a.l, A->rows, a.k, NT)) != FBMM_OK) return rc;
+    if ((rc = scales_map(&msa, A->scales, A->scale_stride, a.l, A->rows, a.k, 1)) != FBMM_OK) return rc;
+    a.a_shared = A->stride == 0; a.sa_shared = A->scale_stride == 0;
+  } else {
+    ma = mw; msa = msw;
+  }
+  a.n_tiles = (a.n + kMxM - 1) / kMxM;
+  rows_splits(sms, a.l, a.n, a.k, &a.splits, &a.blocks_per_split);
+  const long long grid = static_cast<long long>(a.n_tiles) * a.l * a.splits;
+  if (grid > 0x7fffffffLL) return fail(FBMM_ERR_INVALID, "product of %d x %d x %d is too large", a.l, a.m, a.n);
+  const int limit = static_cast<int>(kMxSmemLimit);
+  const int budget = grid > sms && S::smem(3, a.blocks_per_split) <= limit / 2 ? limit / 2 : limit;
+  a.stages = std::min(kMxRowsMaxStages, a.blocks_per_split);
+  while (a.stages > 1 && S::smem(a.stages, a.blocks_per_split) > budget) --a.stages;
+  const int smem = S::smem(a.stages, a.blocks_per_split);
+  if (smem > limit) return fail(FBMM_ERR_INVALID, "internal: few-row kernel wants %d bytes of shared memory", smem);
+  FBMM_HOST_CUDA(cudaFuncSetAttribute(mx_rows_kernel<NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, limit));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(a.splits); attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  FBMM_HOST_CUDA(cudaLaunchKernelEx(&cfg, mx_rows_kernel<NT, T>, mw, msw, ma, msa, a));
+  return FBMM_OK;
+}
+
+template <int NT>
+int launch_mx_rows_fused(cudaStream_t stream, int sms, int dtype, const MxSide& W, const MxRowsArgs& a) {
+  if (dtype == FBMM_F32) return launch_mx_rows<NT, float>(stream, sms, W, nullptr, a);
+  if (dtype == FBMM_F16) return launch_mx_rows<NT, __half>(stream, sms, W, nullptr, a);
+  return launch_mx_rows<NT, __nv_bfloat16>(stream, sms, W, nullptr, a);
 }
 
 // One operand of a 16-bit product: a dense matrix of `rows` x J (J contiguous, or the rows), or a
@@ -227,13 +335,7 @@ int x16_product(cudaStream_t stream, const X16Side& x, const X16Side& y, int dty
     return fail(FBMM_ERR_INVALID, "dtype must be FBMM_F16 (1) or FBMM_BF16 (2), got %d", dtype);
   if ((rc = check_x16_side(xn, x, J, l)) != FBMM_OK) return rc;
   if ((rc = check_x16_side(yn, y, J, l)) != FBMM_OK) return rc;
-  if (C == nullptr) return fail(FBMM_ERR_INVALID, "C is null");
-  if ((reinterpret_cast<uintptr_t>(C) & 1u) != 0) return fail(FBMM_ERR_ALIGN, "C is not 2-byte aligned");
-  if (ldc < y.rows) return fail(FBMM_ERR_INVALID, "ldc %lld smaller than a row of C (%d)", ldc, y.rows);
-  if (l > 1 && stride_c < static_cast<long long>(x.rows - 1) * ldc + y.rows)
-    return fail(FBMM_ERR_INVALID, "batches of C overlap (stride %lld)", stride_c);
-  if (static_cast<long long>((x.rows + 127) / 128) * ((y.rows + 127) / 128) > 0x3fffffffLL)
-    return fail(FBMM_ERR_INVALID, "product of %d x %d is too large", x.rows, y.rows);
+  if ((rc = check_result(C, dtype, ldc, stride_c, l, x.rows, y.rows)) != FBMM_OK) return rc;
   if ((rc = fbmm_host::device_sms(&sms)) != FBMM_OK) return rc;
   CUtensorMap mx, my;
   if ((rc = x16_map(&mx, x, J, l, dtype)) != FBMM_OK) return rc;
@@ -293,15 +395,8 @@ int fbmm_mx_quantize(void* stream_, const void* X, int dtype, int layout, long l
                      unsigned char* codes, unsigned char* scales, int l, int rows, int k) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   int rc, sms;
-  if ((rc = check_shape(l, rows, k)) != FBMM_OK) return rc;
+  if ((rc = check_quantize_source(X, dtype, layout, ldx, stride_x, l, rows, k)) != FBMM_OK) return rc;
   if ((rc = check_bits(bits)) != FBMM_OK) return rc;
-  if ((rc = check_type(dtype)) != FBMM_OK) return rc;
-  if (layout != 'n' && layout != 't') return fail(FBMM_ERR_INVALID, "layout must be 'n' or 't', got %d", layout);
-  if (X == nullptr) return fail(FBMM_ERR_INVALID, "X is null");
-  if ((reinterpret_cast<uintptr_t>(X) & static_cast<uintptr_t>(elem_size(dtype) - 1)) != 0)
-    return fail(FBMM_ERR_ALIGN, "X is not aligned to its element type");
-  if (ldx < (layout == 'n' ? k : rows)) return fail(FBMM_ERR_INVALID, "X pitch %lld smaller than its row length", ldx);
-  if (l > 1 && stride_x < 0) return fail(FBMM_ERR_INVALID, "X batch stride is negative");
   if ((rc = check_mx("output", codes, 0, scales, 0, 1)) != FBMM_OK) return rc;
   if ((rc = fbmm_host::device_sms(&sms)) != FBMM_OK) return rc;
   const MxQuantArgs a{X, ldx, l > 1 ? stride_x : 0, codes, scales, rows, k, l};
@@ -351,17 +446,9 @@ int fbmm_mx4_bmm(void* stream_, const unsigned char* a_codes, long long stride_a
   int rc, sms;
   if ((rc = check_shape(l, m, k)) != FBMM_OK) return rc;
   if ((rc = check_shape(l, n, k)) != FBMM_OK) return rc;
-  if ((rc = check_type(dtype)) != FBMM_OK) return rc;
   if ((rc = check_mx("A", a_codes, stride_a, a_scales, stride_as, l)) != FBMM_OK) return rc;
   if ((rc = check_mx("B", b_codes, stride_b, b_scales, stride_bs, l)) != FBMM_OK) return rc;
-  if (C == nullptr) return fail(FBMM_ERR_INVALID, "C is null");
-  if ((reinterpret_cast<uintptr_t>(C) & static_cast<uintptr_t>(elem_size(dtype) - 1)) != 0)
-    return fail(FBMM_ERR_ALIGN, "C is not aligned to its element type");
-  if (ldc < n) return fail(FBMM_ERR_INVALID, "ldc %lld smaller than n = %d", ldc, n);
-  if (l > 1 && stride_c < static_cast<long long>(m - 1) * ldc + n)
-    return fail(FBMM_ERR_INVALID, "batches of C overlap (stride %lld)", stride_c);
-  if (static_cast<long long>((m + 127) / 128) * ((n + 127) / 128) > 0x7fffffffLL)
-    return fail(FBMM_ERR_INVALID, "product of %d x %d is too large", m, n);
+  if ((rc = check_result(C, dtype, ldc, stride_c, l, m, n)) != FBMM_OK) return rc;
   if ((rc = fbmm_host::device_sms(&sms)) != FBMM_OK) return rc;
   MxGemmArgs a{};
   a.C = C; a.ldc = ldc; a.stride_c = l > 1 ? stride_c : 0;
@@ -369,32 +456,54 @@ int fbmm_mx4_bmm(void* stream_, const unsigned char* a_codes, long long stride_a
   const long long size = elem_size(dtype);
   a.vec_ok = ((reinterpret_cast<uintptr_t>(C) | (ldc * size) | (a.stride_c * size)) & 15) == 0;
   const MxSide A{a_codes, stride_a, a_scales, stride_as, m}, B{b_codes, stride_b, b_scales, stride_bs, n};
-  if (m <= 16) return launch_mx_gemm<16, true>(stream, sms, B, A, a);
-  if (m <= 64) return launch_mx_gemm<64, true>(stream, sms, B, A, a);
+  if (m <= kMxFewRows) {
+    MxRowsArgs r{};
+    r.C = C; r.ldc = ldc; r.stride_c = a.stride_c;
+    r.l = l; r.m = m; r.n = n; r.k = k;
+    r.out_type = dtype; r.vec_ok = a.vec_ok;
+    return m <= 16 ? launch_mx_rows<16, uint8_t>(stream, sms, B, &A, r) : launch_mx_rows<64, uint8_t>(stream, sms, B, &A, r);
+  }
   const long long pairs = static_cast<long long>((m + 255) / 256) * ((n + 255) / 256) * l;
   const long long singles = static_cast<long long>((m + 127) / 128) * ((n + 127) / 128) * l;
   const long long pair_waves = (pairs + sms / 2 - 1) / (sms / 2), single_waves = (singles + sms - 1) / sms;
   if (5 * pair_waves <= 4 * single_waves) return launch_mx_pair(stream, sms, A, B, a);
-  return launch_mx_gemm<128, false>(stream, sms, A, B, a);
+  return launch_mx_gemm(stream, sms, A, B, a);
 }
 
-size_t fbmm_mx4_bmm_tensor_workspace_bytes(int l, int m, int k) {
-  const size_t codes = fbmm_mx_codes_bytes(l, m, k, 4);
-  return (codes + 255) / 256 * 256 + fbmm_mx_scales_bytes(l, m, k);
+size_t fbmm_mx4_bmm_tensor_workspace_bytes(int l, int m, int n, int k, int a_layout) {
+  if (l <= 0 || m <= 0 || n <= 0 || k <= 0 || few_rows_fused(fbmm_host::sms_or_default(), l, m, n, k, a_layout)) return 0;
+  return (fbmm_mx_codes_bytes(l, m, k, 4) + 255) / 256 * 256 + fbmm_mx_scales_bytes(l, m, k);
 }
 
 int fbmm_mx4_bmm_tensor(void* stream, const void* A, int a_dtype, int a_layout, long long lda, long long stride_a,
                         const unsigned char* b_codes, long long stride_b, const unsigned char* b_scales,
                         long long stride_bs, void* C, int dtype, long long ldc, long long stride_c, int l, int m, int n,
                         int k, void* workspace, size_t workspace_bytes) {
-  const size_t need = fbmm_mx4_bmm_tensor_workspace_bytes(l, m, k);
+  int rc, sms;
+  if ((rc = check_quantize_source(A, a_dtype, a_layout, lda, stride_a, l, m, k)) != FBMM_OK) return rc;
+  if ((rc = check_shape(l, n, k)) != FBMM_OK) return rc;
+  if (few_rows_fused(fbmm_host::sms_or_default(), l, m, n, k, a_layout)) {
+    if ((rc = check_mx("B", b_codes, stride_b, b_scales, stride_bs, l)) != FBMM_OK) return rc;
+    if ((rc = check_result(C, dtype, ldc, stride_c, l, m, n)) != FBMM_OK) return rc;
+    if ((rc = fbmm_host::device_sms(&sms)) != FBMM_OK) return rc;
+    MxRowsArgs a{};
+    a.x = A; a.ldx = lda; a.stride_x = l > 1 ? stride_a : 0;
+    a.C = C; a.ldc = ldc; a.stride_c = l > 1 ? stride_c : 0;
+    a.l = l; a.m = m; a.n = n; a.k = k;
+    a.out_type = dtype;
+    const long long size = elem_size(dtype);
+    a.vec_ok = ((reinterpret_cast<uintptr_t>(C) | (ldc * size) | (a.stride_c * size)) & 15) == 0;
+    const MxSide W{b_codes, stride_b, b_scales, stride_bs, n};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return m <= 16 ? launch_mx_rows_fused<16>(s, sms, a_dtype, W, a) : launch_mx_rows_fused<64>(s, sms, a_dtype, W, a);
+  }
+  const size_t need = fbmm_mx4_bmm_tensor_workspace_bytes(l, m, n, k, a_layout);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(FBMM_ERR_WORKSPACE, "fbmm_mx4_bmm_tensor needs %zu workspace bytes, got %zu", need,
                 workspace == nullptr ? static_cast<size_t>(0) : workspace_bytes);
   unsigned char* codes = static_cast<unsigned char*>(workspace);
   unsigned char* scales = codes + (need - fbmm_mx_scales_bytes(l, m, k));
-  const int rc = fbmm_mx_quantize(stream, A, a_dtype, a_layout, lda, stride_a, 4, codes, scales, l, m, k);
-  if (rc != FBMM_OK) return rc;
+  if ((rc = fbmm_mx_quantize(stream, A, a_dtype, a_layout, lda, stride_a, 4, codes, scales, l, m, k)) != FBMM_OK) return rc;
   return fbmm_mx4_bmm(stream, codes, static_cast<long long>(m) * mx_pitch(k, 4), scales, mx_scale_bytes(m, k), b_codes,
                       stride_b, b_scales, stride_bs, C, dtype, ldc, stride_c, l, m, n, k);
 }

@@ -40,8 +40,8 @@ struct MxGemmArgs {
   int vec_ok;    // C's rows are 16-byte aligned
 };
 
-template <int BN>
 struct MxShape {
+  static constexpr int BN = 128;
   static constexpr int kPBytes = kMxM * kMxRowBytes, kQBytes = BN * kMxRowBytes;
   static constexpr int kSfCols = 16;  // tensor-memory columns of a stage's scales
   static constexpr int kStageBytes = kPBytes + kQBytes + 2 * kMxScaleStage;
@@ -49,7 +49,7 @@ struct MxShape {
   static constexpr int kFit = static_cast<int>((kMxSmemLimit - 1024 - 256 - kMxEpiBytes) / kStageBytes);
   static constexpr int kStages = kFit < kMxMaxStages ? kFit : kMxMaxStages;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kMxEpiBytes + 256;
-  static_assert(BN <= 128 && kSfBase + kStages * kSfCols <= 512, "tensor memory");
+  static_assert(kSfBase + kStages * kSfCols <= 512, "tensor memory");
 };
 
 struct MxBarriers {
@@ -177,13 +177,12 @@ __device__ __forceinline__ void mx_store_rows(uint8_t* stage, const uint32_t (&v
   }
 }
 
-// SWAP = false: p = A, q = B, accumulator lanes are rows of C. SWAP = true: p = B, q = A (few rows
-// of A: the weights fill the 128-row side of the MMA), lanes are columns of C.
-template <int BN, bool SWAP>
+// p = A, q = B; a 128 x 128 tile.
 __global__ void __launch_bounds__(kMxThreads, 1)
 mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                const __grid_constant__ CUtensorMap map_sp, const __grid_constant__ CUtensorMap map_sq, const MxGemmArgs a) {
-  using S = MxShape<BN>;
+  using S = MxShape;
+  constexpr int BN = S::BN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* epi = smem + S::kStages * S::kStageBytes;
@@ -293,33 +292,16 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant_
       tcgen05_fence_after_sync();
       const uint32_t t = tmem + acc * BN + ((quarter * 32u) << 16);
       const int p0 = pt * kMxM + static_cast<int>(quarter) * 32;
-      if (SWAP) {
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(t + c, v);
-          tmem_ld_wait();
-          const int q0 = qt * BN + c;
-          const int n = p0 + static_cast<int>(lane);
-          if (n < a.p_rows) {
-            const long long at = b * a.stride_c + static_cast<long long>(q0) * a.ldc + n;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c + j < BN && q0 + j < a.q_rows) mx_store_one(a.C, a.out_type, at + j * a.ldc, __uint_as_float(v[j]));
-          }
-        }
-      } else {
-#pragma unroll 1
-        for (int c = 0; c < BN; c += 64) {
-          const int q0 = qt * BN + c;
-          if (q0 >= a.q_rows || p0 >= a.p_rows) break;  // warp-uniform
-          uint32_t v0[32], v1[32];
-          tmem_ld_32x32b_x32(t + c, v0);
-          tmem_ld_32x32b_x32(t + c + 32, v1);
-          tmem_ld_wait();
-          mx_store_rows(stage_mem, v0, v1, a.C, b * a.stride_c + static_cast<long long>(p0) * a.ldc + q0, a.ldc, a.out_type,
-                        a.p_rows - p0, a.q_rows - q0, a.vec_ok != 0);
-        }
+      for (int c = 0; c < BN; c += 64) {
+        const int q0 = qt * BN + c;
+        if (q0 >= a.q_rows || p0 >= a.p_rows) break;  // warp-uniform
+        uint32_t v0[32], v1[32];
+        tmem_ld_32x32b_x32(t + c, v0);
+        tmem_ld_32x32b_x32(t + c + 32, v1);
+        tmem_ld_wait();
+        mx_store_rows(stage_mem, v0, v1, a.C, b * a.stride_c + static_cast<long long>(p0) * a.ldc + q0, a.ldc, a.out_type,
+                      a.p_rows - p0, a.q_rows - q0, a.vec_ok != 0);
       }
       tcgen05_fence_before_sync();
       __syncwarp();

@@ -103,7 +103,7 @@ SIGNATURES = {
                                     _c_int, _c_int]),
     "fbmm_mx4_bmm": (_c_int, [_c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_int, _c_ll,
                               _c_ll, _c_int, _c_int, _c_int, _c_int]),
-    "fbmm_mx4_bmm_tensor_workspace_bytes": (_c_size, [_c_int] * 3),
+    "fbmm_mx4_bmm_tensor_workspace_bytes": (_c_size, [_c_int] * 5),
     "fbmm_mx4_bmm_tensor": (_c_int, [_c_ptr, _c_ptr, _c_int, _c_int, _c_ll, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_ptr,
                                      _c_int, _c_ll, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_size]),
     "fbmm_dense_bmm_x16": (_c_int, [_c_ptr] + _OPERANDS + [_c_int, _c_ptr, _c_ll, _c_ll] + [_c_int] * 4),

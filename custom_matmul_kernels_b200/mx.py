@@ -295,10 +295,10 @@ def _mx4_product(A, B: MXTensor, out_dtype: torch.dtype) -> torch.Tensor:
         C = A.new_empty((l, m, n), dtype=out_dtype)
         if C.numel():
             A3, layout, ld, step = _dense_layout(A3)
-            need = load_library().fbmm_mx4_bmm_tensor_workspace_bytes(l, m, k)
-            ws = A.new_empty(need, dtype=torch.uint8)
+            need = load_library().fbmm_mx4_bmm_tensor_workspace_bytes(l, m, n, k, layout)
+            ws = A.new_empty(need, dtype=torch.uint8) if need else None
             _call("fbmm_mx4_bmm_tensor", B.device, A3.data_ptr(), _DTYPES[A.dtype], layout, ld, step, *B._arguments(),
-                  C.data_ptr(), _code(out_dtype), n, m * n, l, m, n, k, ws.data_ptr(), need)
+                  C.data_ptr(), _code(out_dtype), n, m * n, l, m, n, k, ws.data_ptr() if need else None, need)
     return C[0] if two_d else C
 
 

@@ -207,6 +207,62 @@ def test_product_of_a_tensor(dev, l, m, n, k, dtype):
         assert torch.equal(MXBMMCUDA()(X[0].to(dev), B2), C[0])
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("m", [1, 3, 16, 17, 64])
+@pytest.mark.parametrize("l,n,k", [(1, 1, 1), (1, 130, 31), (1, 200, 256), (1, 100, 257), (2, 129, 2500), (1, 128, 9000), (40, 300, 600)])
+def test_product_few_rows(dev, l, m, n, k, dtype):
+    """One kernel for up to 64 rows: k split over clusters of 1 to 8 CTAs, ragged everywhere; the plain
+    form takes the values that the quantiser (tested above) gives."""
+    X = rnd((l, m, k), 31 + m, dtype).to(dev)
+    if m > 2:
+        X[0, 1] = 0
+    B, b = as_mx(n, k, 4, 9, dev, l, dim=-2, lo=119, hi=123)
+    a, b = MXQuantizeCUDA(4)(X).dequantize().double(), b.to(dev)
+    want, mag = (a @ b.transpose(1, 2)).cpu(), (a.abs() @ b.abs().transpose(1, 2)).cpu()
+    C = MXBMMCUDA()(X, B)
+    assert_sum_close(C, want, mag, k, dtype)
+    for _ in range(2):  # the order of the sums does not depend on timing
+        assert torch.equal(MXBMMCUDA()(X, B), C)
+    wide = torch.zeros((l, m, k + 3), dtype=dtype, device=dev)
+    wide[:, :, 1:k + 1] = X
+    assert torch.equal(MXBMMCUDA()(wide[:, :, 1:k + 1], B), C)  # rows at any alignment
+    one = MXTensor(B.codes[:1].expand(l, -1, -1), B.scales[:1].expand(l, -1, -1, -1), k=k, dim=-2)
+    assert torch.equal(MXBMMCUDA()(X, one)[0], C[0])
+    A4 = MXQuantizeCUDA(4)(X)  # the same kernel on codes
+    C4 = MXBMMCUDA(out_dtype=dtype)(A4, B)
+    assert_sum_close(C4, want, mag, k, dtype)
+    assert torch.equal(MXBMMCUDA(out_dtype=dtype)(A4, B), C4)
+    if k > 64:  # the other layout goes through the workspace
+        assert_sum_close(MXBMMCUDA()(X.transpose(1, 2).contiguous().transpose(1, 2), B), want, mag, k, dtype)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 64, 1 << 18), (1, 40, 1 << 19), (9, 19000, 1100), (64, 19000, 520)])
+def test_product_few_rows_long(dev, m, n, k):
+    """A k of which no CTA can keep its rows beside the ring, and more tiles than SMs."""
+    X = rnd((1, m, k), 3, BF16).to(dev)
+    g = torch.Generator("cuda").manual_seed(1)
+    W = MXQuantizeCUDA(4)(torch.randn((1, n, k), device=dev, generator=g, dtype=BF16)).mT
+    a, b = MXQuantizeCUDA(4)(X).dequantize(), W.dequantize()
+    want, mag = torch.zeros(1, m, n, dtype=torch.float64, device=dev), torch.zeros(1, m, n, dtype=torch.float64, device=dev)
+    for i in range(0, k, 1 << 16):
+        x, y = a[:, :, i:i + (1 << 16)].double(), b[:, i:i + (1 << 16)].double()
+        want += x @ y
+        mag += x.abs() @ y.abs()
+    assert_sum_close(MXBMMCUDA()(X, W), want.cpu(), mag.cpu(), k, BF16)
+
+
+def test_product_few_rows_non_finite(dev):
+    """A row with an infinity or a NaN is NaN in its whole row and leaves the others alone."""
+    X = rnd((1, 8, 3000), 3)
+    B, b = as_mx(200, 3000, 4, 9, dev, dim=-2, lo=119, hi=123)
+    clean = MXBMMCUDA()(X.to(dev), B)
+    X[0, 2, 2999], X[0, 5, 0] = float("inf"), float("nan")
+    C = MXBMMCUDA()(X.to(dev), B)
+    assert bool(torch.isnan(C[0, [2, 5]]).all())
+    keep = [0, 1, 3, 4, 6, 7]
+    assert torch.equal(C[0, keep], clean[0, keep])
+
+
 def test_product_shared_operands(dev):
     """Batch strides of 0 on either side give what copies give."""
     for m in (4, 150):
