@@ -19,7 +19,7 @@ int check_shape(int l, int rows, int k) {
   if (l <= 0 || rows <= 0 || k <= 0) return fail(FBMM_ERR_INVALID, "l, rows, k must be positive, got %d %d %d", l, rows, k);
   const long long groups = static_cast<long long>(l) * ((rows + 127) / 128) * ((k + 127) / 128);
   if (groups > 0x7fffffffLL) return fail(FBMM_ERR_INVALID, "matrix of %d x %d x %d is too large", l, rows, k);
-  if (k > (1 << 29)) return fail(FBMM_ERR_INVALID, "k = %d is too large", k);
+  if (k > (1 << 29) || rows > 0x7fffff00) return fail(FBMM_ERR_INVALID, "matrix of %d x %d is too large", rows, k);
   return FBMM_OK;
 }
 
@@ -330,7 +330,9 @@ int x16_product(cudaStream_t stream, const X16Side& x, const X16Side& y, int dty
                 long long stride_c, int l, int J, const char* xn, const char* yn) {
   int rc, sms;
   if (l <= 0 || x.rows <= 0 || y.rows <= 0 || J <= 0)
-    return fail(FBMM_ERR_INVALID, "all extents must be positive, got %d %d %d %d", l, x.rows, y.rows, J);
+    return fail(FBMM_ERR_INVALID, "l, m, n, k must be positive, got %d %d %d %d", l, x.rows, y.rows, J);
+  if (x.rows > 0x7fffff00 || y.rows > 0x7fffff00 || J > 0x7fffff00)
+    return fail(FBMM_ERR_INVALID, "product of %d x %d x %d is too large", x.rows, y.rows, J);
   if (dtype != FBMM_F16 && dtype != FBMM_BF16)
     return fail(FBMM_ERR_INVALID, "dtype must be FBMM_F16 (1) or FBMM_BF16 (2), got %d", dtype);
   if ((rc = check_x16_side(xn, x, J, l)) != FBMM_OK) return rc;

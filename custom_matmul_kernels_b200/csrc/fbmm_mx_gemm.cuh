@@ -134,25 +134,43 @@ __device__ __forceinline__ void mx_store_lines(uint8_t* stage, Word word, void* 
 #pragma unroll
   for (int c = 0; c < 8; ++c) st[lane * 8 + (c ^ (lane & 7))] = word(c);
   __syncwarp();
-  const int per = 16 / size;  // elements of a piece
-  const int c = lane & 7;
+  if (vec) {
+    const int c = lane & 7, per = 16 / size;  // piece of a row, its elements
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + (lane >> 3);
-    const uint4 x = st[r * 8 + (c ^ (r & 7))];
-    if (r < rows) {
-      uint8_t* at = static_cast<uint8_t*>(C) + (c0 + r * ldc) * size + c * 16;
-      if (vec && (c + 1) * per <= cols) {
-        *reinterpret_cast<uint4*>(at) = x;
-      } else {
-        const uint32_t e[4] = {x.x, x.y, x.z, x.w};
-        if (size == 4) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) if (c * 4 + j < cols) reinterpret_cast<uint32_t*>(at)[j] = e[j];
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (lane >> 3);
+      const uint4 x = st[r * 8 + (c ^ (r & 7))];
+      if (r < rows) {
+        uint8_t* at = static_cast<uint8_t*>(C) + (c0 + r * ldc) * size + c * 16;
+        if ((c + 1) * per <= cols) {
+          *reinterpret_cast<uint4*>(at) = x;
         } else {
+          const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+          if (size == 4) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (c * 8 + j < cols) reinterpret_cast<uint16_t*>(at)[j] = static_cast<uint16_t>(e[j >> 1] >> (16 * (j & 1)));
+            for (int j = 0; j < 4; ++j) if (c * 4 + j < cols) reinterpret_cast<uint32_t*>(at)[j] = e[j];
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (c * 8 + j < cols) reinterpret_cast<uint16_t*>(at)[j] = static_cast<uint16_t>(e[j >> 1] >> (16 * (j & 1)));
+          }
+        }
+      }
+    }
+  } else {  // rows at any alignment: neighbouring lanes store neighbouring elements of one row
+    const int end = rows < 32 ? rows : 32;
+#pragma unroll 4
+    for (int r = 0; r < end; ++r) {
+      uint8_t* row = static_cast<uint8_t*>(C) + (c0 + r * ldc) * size;
+      if (size == 4) {
+        const uint32_t x = reinterpret_cast<const uint32_t*>(st + r * 8 + ((lane >> 2) ^ (r & 7)))[lane & 3];
+        if (lane < cols) reinterpret_cast<uint32_t*>(row)[lane] = x;
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int e = h * 32 + lane;
+          const uint16_t x = reinterpret_cast<const uint16_t*>(st + r * 8 + ((e >> 3) ^ (r & 7)))[e & 7];
+          if (e < cols) reinterpret_cast<uint16_t*>(row)[e] = x;
         }
       }
     }
@@ -292,6 +310,13 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant_
       tcgen05_fence_after_sync();
       const uint32_t t = tmem + acc * BN + ((quarter * 32u) << 16);
       const int p0 = pt * kMxM + static_cast<int>(quarter) * 32;
+      bool held = true;  // released with the last load, before the stores behind it
+      auto release = [&]() {
+        tcgen05_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->acc_empty[acc]);
+        held = false;
+      };
 #pragma unroll 1
       for (int c = 0; c < BN; c += 64) {
         const int q0 = qt * BN + c;
@@ -300,12 +325,11 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant_
         tmem_ld_32x32b_x32(t + c, v0);
         tmem_ld_32x32b_x32(t + c + 32, v1);
         tmem_ld_wait();
+        if (c + 64 >= BN || q0 + 64 >= a.q_rows) release();
         mx_store_rows(stage_mem, v0, v1, a.C, b * a.stride_c + static_cast<long long>(p0) * a.ldc + q0, a.ldc, a.out_type,
                       a.p_rows - p0, a.q_rows - q0, a.vec_ok != 0);
       }
-      tcgen05_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->acc_empty[acc]);
+      if (held) release();
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
   }

@@ -95,9 +95,9 @@ __device__ __forceinline__ uint64_t x16_desc(uint32_t smem_addr, bool mn_major) 
          (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
 
-// Reports to the pair's issuing CTA that this warp's values lie in THIS CTA's shared memory, behind its
-// proxy fence, where only this CTA's tensor core reads them. So the release covers this CTA; with
-// one at cluster scope the arrival itself took about 1400 cycles beside 16 writing warps, twice the expansion
+// Reports to the pair's issuing CTA what concerns only THIS CTA's memories: that this warp's values lie in its
+// shared memory, behind their proxy fence, where its own tensor core reads them, or that the warp has
+// read its accumulators. So the release covers this CTA; with one at cluster scope the arrival itself took about 1400 cycles beside 16 writing warps, twice the expansion
 // (8-bit gradient of weights at 4096^3: 145 us with it, 115 us without).
 __device__ __forceinline__ void mbar_arrive_values(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
@@ -200,12 +200,6 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   auto commit = [&](uint64_t* bar) {
     if (PAIR) { umma_commit_pair(bars0 + off(bar)); umma_commit_pair(bars1 + off(bar)); }
     else umma_commit(bar);
-  };
-  auto arrive_leader = [&](uint64_t* bar) {  // one arrival per warp
-    __syncwarp();
-    if (lane == 0) {
-      if (PAIR && rank != 0) mbar_arrive_cluster(bars0 + off(bar)); else mbar_arrive(bar);
-    }
   };
 
   const int jblocks = (a.J + kX16J - 1) / kX16J;
@@ -336,6 +330,13 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       tcgen05_fence_after_sync();
       const uint32_t t = tmem + acc * 256 + ((quarter * 32u) << 16);
       const int x0 = xt * kTile + static_cast<int>(rank) * 128 + static_cast<int>(quarter) * 32;
+      bool held = true;  // released with the last load, before the stores behind it
+      auto release = [&]() {
+        tcgen05_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_values(bars0 + off(&bars->acc_empty[acc]));
+        held = false;
+      };
 #pragma unroll 1
       for (int c = 0; c < kTile; c += 64) {
         const int y0 = yt * kTile + c;
@@ -344,6 +345,7 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         tmem_ld_32x32b_x32(t + c, v0);
         tmem_ld_32x32b_x32(t + c + 32, v1);
         tmem_ld_wait();
+        if (c + 64 >= kTile || y0 + 64 >= a.y.rows) release();
         mx_store_lines(stage_mem, [&](int i) {
           const uint32_t (&v)[32] = i < 4 ? v0 : v1;
           uint32_t p[4];
@@ -354,8 +356,7 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }, a.C, b * a.stride_c + static_cast<long long>(x0) * a.ldc + y0, a.ldc, 2, a.x.rows - x0, a.y.rows - y0,
                        a.vec_ok != 0);
       }
-      tcgen05_fence_before_sync();
-      arrive_leader(&bars->acc_empty[acc]);
+      if (held) release();
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
   }

@@ -32,10 +32,19 @@ except AttributeError:
         return torch.cuda.current_stream(index).cuda_stream
 
 
+_functions = {}
+
+
+def _function(name: str):
+    """The library's entry point `name` (load_library raises where the library is not built)."""
+    fn = _functions[name] = getattr(load_library(), name)
+    return fn
+
+
 def _call(name: str, device: torch.device, *args) -> None:
     """One library call on the stream that is current on `device`; the device is only switched when
     it is not the current one (the switch costs more than the call)."""
-    fn = getattr(load_library(), name)
+    fn = _functions.get(name) or _function(name)
     index = device.index
     if torch.cuda.current_device() == index:
         rc = fn(_raw_stream(index), *args)
@@ -295,7 +304,8 @@ def _mx4_product(A, B: MXTensor, out_dtype: torch.dtype) -> torch.Tensor:
         C = A.new_empty((l, m, n), dtype=out_dtype)
         if C.numel():
             A3, layout, ld, step = _dense_layout(A3)
-            need = load_library().fbmm_mx4_bmm_tensor_workspace_bytes(l, m, n, k, layout)
+            query = "fbmm_mx4_bmm_tensor_workspace_bytes"
+            need = (_functions.get(query) or _function(query))(l, m, n, k, layout)
             ws = A.new_empty(need, dtype=torch.uint8) if need else None
             _call("fbmm_mx4_bmm_tensor", B.device, A3.data_ptr(), _DTYPES[A.dtype], layout, ld, step, *B._arguments(),
                   C.data_ptr(), _code(out_dtype), n, m * n, l, m, n, k, ws.data_ptr() if need else None, need)
@@ -317,15 +327,16 @@ class _MX4Product(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, A, B, out_dtype):
-        ctx.B, ctx.dtype = B, A.dtype
+        ctx.k, ctx.two_d, ctx.dtype = B.k, B.two_d, A.dtype
         ctx.save_for_backward(B.codes, B.scales)
         return _mx4_product(A, B, out_dtype)
 
     @staticmethod
     @_once
     def backward(ctx, dC):
-        ctx.saved_tensors  # raises if the weights were written to since the forward pass
-        dC, BT = dC.to(ctx.dtype), ctx.B.mT
+        codes, scales = ctx.saved_tensors
+        BT = MXTensor._of(codes, scales, 4, ctx.k, -1, ctx.two_d)  # [l, n, k]
+        dC = dC.to(ctx.dtype)
         if ctx.dtype in _X16:
             return MXDenseBMMCUDA()(dC, BT), None, None
         return BMMCUDA()(dC, BT.dequantize(ctx.dtype)), None, None
@@ -368,30 +379,31 @@ class _CheckpointProduct(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, A, B):
-        x16 = A.dtype in _X16
-        C = _dense_bmm(A, B) if x16 else BMMCUDA()(A, B)
+        C = _dense_bmm(A, B) if A.dtype in _X16 else BMMCUDA()(A, B)
         need_a, need_b = ctx.needs_input_grad
-        ctx.q = MXQuantizeCUDA(8)(A) if need_b else None
+        ctx.k = A.shape[2]
         ctx.b_transposed = B.stride(2) != 1 and B.stride(1) == 1
-        ctx.save_for_backward(B if need_a else None)
+        q = MXQuantizeCUDA(8)(A) if need_b else None
+        ctx.save_for_backward(B if need_a else None, q and q.codes, q and q.scales)
         return C
 
     @staticmethod
     @_once
     def backward(ctx, dC):
-        need_a, need_b = ctx.needs_input_grad
+        B, codes, scales = ctx.saved_tensors
         x16 = dC.dtype in _X16
         dA = dB = None
-        if need_a:
-            BT = ctx.saved_tensors[0].transpose(1, 2)
+        if B is not None:
+            BT = B.transpose(1, 2)
             dA = _dense_bmm(dC, BT) if x16 else BMMCUDA()(dC, BT)
-        if need_b:
+        if codes is not None:
+            A8 = MXTensor._of(codes, scales, 8, ctx.k, -1, False)
             if not x16:
-                dB = BMMCUDA()(ctx.q.mT.dequantize(dC.dtype), dC)
+                dB = BMMCUDA()(A8.mT.dequantize(dC.dtype), dC)
             elif ctx.b_transposed:  # in B's own storage order
-                dB = MXDenseBMMCUDA()(dC.transpose(1, 2), ctx.q).transpose(1, 2)
+                dB = MXDenseBMMCUDA()(dC.transpose(1, 2), A8).transpose(1, 2)
             else:
-                dB = MXDenseBMMCUDA()(ctx.q.mT, dC)
+                dB = MXDenseBMMCUDA()(A8.mT, dC)
         return dA, dB
 
 

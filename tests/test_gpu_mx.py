@@ -381,3 +381,220 @@ def test_checkpoint_gradients(dev, l, m, n, k, dtype):
     assert_sum_close(Ct.detach(), a @ b, a.abs() @ b.abs(), f * k, dtype)
     assert_sum_close(dA2, d @ b.transpose(1, 2), d.abs() @ b.abs().transpose(1, 2), f * n, dtype)
     assert_sum_close(dW, d.transpose(1, 2) @ a8, d.abs().transpose(1, 2) @ a8.abs(), f * m, dtype)
+
+
+def test_checkpoint_keeps_eight_bits(dev):
+    """What waits for the backward pass: B, and A at 33/32 byte per element; released by it."""
+    A = torch.randn(1, 512, 1024, device=dev, dtype=BF16).requires_grad_()
+    B = torch.randn(1, 1024, 256, device=dev, dtype=BF16).requires_grad_()
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        C = CheckpointBMMCUDA()(A, B)
+    assert sum(t.numel() for t in kept if t.dtype == torch.uint8) == 512 * 1024 * 33 // 32
+    assert [t.shape for t in kept if t.dtype != torch.uint8] == [B.shape]
+    C.sum().backward()  # an expanded gradient
+    with pytest.raises(RuntimeError, match="second time"):
+        C.sum().backward()
+
+
+@pytest.mark.parametrize("need", ["A", "B"])
+def test_checkpoint_one_gradient(dev, need):
+    A, B = rnd((2, 70, 96), 1, BF16, 0.5).to(dev), rnd((2, 96, 64), 2, BF16, 0.5).to(dev)
+    both = [t.clone().requires_grad_() for t in (A, B)]
+    want = torch.autograd.grad(CheckpointBMMCUDA()(*both).square().sum(), both)
+    one = [A.clone().requires_grad_(need == "A"), B.clone().requires_grad_(need == "B")]
+    C = CheckpointBMMCUDA()(*one)
+    got, = torch.autograd.grad(C.square().sum(), [t for t in one if t.requires_grad])
+    assert torch.equal(got, want[need == "B"])
+    with torch.no_grad():
+        assert not CheckpointBMMCUDA()(*both).requires_grad
+
+
+def test_checkpoint_broadcast_and_2d(dev):
+    """One B for every batch: its gradient is the sum over the batches; 2-D operands."""
+    A, B = rnd((3, 40, 64), 1, BF16, 0.5).to(dev), rnd((64, 48), 2, BF16, 0.5).to(dev).requires_grad_()
+    dC = rnd((3, 40, 48), 3, BF16, 0.5).to(dev)
+    C = CheckpointBMMCUDA()(A, B.expand(3, -1, -1))
+    dB, = torch.autograd.grad(C, B, dC)
+    each = []
+    for i in range(3):
+        Ci = CheckpointBMMCUDA()(A[i], B)
+        assert torch.equal(Ci, C[i])
+        each.append(torch.autograd.grad(Ci, B, dC[i])[0])
+    want = torch.stack(each).double().sum(0)
+    # three results of half a step each, and the sum's own rounding
+    tol = torch.stack(each).double().abs().sum(0) * torch.finfo(BF16).eps / 2 + want.abs() * torch.finfo(BF16).eps
+    assert bool(((dB.double() - want).abs() <= tol + 1e-6).all())
+
+
+@pytest.mark.parametrize("kind", ["checkpoint", "frozen"])
+def test_gradient_by_differences(dev, kind):
+    """L = sum(C * D) is linear in each operand, so (L(x + h) - L(x - h)) / 2h is its derivative; operands
+    whose quantisation is exact (small integers in blocks with a 4 or a 448) and fp32 products."""
+    g = torch.Generator().manual_seed(5)
+    A = torch.randint(-2, 3, (1, 6, 64), generator=g).float()
+    D = torch.randint(-3, 4, (1, 6, 40), generator=g).float()
+    if kind == "checkpoint":
+        B = torch.randint(-2, 3, (1, 64, 40), generator=g).float()
+        Ad, Bd = A.to(dev).requires_grad_(), B.to(dev).requires_grad_()
+        dA, dB = torch.autograd.grad((CheckpointBMMCUDA()(Ad, Bd) * D.to(dev)).sum(), (Ad, Bd))
+        run = lambda a, b: float((CheckpointBMMCUDA()(a.to(dev), b.to(dev)).cpu() * D).double().sum())  # noqa: E731
+        for i, j in ((0, 0), (3, 17), (5, 63)):
+            h = torch.zeros_like(A)
+            h[0, i, j] = 1.0
+            assert (run(A + h, B) - run(A - h, B)) / 2 == float(dA[0, i, j])
+        for i, j in ((0, 0), (31, 20), (63, 39)):
+            h = torch.zeros_like(B)
+            h[0, i, j] = 1.0
+            assert (run(A, B + h) - run(A, B - h)) / 2 == float(dB[0, i, j])
+    else:
+        A[:, :, ::32] = 4.0  # every block's scale stays 1, and 0, 1, 2, 3 are elements
+        W, _ = as_mx(40, 64, 4, 3, dev, dim=-2, lo=127, hi=128)
+        Ad = A.to(dev).requires_grad_()
+        dA, = torch.autograd.grad((MXBMMCUDA()(Ad, W) * D.to(dev)).sum(), Ad)
+        run = lambda a: float((MXBMMCUDA()(a.to(dev), W).cpu() * D).double().sum())  # noqa: E731
+        for i, j in ((0, 1), (3, 17), (5, 63)):
+            h = torch.zeros_like(A)
+            h[0, i, j] = 1.0
+            assert (run(A + h) - run(A - h)) / 2 == float(dA[0, i, j])
+
+
+def test_written_weights_are_noticed(dev):
+    W, _ = as_mx(40, 64, 4, 3, dev, dim=-2)
+    A = torch.randn(1, 4, 64, device=dev, requires_grad=True)
+    C = MXBMMCUDA()(A, W)
+    W.codes.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(C.sum(), A)
+
+
+def test_higher_order_is_refused(dev):
+    A = torch.randn(1, 4, 64, device=dev, requires_grad=True)
+    B = torch.randn(1, 64, 8, device=dev, requires_grad=True)
+    g, = torch.autograd.grad(CheckpointBMMCUDA()(A, B).square().sum(), A, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
+# ---- as they are used together ---------------------------------------------------------------------
+def test_training_step_captured(dev):
+    """Two projections, one over frozen 4-bit weights and one with its activations in 8 bits, forward
+    and backward in one CUDA graph: replays follow the inputs, and equal the eager step bit for bit."""
+    W = MXQuantizeCUDA(4)(rnd((1, 192, 256), 4, BF16, 0.2).to(dev), dim=-2)
+    A, B = rnd((1, 300, 192), 1, BF16, 0.5).to(dev).requires_grad_(), rnd((1, 256, 128), 2, BF16, 0.2).to(dev).requires_grad_()
+    dC = rnd((1, 300, 128), 3, BF16, 0.2).to(dev)
+
+    def step(a, b):
+        H = MXBMMCUDA()(a, W)
+        C = CheckpointBMMCUDA()(H, b)
+        return (C.detach(),) + torch.autograd.grad(C, (a, b), dC)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(A, B)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(A, B)
+    for seed in (11, 12):
+        with torch.no_grad():
+            A.copy_(rnd((1, 300, 192), seed, BF16, 0.5))
+            B.copy_(rnd((1, 256, 128), seed + 100, BF16, 0.2))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        want = step(A.detach().clone().requires_grad_(), B.detach().clone().requires_grad_())
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_decoding_captured_on_another_stream(dev):
+    """A decoding step (few rows, fused) and a longer product share weights on two streams and in two graphs."""
+    W = MXQuantizeCUDA(4)(rnd((1, 512, 640), 4, BF16, 0.2).to(dev), dim=-2)
+    x, y = rnd((1, 3, 512), 1, BF16).to(dev), rnd((1, 200, 512), 2, BF16).to(dev)
+    want = MXBMMCUDA()(x, W), MXBMMCUDA()(y, W)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for t in (x, y, x, y):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(MXBMMCUDA()(t, W))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for i, o in enumerate(outs):
+        assert torch.equal(o, want[i % 2])
+
+
+def test_library_reports_no_trouble(dev, lib):
+    assert lib.fbmm_check(None) == 0, lib.fbmm_last_error()
+
+
+# ---- refusals ----------------------------------------------------------------------------------------
+def test_refusals(dev):
+    X = torch.randn(2, 8, 64, device=dev)
+    W = MXQuantizeCUDA(4)(torch.randn(2, 64, 16, device=dev), dim=-2)
+    P = MXBMMCUDA()
+    with pytest.raises(ValueError, match="batch sizes"):
+        P(X[:1], W)
+    with pytest.raises(ValueError, match="inner dimensions"):
+        P(X[:, :, :32], W)
+    with pytest.raises(ValueError, match="same number of dimensions"):
+        P(X[0], W)
+    with pytest.raises(ValueError, match="dim=-2"):
+        P(X[:, :, :16], W.mT)
+    with pytest.raises(ValueError, match="4-bit"):
+        P(X, MXQuantizeCUDA(8)(torch.randn(2, 64, 16, device=dev), dim=-2))
+    with pytest.raises(ValueError, match="A must hold"):
+        P(MXQuantizeCUDA(8)(X), W)
+    with pytest.raises(TypeError):
+        P(X, torch.randn(2, 64, 16, device=dev))
+    with pytest.raises(TypeError):
+        P(X.double(), W)
+    with pytest.raises(ValueError, match="CUDA"):
+        P(X.cpu(), W)
+    D = MXDenseBMMCUDA()
+    with pytest.raises(TypeError):
+        D(X.half(), X.half())
+    with pytest.raises(TypeError):
+        D(torch.randn(2, 8, 16, device=dev), W.mT)  # fp32
+    with pytest.raises(ValueError, match="own axis"):
+        D(X.half(), W)
+    with pytest.raises(ValueError, match="2d or 3d"):
+        MXQuantizeCUDA(4)(X[0, 0])
+    with pytest.raises(ValueError, match="empty"):
+        MXQuantizeCUDA(4)(X[:, :, :0])
+    with pytest.raises(TypeError):
+        MXQuantizeCUDA(4)(X.double())
+    with pytest.raises(TypeError):
+        W.dequantize(torch.float64)
+    with pytest.raises(ValueError, match="what k"):
+        MXTensor(W.codes, W.scales, k=65)
+    with pytest.raises(ValueError, match="scales have shape"):
+        MXTensor(W.codes, W.scales[:, :, :, :256], k=64)
+    with pytest.raises(TypeError):
+        MXTensor(W.codes.int(), W.scales, k=64)
+    with pytest.raises(TypeError):
+        CheckpointBMMCUDA()(X.double().requires_grad_(), X.double().transpose(1, 2))
+    with pytest.raises(ValueError, match="inner dimensions"):
+        CheckpointBMMCUDA()(X.requires_grad_(), X)
+
+
+def test_unaligned_storage_is_copied(dev):
+    """Codes and scales at odd addresses or batch strides give what aligned ones give."""
+    B, _ = as_mx(40, 96, 4, 3, dev, 2, dim=-2)
+    A = torch.randn(2, 5, 96, device=dev)
+    want = MXBMMCUDA()(A, B)
+    raw = torch.empty(B.codes.numel() + 1, dtype=torch.uint8, device=dev)
+    raw[1:] = B.codes.reshape(-1)
+    odd = MXTensor(raw[1:].view_as(B.codes), B.scales, k=96, dim=-2)
+    assert torch.equal(MXBMMCUDA()(A, odd), want)
+    wide = torch.zeros(2, 41, B.codes.shape[2] + 1, dtype=torch.uint8, device=dev)
+    wide[:, :40, :-1] = B.codes
+    assert torch.equal(MXBMMCUDA()(A, MXTensor(wide[:, :40, :-1], B.scales, k=96, dim=-2)), want)
