@@ -41,15 +41,14 @@ def _function(name: str):
     return fn
 
 
-def _call(name: str, device: torch.device, *args) -> None:
-    """One library call on the stream that is current on `device`; the device is only switched when
-    it is not the current one (the switch costs more than the call)."""
+def _call(name: str, index: int, *args) -> None:
+    """One library call on the stream that is current on device `index`; the device is only switched
+    when it is not the current one (the switch costs more than the call)."""
     fn = _functions.get(name) or _function(name)
-    index = device.index
     if torch.cuda.current_device() == index:
         rc = fn(_raw_stream(index), *args)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             rc = fn(_raw_stream(index), *args)
     if rc:
         check(rc)
@@ -93,7 +92,9 @@ class MXTensor:
     serves every batch with one matrix. 2-D codes with 3-D scales make a 2-D matrix. The codes
     behind k must be zero, as ``MXQuantizeCUDA`` leaves them."""
 
-    __slots__ = ("codes", "scales", "bits", "k", "dim", "two_d")
+    # Storage is either the caller's two tensors or one buffer (codes, then scales), of which `codes`
+    # and `scales` are views made when asked for: one allocation per quantisation.
+    __slots__ = ("_buffer", "_codes", "_scales", "_l", "rows", "bits", "k", "dim", "two_d")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, bits: int = 4, k: int | None = None, dim: int = -1):
         if bits not in (4, 8):
@@ -105,7 +106,7 @@ class MXTensor:
         two_d = codes.dim() == 2
         if codes.dim() not in (2, 3) or scales.dim() != codes.dim() + 1:
             raise ValueError("codes must be 2d or 3d and scales one dimension more")
-        if codes.device.type != "cuda" or scales.device != codes.device:
+        if not codes.is_cuda or not scales.is_cuda or codes.get_device() != scales.get_device():
             raise ValueError("codes and scales must be CUDA tensors on one device")
         if two_d:
             codes, scales = codes[None], scales[None]
@@ -115,12 +116,13 @@ class MXTensor:
         blocks = (k + BLOCK - 1) // BLOCK
         if k <= 0 or pitch != blocks * (4 * bits):
             raise ValueError(f"codes have {pitch} bytes per row, which is not what k = {k} takes at {bits} bits")
-        groups = (rows + 127) // 128, (blocks + 3) // 4
-        if scales.shape != (l, *groups, 512):
-            raise ValueError(f"scales have shape {tuple(scales.shape)}, expected {(l, *groups, 512)}")
-        self.codes = self._addressable(codes, rows * pitch)
-        self.scales = self._addressable(scales, groups[0] * groups[1] * 512)
-        self.bits, self.k, self.dim, self.two_d = bits, k, dim, two_d
+        want = (l, (rows + 127) // 128, (blocks + 3) // 4, 512)
+        if scales.shape != want:
+            raise ValueError(f"scales have shape {tuple(scales.shape)}, expected {want}")
+        self._buffer = None
+        self._codes = self._addressable(codes, rows * pitch)
+        self._scales = self._addressable(scales, want[1] * want[2] * 512)
+        self._l, self.rows, self.bits, self.k, self.dim, self.two_d = l, rows, bits, k, dim, two_d
 
     @staticmethod
     def _addressable(t: torch.Tensor, per_batch: int) -> torch.Tensor:
@@ -133,45 +135,72 @@ class MXTensor:
             return t
         return t.clone(memory_format=torch.contiguous_format)
 
-    @property
-    def device(self) -> torch.device:
-        return self.codes.device
+    @classmethod
+    def _around(cls, tensors, l, rows, k, bits, dim, two_d) -> "MXTensor":
+        """One made of `_tensors()` of another (a buffer, or codes and scales)."""
+        t = object.__new__(cls)
+        if len(tensors) == 1:
+            t._buffer, t._codes, t._scales = tensors[0], None, None
+        else:
+            t._buffer, (t._codes, t._scales) = None, tensors
+        t._l, t.rows, t.bits, t.k, t.dim, t.two_d = l, rows, bits, k, dim, two_d
+        return t
+
+    def _tensors(self) -> tuple:
+        return (self._codes, self._scales) if self._buffer is None else (self._buffer,)
+
+    def _sizes(self):
+        """Bytes per batch of codes and scales."""
+        blocks = (self.k + BLOCK - 1) // BLOCK
+        return self.rows * blocks * (4 * self.bits), (self.rows + 127) // 128 * ((blocks + 3) // 4) * 512
 
     @property
-    def rows(self) -> int:
-        return self.codes.shape[1]
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            per, _ = self._sizes()
+            self._codes = self._buffer[:self._l * per].view(self._l, self.rows, (self.k + BLOCK - 1) // BLOCK * (4 * self.bits))
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            per, _ = self._sizes()
+            self._scales = self._buffer[self._l * per:].view(self._l, (self.rows + 127) // 128, (self.k + 127) // 128, 512)
+        return self._scales
+
+    @property
+    def device(self) -> torch.device:
+        return self._tensors()[0].device
 
     @property
     def shape(self) -> tuple:
-        l, rows, _ = self.codes.shape
-        s = (rows, self.k) if self.dim == -1 else (self.k, rows)
-        return s if self.two_d else (l,) + s
+        s = (self.rows, self.k) if self.dim == -1 else (self.k, self.rows)
+        return s if self.two_d else (self._l,) + s
 
     @property
     def mT(self) -> "MXTensor":
         """The transposed matrix: the same storage with the blocks along the other axis."""
-        return self._of(self.codes, self.scales, self.bits, self.k, -3 - self.dim, self.two_d)
-
-    @classmethod
-    def _of(cls, codes, scales, bits, k, dim, two_d) -> "MXTensor":
-        t = object.__new__(cls)
-        t.codes, t.scales, t.bits, t.k, t.dim, t.two_d = codes, scales, bits, k, dim, two_d
-        return t
+        return self._around(self._tensors(), self._l, self.rows, self.k, self.bits, -3 - self.dim, self.two_d)
 
     def _arguments(self):
         """codes, their batch stride, scales, their batch stride (bytes; 0: one matrix for all)."""
-        return self.codes.data_ptr(), self.codes.stride(0), self.scales.data_ptr(), self.scales.stride(0)
+        if self._buffer is None:
+            return self._codes.data_ptr(), self._codes.stride(0), self._scales.data_ptr(), self._scales.stride(0)
+        per, groups = self._sizes()
+        at = self._buffer.data_ptr()
+        return at, per, at + self._l * per, groups  # a row of codes is a multiple of 16 bytes
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """Element times scale, rounded once to `dtype`; with dim=-2 a transposed view of
         k-contiguous storage."""
         code = _code(dtype)
-        l, rows, _ = self.codes.shape
-        out = self.codes.new_empty((l, rows, self.k), dtype=dtype)
+        l, rows, k = self._l, self.rows, self.k
+        t = self._tensors()[0]
+        out = t.new_empty((l, rows, k), dtype=dtype)
         if l and rows:
             codes, sc, scales, ss = self._arguments()
-            _call("fbmm_mx_dequantize", self.device, codes, sc, scales, ss, self.bits, out.data_ptr(), code, self.k,
-                  rows * self.k, l, rows, self.k)
+            _call("fbmm_mx_dequantize", t.get_device(), codes, sc, scales, ss, self.bits, out.data_ptr(), code, k, rows * k,
+                  l, rows, k)
         if self.dim == -2:
             out = out.transpose(1, 2)
         return out[0] if self.two_d else out
@@ -205,7 +234,7 @@ class MXQuantizeCUDA(CustomKernel):
         if X.dim() not in (2, 3):
             raise ValueError("X needs to be 2d or 3d")
         dtype = _code(X.dtype)
-        if X.device.type != "cuda":
+        if not X.is_cuda:
             raise ValueError("X must be a CUDA tensor")
         X3 = X[None] if two_d else X
         if dim == -2:
@@ -213,13 +242,15 @@ class MXQuantizeCUDA(CustomKernel):
         l, rows, k = X3.shape
         if k == 0:
             raise ValueError("the axis the blocks run along is empty")
-        codes = X.new_empty((l, rows, (k + BLOCK - 1) // BLOCK * (4 * self.bits)), dtype=torch.uint8)
-        scales = X.new_empty((l, (rows + 127) // 128, (k + 127) // 128, 512), dtype=torch.uint8)
+        q = MXTensor._around((None,), l, rows, k, self.bits, dim, two_d)
+        codes, scales = q._sizes()
+        q._buffer = X.new_empty(l * (codes + scales), dtype=torch.uint8)
         if l and rows:
             X3, layout, ld, step = _dense_layout(X3)
-            _call("fbmm_mx_quantize", X.device, X3.data_ptr(), dtype, layout, ld, step, self.bits, codes.data_ptr(),
-                  scales.data_ptr(), l, rows, k)
-        return MXTensor._of(codes, scales, self.bits, k, dim, two_d)
+            at = q._buffer.data_ptr()
+            _call("fbmm_mx_quantize", X.get_device(), X3.data_ptr(), dtype, layout, ld, step, self.bits, at, at + l * codes, l,
+                  rows, k)
+        return q
 
 
 def _check_product(A, B) -> bool:
@@ -233,11 +264,17 @@ def _check_product(A, B) -> bool:
         raise ValueError(f"batch sizes differ: {a[0]} vs {b[0]}")
     if a[-1] != b[-2]:
         raise ValueError(f"inner dimensions differ: A {tuple(a)} B {tuple(b)}")
-    if A.device.type != "cuda":
-        raise ValueError("A and B must be CUDA tensors")
-    if A.device != B.device:
+    for X in (A, B):
+        if isinstance(X, torch.Tensor) and not X.is_cuda:
+            raise ValueError("A and B must be CUDA tensors")
+    if _index(A) != _index(B):
         raise ValueError("A and B must be on the same device")
     return len(a) == 2
+
+
+def _index(X) -> int:
+    """Device index of a tensor or MXTensor."""
+    return (X if isinstance(X, torch.Tensor) else X._tensors()[0]).get_device()
 
 
 def _dense_bmm(A: torch.Tensor, B: torch.Tensor) -> torch.Tensor:
@@ -248,7 +285,7 @@ def _dense_bmm(A: torch.Tensor, B: torch.Tensor) -> torch.Tensor:
     if l and m and n:
         a, la, lda, sa = _aligned_layout(A)
         b, lb, ldb, sb = _aligned_layout(B)
-        _call("fbmm_dense_bmm_x16", A.device, a.data_ptr(), la, lda, sa, b.data_ptr(), lb, ldb, sb, _DTYPES[A.dtype],
+        _call("fbmm_dense_bmm_x16", A.get_device(), a.data_ptr(), la, lda, sa, b.data_ptr(), lb, ldb, sb, _DTYPES[A.dtype],
               C.data_ptr(), n, m * n, l, m, n, k)
     return C
 
@@ -278,13 +315,13 @@ class MXDenseBMMCUDA(CustomKernel):
             C.zero_()
         elif mx is B:
             d, letter, ld, step = _aligned_layout(D)
-            _call("fbmm_dense_mx_bmm_x16", D.device, d.data_ptr(), letter, ld, step, _DTYPES[D.dtype], *mx._arguments(),
+            _call("fbmm_dense_mx_bmm_x16", D.get_device(), d.data_ptr(), letter, ld, step, _DTYPES[D.dtype], *mx._arguments(),
                   mx.bits, C.data_ptr(), n, m * n, l, m, n, k)
         else:
             d, letter, ld, step = _aligned_layout(D)
             if letter != _N:
                 d, letter, ld, step = _aligned_layout(D.contiguous())
-            _call("fbmm_mx_dense_bmm_x16", D.device, *mx._arguments(), mx.bits, d.data_ptr(), ld, step, _DTYPES[D.dtype],
+            _call("fbmm_mx_dense_bmm_x16", D.get_device(), *mx._arguments(), mx.bits, d.data_ptr(), ld, step, _DTYPES[D.dtype],
                   C.data_ptr(), n, m * n, l, m, n, k)
         return C[0] if two_d else C
 
@@ -293,22 +330,22 @@ def _mx4_product(A, B: MXTensor, out_dtype: torch.dtype) -> torch.Tensor:
     two_d = B.two_d
     n, k = B.rows, B.k
     if isinstance(A, MXTensor):
-        l, m, _ = A.codes.shape
-        C = A.codes.new_empty((l, m, n), dtype=out_dtype)
-        if C.numel():
-            _call("fbmm_mx4_bmm", B.device, *A._arguments(), *B._arguments(), C.data_ptr(), _code(out_dtype), n, m * n, l, m,
-                  n, k)
+        l, m, t = A._l, A.rows, A._tensors()[0]
     else:
-        A3 = A[None] if two_d else A
-        l, m, _ = A3.shape
-        C = A.new_empty((l, m, n), dtype=out_dtype)
-        if C.numel():
-            A3, layout, ld, step = _dense_layout(A3)
+        t = A[None] if two_d else A
+        l, m, _ = t.shape
+    C = t.new_empty((l, m, n), dtype=out_dtype)
+    if l and m and n:
+        result = C.data_ptr(), _DTYPES[out_dtype], n, m * n, l, m, n, k
+        if isinstance(A, MXTensor):
+            _call("fbmm_mx4_bmm", t.get_device(), *A._arguments(), *B._arguments(), *result)
+        else:
+            t, layout, ld, step = _dense_layout(t)
             query = "fbmm_mx4_bmm_tensor_workspace_bytes"
             need = (_functions.get(query) or _function(query))(l, m, n, k, layout)
-            ws = A.new_empty(need, dtype=torch.uint8) if need else None
-            _call("fbmm_mx4_bmm_tensor", B.device, A3.data_ptr(), _DTYPES[A.dtype], layout, ld, step, *B._arguments(),
-                  C.data_ptr(), _code(out_dtype), n, m * n, l, m, n, k, ws.data_ptr() if need else None, need)
+            ws = t.new_empty(need, dtype=torch.uint8) if need else None
+            _call("fbmm_mx4_bmm_tensor", t.get_device(), t.data_ptr(), _DTYPES[t.dtype], layout, ld, step, *B._arguments(),
+                  *result, ws.data_ptr() if need else None, need)
     return C[0] if two_d else C
 
 
@@ -327,15 +364,14 @@ class _MX4Product(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, A, B, out_dtype):
-        ctx.k, ctx.two_d, ctx.dtype = B.k, B.two_d, A.dtype
-        ctx.save_for_backward(B.codes, B.scales)
+        ctx.dtype, ctx.shape = A.dtype, (B._l, B.rows, B.k, 4, -1, B.two_d)  # of B^T, [l, n, k]
+        ctx.save_for_backward(*B._tensors())
         return _mx4_product(A, B, out_dtype)
 
     @staticmethod
     @_once
     def backward(ctx, dC):
-        codes, scales = ctx.saved_tensors
-        BT = MXTensor._of(codes, scales, 4, ctx.k, -1, ctx.two_d)  # [l, n, k]
+        BT = MXTensor._around(ctx.saved_tensors, *ctx.shape)
         dC = dC.to(ctx.dtype)
         if ctx.dtype in _X16:
             return MXDenseBMMCUDA()(dC, BT), None, None
@@ -381,23 +417,22 @@ class _CheckpointProduct(torch.autograd.Function):
     def forward(ctx, A, B):
         C = _dense_bmm(A, B) if A.dtype in _X16 else BMMCUDA()(A, B)
         need_a, need_b = ctx.needs_input_grad
-        ctx.k = A.shape[2]
+        ctx.shape = (*A.shape, 8, -1, False)
         ctx.b_transposed = B.stride(2) != 1 and B.stride(1) == 1
-        q = MXQuantizeCUDA(8)(A) if need_b else None
-        ctx.save_for_backward(B if need_a else None, q and q.codes, q and q.scales)
+        ctx.save_for_backward(B if need_a else None, *(MXQuantizeCUDA(8)(A)._tensors() if need_b else ()))
         return C
 
     @staticmethod
     @_once
     def backward(ctx, dC):
-        B, codes, scales = ctx.saved_tensors
+        B, *kept = ctx.saved_tensors
         x16 = dC.dtype in _X16
         dA = dB = None
         if B is not None:
             BT = B.transpose(1, 2)
             dA = _dense_bmm(dC, BT) if x16 else BMMCUDA()(dC, BT)
-        if codes is not None:
-            A8 = MXTensor._of(codes, scales, 8, ctx.k, -1, False)
+        if kept:
+            A8 = MXTensor._around(kept, *ctx.shape)
             if not x16:
                 dB = BMMCUDA()(A8.mT.dequantize(dC.dtype), dC)
             elif ctx.b_transposed:  # in B's own storage order
