@@ -191,7 +191,7 @@ void rows_splits(int sms, int l, int n, int k, int* splits, int* blocks) {
 
 // Whether the kernel quantises A itself. Every CTA quantises its range of k of all rows: up to 1024 blocks
 // of 32 (four a thread) that hides behind the first weights; beyond, a pass of its own is faster
-// (16 rows: 8.6 against 9.8 us at 4096 x 4096, 512 blocks; 16.6 against 14.4 us at n = 16384, k = 8192, 2048 blocks).
+// (16 rows: 6.2 against 6.9 us at 4096 x 4096, 512 blocks; 15.6 against 12.5 us at n = 16384, k = 8192, 2048 blocks).
 // The quantised rows also have to fit beside the ring.
 bool few_rows_fused(int sms, int l, int m, int n, int k, int layout) {
   if (m > kMxFewRows || layout != 'n') return false;

@@ -87,18 +87,31 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   const int kblocks = (a.k + kMxStageK - 1) / kMxStageK;
   const int first = static_cast<int>(split) * a.blocks_per_split;
   const int count = max(0, min(a.blocks_per_split, kblocks - first));  // this CTA's blocks of 256 k
-  if (threadIdx.x == 0) {
-    bars->abort_flag = 0;
-    for (int s = 0; s < a.stages; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
-    mbar_init(&bars->a_ready, S::kQuantWarps);
-    mbar_init(&bars->acc_full, 1);
-    fence_barrier_init();
-    tma_prefetch_desc(&map_w);
-    tma_prefetch_desc(&map_sw);
+  auto load = [&](int stage, int i) {  // block i of this CTA's range
+    uint8_t* st = smem + stage * S::kStage;
+    mbar_arrive_expect_tx(&bars->full[stage], S::kStage);
+    tma_load_3d_normal(st, &map_w, &bars->full[stage], (first + i) * kMxRowBytes, n0, a.w_shared ? 0 : b);
+    tma_load_3d_normal(st + kMxM * kMxRowBytes, &map_sw, &bars->full[stage], (first + i) * (kMxScaleStage / 4), n0 / kMxM,
+                       a.sw_shared ? 0 : b);
     if (S::kCodes) {
-      tma_prefetch_desc(&map_a);
-      tma_prefetch_desc(&map_sa);
+      tma_load_3d(st + kMxRowsWeights, &map_a, &bars->full[stage], (first + i) * kMxRowBytes, 0, a.a_shared ? 0 : b,
+                  kL2EvictLast);
+      tma_load_3d(st + kMxRowsWeights + NT * kMxRowBytes, &map_sa, &bars->full[stage], (first + i) * (kMxScaleStage / 4), 0,
+                  a.sa_shared ? 0 : b, kL2EvictLast);
     }
+  };
+  const int early = min(count, a.stages);
+  if (warp == 0) {
+    // the first copies of the ring leave before anything else: nothing waits for them to be asked for
+    if (elect_one()) {
+      bars->abort_flag = 0;
+      for (int s = 0; s < a.stages; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
+      mbar_init(&bars->a_ready, S::kQuantWarps);
+      mbar_init(&bars->acc_full, 1);
+      fence_barrier_init();
+      for (int i = 0; i < early; ++i) load(i, i);
+    }
+    __syncwarp();
   }
   if (warp == 1) {
     tmem_alloc(&bars->tmem_base, 256);
@@ -111,24 +124,12 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   bool ok = true;
 
   if (warp == 0) {
-    int stage = 0;
-    uint32_t phase = 0;
-    for (int i = 0; i < count; ++i) {
+    int stage = early == a.stages ? 0 : early;
+    uint32_t phase = 1;  // a stage is used again once its first use is done
+    for (int i = early; i < count; ++i) {
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag));
       if (!ok) break;
-      uint8_t* st = smem + stage * S::kStage;
-      if (elect_one()) {
-        mbar_arrive_expect_tx(&bars->full[stage], S::kStage);
-        tma_load_3d_normal(st, &map_w, &bars->full[stage], (first + i) * kMxRowBytes, n0, a.w_shared ? 0 : b);
-        tma_load_3d_normal(st + kMxM * kMxRowBytes, &map_sw, &bars->full[stage], (first + i) * (kMxScaleStage / 4), n0 / kMxM,
-                           a.sw_shared ? 0 : b);
-        if (S::kCodes) {
-          tma_load_3d(st + kMxRowsWeights, &map_a, &bars->full[stage], (first + i) * kMxRowBytes, 0, a.a_shared ? 0 : b,
-                      kL2EvictLast);
-          tma_load_3d(st + kMxRowsWeights + NT * kMxRowBytes, &map_sa, &bars->full[stage], (first + i) * (kMxScaleStage / 4), 0,
-                      a.sa_shared ? 0 : b, kL2EvictLast);
-        }
-      }
+      if (elect_one()) load(stage, i);
       __syncwarp();
       if (++stage == a.stages) { stage = 0; phase ^= 1u; }
     }
