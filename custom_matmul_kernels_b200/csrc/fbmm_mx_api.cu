@@ -171,16 +171,20 @@ int launch_mx_pair(cudaStream_t stream, int sms, const MxSide& A, const MxSide& 
 constexpr int kMxFewRows = 64;  // rows of A up to which the weights take the 128-row side of the MMA
 
 // How many CTAs share the k of a tile in the few-row kernel. A CTA takes about 0.25 us per 256 k (one
-// stage's latency over the depth of the ring), joining the sums 0.7 us, and a second CTA on an SM starts 0.7 us
-// late; two fit an SM. The least sum of these decides (measured: n = 4096, k = 4096 on 128 CTAs; n = 16384, k = 8192
-// 11.0 us on 256 against 12.4 on 128; n = 1024, k = 8192 4.9 us on 64 against 11.2 on 8).
-void rows_splits(int sms, int l, int n, int k, int* splits, int* blocks) {
+// stage's latency over the depth of the ring; 0.35 us with 128 rows), joining the sums 0.7 us (4), and a second CTA
+// on an SM starts 0.7 us late; two fit an SM (one with 128 rows). The least sum of these decides (measured: n = 16384,
+// k = 8192 11.0 us on 256 CTAs against 12.4 on 128; n = 1024, k = 8192 4.9 us on 64 against 11.2 on 8;
+// 128 rows at 4096 x 4096 8.1 us on 128 against 9.0 on 32, 256 rows 10.8 on 128 against 9.3 on 64).
+void rows_splits(int sms, int l, int m, int n, int k, int* splits, int* blocks) {
   const int kblocks = (k + kMxStageK - 1) / kMxStageK;
-  const long long base = static_cast<long long>((n + kMxM - 1) / kMxM) * l;
+  const bool tall = m > kMxFewRows;
+  const long long base = static_cast<long long>((n + kMxM - 1) / kMxM) * l * (tall ? (m + 127) / 128 : 1);
+  const long long slots = tall ? sms : 2ll * sms;
   long long best = 0;
   for (int s = 1; s <= 8 && (s == 1 || s <= kblocks); s *= 2) {
     const long long ctas = base * s, per = (kblocks + s - 1) / s;
-    const long long cost = (s > 1 ? 700 : 0) + 250 * per * ((ctas + 2 * sms - 1) / (2 * sms)) + 700 * ((ctas - 1) / sms);
+    const long long cost = (s > 1 ? (tall ? 4000 : 700) : 0) + (tall ? 350 : 250) * per * ((ctas + slots - 1) / slots) +
+                           700 * ((ctas - 1) / sms);
     if (s == 1 || cost < best) {
       best = cost;
       *splits = s;
@@ -196,7 +200,7 @@ void rows_splits(int sms, int l, int n, int k, int* splits, int* blocks) {
 bool few_rows_fused(int sms, int l, int m, int n, int k, int layout) {
   if (m > kMxFewRows || layout != 'n') return false;
   int splits, blocks;
-  rows_splits(sms, l, n, k, &splits, &blocks);
+  rows_splits(sms, l, m, n, k, &splits, &blocks);
   const int stages = std::min(4, blocks);
   const int smem = m <= 16 ? MxRowsShape<16, float>::smem(stages, blocks) : MxRowsShape<64, float>::smem(stages, blocks);
   return static_cast<long long>(m) * blocks * (kMxStageK / kMxBlock) <= 1024 && smem <= static_cast<int>(kMxSmemLimit);
@@ -218,12 +222,13 @@ int launch_mx_rows(cudaStream_t stream, int sms, const MxSide& W, const MxSide* 
     ma = mw; msa = msw;
   }
   a.n_tiles = (a.n + kMxM - 1) / kMxM;
-  rows_splits(sms, a.l, a.n, a.k, &a.splits, &a.blocks_per_split);
-  const long long grid = static_cast<long long>(a.n_tiles) * a.l * a.splits;
+  a.m_tiles = NT == 128 ? (a.m + NT - 1) / NT : 1;
+  rows_splits(sms, a.l, a.m, a.n, a.k, &a.splits, &a.blocks_per_split);
+  const long long grid = static_cast<long long>(a.n_tiles) * a.m_tiles * a.l * a.splits;
   if (grid > 0x7fffffffLL) return fail(FBMM_ERR_INVALID, "product of %d x %d x %d is too large", a.l, a.m, a.n);
   const int limit = static_cast<int>(kMxSmemLimit);
   const int budget = grid > sms && S::smem(3, a.blocks_per_split) <= limit / 2 ? limit / 2 : limit;
-  a.stages = std::min(kMxRowsMaxStages, a.blocks_per_split);
+  a.stages = std::min(S::kMaxStages, a.blocks_per_split);
   while (a.stages > 1 && S::smem(a.stages, a.blocks_per_split) > budget) --a.stages;
   const int smem = S::smem(a.stages, a.blocks_per_split);
   if (smem > limit) return fail(FBMM_ERR_INVALID, "internal: few-row kernel wants %d bytes of shared memory", smem);
@@ -458,11 +463,14 @@ int fbmm_mx4_bmm(void* stream_, const unsigned char* a_codes, long long stride_a
   const long long size = elem_size(dtype);
   a.vec_ok = ((reinterpret_cast<uintptr_t>(C) | (ldc * size) | (a.stride_c * size)) & 15) == 0;
   const MxSide A{a_codes, stride_a, a_scales, stride_as, m}, B{b_codes, stride_b, b_scales, stride_bs, n};
-  if (m <= kMxFewRows) {
+  int splits, blocks;
+  rows_splits(sms, l, m, n, k, &splits, &blocks);
+  if (m <= kMxFewRows || splits > 1) {
     MxRowsArgs r{};
     r.C = C; r.ldc = ldc; r.stride_c = a.stride_c;
     r.l = l; r.m = m; r.n = n; r.k = k;
     r.out_type = dtype; r.vec_ok = a.vec_ok;
+    if (m > kMxFewRows) return launch_mx_rows<128, uint8_t>(stream, sms, B, &A, r);
     return m <= 16 ? launch_mx_rows<16, uint8_t>(stream, sms, B, &A, r) : launch_mx_rows<64, uint8_t>(stream, sms, B, &A, r);
   }
   const long long pairs = static_cast<long long>((m + 255) / 256) * ((n + 255) / 256) * l;

@@ -1,4 +1,5 @@
-// The 4-bit product for few rows of A (a decoding step): C[m][n] for m <= NT rows. The weights fill the
+// The 4-bit product for few rows of A (a decoding step): C[m][n] for m <= NT rows, and for tiles of 128 rows where
+// whole tiles are too few for the SMs. The weights fill the
 // 128-row side of the MMA and are streamed once, which is what bounds the product (17/32 byte per weight).
 // A comes as codes (T = uint8_t), copied beside the weights, or as fp32 / fp16 / bf16, which every CTA
 // quantises for its own range of k (fbmm_mx_quant.cuh's rules, straight into the swizzled tiles and scale
@@ -30,7 +31,7 @@ struct MxRowsArgs {
   int w_shared, sw_shared, a_shared, sa_shared;
   int out_type;
   int vec_ok;               // C's rows are 16-byte aligned
-  int n_tiles, splits, blocks_per_split;  // blocks of 256 k
+  int n_tiles, m_tiles, splits, blocks_per_split;  // blocks of 256 k
   int stages;
 };
 
@@ -46,6 +47,8 @@ struct MxRowsShape {
   static constexpr int kABlock = NT * kMxRowBytes + kMxScaleStage;  // per 256 k: codes of A, scales
   static constexpr int kStage = kMxRowsWeights + (kCodes ? kABlock : 0);
   static constexpr int kSums = NT * 128 * 4;
+  static constexpr int kSfBase = NT > 64 ? NT : 64;  // tensor-memory column of the scales, 16 per stage
+  static constexpr int kMaxStages = (256 - kSfBase) / 16 < kMxRowsMaxStages ? (256 - kSfBase) / 16 : kMxRowsMaxStages;
   static constexpr int kThreads = kCodes ? 192 : 320;
   static constexpr int kQuantWarps = kThreads / 32 - 2;
   __host__ __device__ static constexpr int ring(int stages) {
@@ -83,7 +86,9 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   const uint32_t warp = warp_index(), lane = lane_id();
   const uint32_t split = cluster_cta_rank();
   const int unit = static_cast<int>(blockIdx.x / static_cast<uint32_t>(a.splits));
-  const int b = unit / a.n_tiles, n0 = (unit - b * a.n_tiles) * kMxM;
+  const int mt = unit % a.m_tiles, column = unit / a.m_tiles;
+  const int b = column / a.n_tiles, n0 = (column - b * a.n_tiles) * kMxM;
+  const int m0 = mt * NT, rows = min(NT, a.m - m0);  // more than one tile of rows only at NT = 128
   const int kblocks = (a.k + kMxStageK - 1) / kMxStageK;
   const int first = static_cast<int>(split) * a.blocks_per_split;
   const int count = max(0, min(a.blocks_per_split, kblocks - first));  // this CTA's blocks of 256 k
@@ -94,9 +99,9 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     tma_load_3d_normal(st + kMxM * kMxRowBytes, &map_sw, &bars->full[stage], (first + i) * (kMxScaleStage / 4), n0 / kMxM,
                        a.sw_shared ? 0 : b);
     if (S::kCodes) {
-      tma_load_3d(st + kMxRowsWeights, &map_a, &bars->full[stage], (first + i) * kMxRowBytes, 0, a.a_shared ? 0 : b,
+      tma_load_3d(st + kMxRowsWeights, &map_a, &bars->full[stage], (first + i) * kMxRowBytes, m0, a.a_shared ? 0 : b,
                   kL2EvictLast);
-      tma_load_3d(st + kMxRowsWeights + NT * kMxRowBytes, &map_sa, &bars->full[stage], (first + i) * (kMxScaleStage / 4), 0,
+      tma_load_3d(st + kMxRowsWeights + NT * kMxRowBytes, &map_sa, &bars->full[stage], (first + i) * (kMxScaleStage / 4), m0 / 128,
                   a.sa_shared ? 0 : b, kL2EvictLast);
     }
   };
@@ -120,7 +125,7 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   tcgen05_fence_before_sync();
   __syncthreads();
   tcgen05_fence_after_sync();
-  const uint32_t tmem = bars->tmem_base;  // columns 0-63 sums, 64 + 16 per stage scales
+  const uint32_t tmem = bars->tmem_base;  // sums, then scales
   bool ok = true;
 
   if (warp == 0) {
@@ -148,7 +153,7 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       const uint32_t st = smem_u32(smem + stage * S::kStage);
       const uint32_t qa = S::kCodes ? st + kMxRowsWeights : smem_u32(a_codes + i * (NT * kMxRowBytes));
       const uint32_t qs = S::kCodes ? qa + NT * kMxRowBytes : smem_u32(a_scales + i * kMxScaleStage);
-      const uint32_t t_sf = tmem + 64 + stage * 16;
+      const uint32_t t_sf = tmem + S::kSfBase + stage * 16;
       const uint64_t pd = mx_desc_codes(st), qd = mx_desc_codes(qa);
       if (elect_one()) {
 #pragma unroll
@@ -213,7 +218,7 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     if (ok) {
       tcgen05_fence_after_sync();
 #pragma unroll 1
-      for (int c = 0; c < NT && c < a.m; c += 32) {
+      for (int c = 0; c < NT && c < rows; c += 32) {
         uint32_t v[32];
         if (count > 0) {
           tmem_ld_32x32b_x32(tmem + ((quarter * 32u) << 16) + c, v);
@@ -232,13 +237,14 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   cluster_sync_all();
   const int failed = *abort_flag != 0;
   if (!failed) {
-    // a warp per row of this CTA's share, four columns a lane
+    // a warp per row of this CTA's share, four columns a lane (four rows at once measured slower by a microsecond:
+    // more instructions to fetch outweigh the loads in flight)
     constexpr int kWarps = S::kThreads / 32;
     const int col = n0 + static_cast<int>(lane) * 4;
     const uint32_t at = smem_u32(sums) + lane * 16;
     const int size = a.out_type == 0 ? 4 : 2;
     const bool vec = a.vec_ok && col + 4 <= a.n;
-    for (int r = static_cast<int>(split) + a.splits * static_cast<int>(warp); r < a.m; r += kWarps * a.splits) {
+    for (int r = static_cast<int>(split) + a.splits * static_cast<int>(warp); r < rows; r += kWarps * a.splits) {
       float s[4] = {0.f, 0.f, 0.f, 0.f};
       for (int q0 = 0; q0 < a.splits; q0 += 4) {
         float4 v[4];
@@ -249,7 +255,7 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
         for (int q = 0; q < 4; ++q)
           if (q0 + q < a.splits) { s[0] += v[q].x; s[1] += v[q].y; s[2] += v[q].z; s[3] += v[q].w; }
       }
-      const long long to = b * a.stride_c + static_cast<long long>(r) * a.ldc + col;
+      const long long to = b * a.stride_c + static_cast<long long>(m0 + r) * a.ldc + col;
       if (vec) {
         uint8_t* p = static_cast<uint8_t*>(a.C) + to * size;
         if (size == 4) *reinterpret_cast<float4*>(p) = make_float4(s[0], s[1], s[2], s[3]);

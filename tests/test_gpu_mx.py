@@ -153,6 +153,18 @@ def test_product_many_tiles(dev, l, m, n, k, dtype):
         assert bool(torch.isnan(C2[0, -1]).all()) and torch.equal(C2[0, :-1], C[0, :-1])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("l,m,n,k", [(1, 65, 130, 2500), (1, 128, 256, 9000), (2, 200, 500, 1800), (1, 300, 900, 4100), (1, 129, 1, 520)])
+def test_product_split_tiles(dev, l, m, n, k, dtype):
+    """Few whole tiles: k split over clusters, several tiles of rows."""
+    A, a = as_mx(m, k, 4, 11, dev, l, lo=121, hi=125)
+    B, b = as_mx(n, k, 4, 977, dev, l, dim=-2, lo=121, hi=125)
+    a, b = a.to(dev), b.to(dev)
+    C = MXBMMCUDA(out_dtype=dtype)(A, B)
+    assert_sum_close(C, (a @ b.transpose(1, 2)).cpu(), (a.abs() @ b.abs().transpose(1, 2)).cpu(), k, dtype)
+    assert torch.equal(MXBMMCUDA(out_dtype=dtype)(A, B), C)
+
+
 @pytest.mark.parametrize("m", [1, 16, 40, 200])
 def test_product_exact_integers(dev, m):
     """Scales of one: every sum is a multiple of 1/4 below 2^22, so the result is exact."""
