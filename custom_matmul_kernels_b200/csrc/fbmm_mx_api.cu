@@ -34,6 +34,12 @@ int check_type(int dtype) {
   return FBMM_OK;
 }
 
+// 'n' or 't' in either case; 0 for anything else.
+int layout_letter(int letter) {
+  if (letter == 'n' || letter == 'N') return 'n';
+  return letter == 't' || letter == 'T' ? 't' : 0;
+}
+
 int elem_size(int dtype) { return dtype == FBMM_F32 ? 4 : 2; }
 
 // A microscaled operand as the entry points take it.
@@ -52,11 +58,11 @@ int check_quantize_source(const void* X, int dtype, int layout, long long ldx, l
   int rc;
   if ((rc = check_shape(l, rows, k)) != FBMM_OK) return rc;
   if ((rc = check_type(dtype)) != FBMM_OK) return rc;
-  if (layout != 'n' && layout != 't') return fail(FBMM_ERR_INVALID, "layout must be 'n' or 't', got %d", layout);
+  if (layout_letter(layout) == 0) return fail(FBMM_ERR_INVALID, "layout must be 'n' or 't', got %d", layout);
   if (X == nullptr) return fail(FBMM_ERR_INVALID, "the source is null");
   if ((reinterpret_cast<uintptr_t>(X) & static_cast<uintptr_t>(elem_size(dtype) - 1)) != 0)
     return fail(FBMM_ERR_ALIGN, "the source is not aligned to its element type");
-  if (ldx < (layout == 'n' ? k : rows)) return fail(FBMM_ERR_INVALID, "source pitch %lld smaller than its row length", ldx);
+  if (ldx < (layout_letter(layout) == 'n' ? k : rows)) return fail(FBMM_ERR_INVALID, "source pitch %lld smaller than its row length", ldx);
   if (l > 1 && stride_x < 0) return fail(FBMM_ERR_INVALID, "source batch stride is negative");
   return FBMM_OK;
 }
@@ -198,7 +204,7 @@ void rows_splits(int sms, int l, int m, int n, int k, int* splits, int* blocks) 
 // (16 rows: 6.2 against 6.9 us at 4096 x 4096, 512 blocks; 15.6 against 12.5 us at n = 16384, k = 8192, 2048 blocks).
 // The quantised rows also have to fit beside the ring.
 bool few_rows_fused(int sms, int l, int m, int n, int k, int layout) {
-  if (m > kMxFewRows || layout != 'n') return false;
+  if (m > kMxFewRows || layout_letter(layout) != 'n') return false;
   int splits, blocks;
   rows_splits(sms, l, m, n, k, &splits, &blocks);
   const int stages = std::min(4, blocks);
@@ -370,8 +376,8 @@ int x16_product(cudaStream_t stream, const X16Side& x, const X16Side& y, int dty
 }
 
 int layout_kind(const char* name, int letter, int k_major_letter, int* kind) {
-  if (letter != 'n' && letter != 't') return fail(FBMM_ERR_INVALID, "%s layout must be 'n' or 't', got %d", name, letter);
-  *kind = letter == k_major_letter ? kX16K : kX16MN;
+  if (layout_letter(letter) == 0) return fail(FBMM_ERR_INVALID, "%s layout must be 'n' or 't', got %d", name, letter);
+  *kind = layout_letter(letter) == k_major_letter ? kX16K : kX16MN;
   return FBMM_OK;
 }
 
@@ -407,7 +413,7 @@ int fbmm_mx_quantize(void* stream_, const void* X, int dtype, int layout, long l
   if ((rc = check_mx("output", codes, 0, scales, 0, 1)) != FBMM_OK) return rc;
   if ((rc = fbmm_host::device_sms(&sms)) != FBMM_OK) return rc;
   const MxQuantArgs a{X, ldx, l > 1 ? stride_x : 0, codes, scales, rows, k, l};
-  const bool t = layout == 't';
+  const bool t = layout_letter(layout) == 't';
   if (bits == 4) {
     if (dtype == FBMM_F32) return launch_quantize<4, float>(stream, a, t);
     if (dtype == FBMM_F16) return launch_quantize<4, __half>(stream, a, t);

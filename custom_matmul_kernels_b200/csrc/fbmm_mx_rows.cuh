@@ -233,7 +233,14 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       }
     }
   }
+  // Tensor memory goes back before anything waits for another CTA: several CTAs fit an SM, and one that
+  // held columns here while its peer waited for columns elsewhere could close a circle.
   tcgen05_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after_sync();
+    tmem_dealloc(tmem, 256);
+  }
   cluster_sync_all();
   const int failed = *abort_flag != 0;
   if (!failed) {
@@ -271,10 +278,6 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (threadIdx.x == 0 && failed) atomicOr(&g_mx_status[0], 1u);
-  if (warp == 1) {
-    tcgen05_fence_after_sync();
-    tmem_dealloc(tmem, 256);
-  }
 }
 
 }  // namespace fbmm
