@@ -111,6 +111,35 @@ int codes_map(CUtensorMap* map, const unsigned char* codes, long long stride, in
   return fbmm_host::tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, dims, strides, box, true);
 }
 
+// A launch with a cluster and, where the kernel before it in the stream quantises its operand, the
+// right to start before that one has ended.
+template <typename... Args>
+int launch(cudaStream_t stream, long long grid, int threads, int smem, int cluster, bool overlap, void (*kernel)(Args...),
+           Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2] = {};
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (overlap) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  cfg.attrs = attr;
+  FBMM_HOST_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMxSmemLimit)));
+  FBMM_HOST_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  return FBMM_OK;
+}
+
 struct MxSide {
   const unsigned char* codes;
   long long stride;
@@ -131,7 +160,7 @@ int scales_map(CUtensorMap* map, const unsigned char* scales, long long stride, 
   return fbmm_host::tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, scales, dims, strides, box, false);
 }
 
-int launch_mx_gemm(cudaStream_t stream, int sms, const MxSide& p, const MxSide& q, MxGemmArgs a) {
+int launch_mx_gemm(cudaStream_t stream, int sms, bool overlap, const MxSide& p, const MxSide& q, MxGemmArgs a) {
   CUtensorMap mp, mq, msp, msq;
   int rc;
   if ((rc = codes_map(&mp, p.codes, p.stride, a.l, p.rows, a.k, kMxM)) != FBMM_OK) return rc;
@@ -144,14 +173,10 @@ int launch_mx_gemm(cudaStream_t stream, int sms, const MxSide& p, const MxSide& 
   a.p_tiles = (p.rows + kMxM - 1) / kMxM;
   a.q_tiles = (q.rows + MxShape::BN - 1) / MxShape::BN;
   const long long units = static_cast<long long>(a.p_tiles) * a.q_tiles * a.l;
-  using S = MxShape;
-  FBMM_HOST_CUDA(cudaFuncSetAttribute(mx_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-  mx_gemm_kernel<<<static_cast<unsigned>(std::min<long long>(units, sms)), kMxThreads, S::kSmem, stream>>>(mp, mq, msp, msq, a);
-  FBMM_HOST_CUDA(cudaGetLastError());
-  return FBMM_OK;
+  return launch(stream, std::min<long long>(units, sms), kMxThreads, MxShape::kSmem, 1, overlap, mx_gemm_kernel, mp, mq, msp, msq, a);
 }
 
-int launch_mx_pair(cudaStream_t stream, int sms, const MxSide& A, const MxSide& B, const MxGemmArgs& g) {
+int launch_mx_pair(cudaStream_t stream, int sms, bool overlap, const MxSide& A, const MxSide& B, const MxGemmArgs& g) {
   CUtensorMap ma, mb, msa, msb;
   int rc;
   if ((rc = codes_map(&ma, A.codes, A.stride, g.l, A.rows, g.k, 128)) != FBMM_OK) return rc;
@@ -167,11 +192,8 @@ int launch_mx_pair(cudaStream_t stream, int sms, const MxSide& A, const MxSide& 
   a.m_tiles = (a.m + 255) / 256;
   a.n_tiles = (a.n + 255) / 256;
   const long long units = static_cast<long long>(a.m_tiles) * a.n_tiles * a.l;
-  FBMM_HOST_CUDA(cudaFuncSetAttribute(mx_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMxPairSmem));
-  mx_gemm_pair_kernel<<<static_cast<unsigned>(2 * std::min<long long>(units, sms / 2)), kMxPairThreads, kMxPairSmem, stream>>>(
-      ma, mb, msa, msb, a);
-  FBMM_HOST_CUDA(cudaGetLastError());
-  return FBMM_OK;
+  return launch(stream, 2 * std::min<long long>(units, sms / 2), kMxPairThreads, kMxPairSmem, 2, overlap, mx_gemm_pair_kernel, ma, mb,
+                msa, msb, a);
 }
 
 constexpr int kMxFewRows = 64;  // rows of A up to which the weights take the 128-row side of the MMA
@@ -213,7 +235,7 @@ bool few_rows_fused(int sms, int l, int m, int n, int k, int layout) {
 }
 
 template <int NT, typename T>
-int launch_mx_rows(cudaStream_t stream, int sms, const MxSide& W, const MxSide* A, MxRowsArgs a) {
+int launch_mx_rows(cudaStream_t stream, int sms, bool overlap, const MxSide& W, const MxSide* A, MxRowsArgs a) {
   using S = MxRowsShape<NT, T>;
   CUtensorMap mw, msw, ma, msa;
   int rc;
@@ -238,26 +260,49 @@ int launch_mx_rows(cudaStream_t stream, int sms, const MxSide& W, const MxSide* 
   while (a.stages > 1 && S::smem(a.stages, a.blocks_per_split) > budget) --a.stages;
   const int smem = S::smem(a.stages, a.blocks_per_split);
   if (smem > limit) return fail(FBMM_ERR_INVALID, "internal: few-row kernel wants %d bytes of shared memory", smem);
-  FBMM_HOST_CUDA(cudaFuncSetAttribute(mx_rows_kernel<NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, limit));
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(S::kThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(a.splits); attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  FBMM_HOST_CUDA(cudaLaunchKernelEx(&cfg, mx_rows_kernel<NT, T>, mw, msw, ma, msa, a));
-  return FBMM_OK;
+  return launch(stream, grid, S::kThreads, smem, a.splits, overlap, mx_rows_kernel<NT, T>, mw, msw, ma, msa, a);
 }
 
 template <int NT>
 int launch_mx_rows_fused(cudaStream_t stream, int sms, int dtype, const MxSide& W, const MxRowsArgs& a) {
-  if (dtype == FBMM_F32) return launch_mx_rows<NT, float>(stream, sms, W, nullptr, a);
-  if (dtype == FBMM_F16) return launch_mx_rows<NT, __half>(stream, sms, W, nullptr, a);
-  return launch_mx_rows<NT, __nv_bfloat16>(stream, sms, W, nullptr, a);
+  if (dtype == FBMM_F32) return launch_mx_rows<NT, float>(stream, sms, false, W, nullptr, a);
+  if (dtype == FBMM_F16) return launch_mx_rows<NT, __half>(stream, sms, false, W, nullptr, a);
+  return launch_mx_rows<NT, __nv_bfloat16>(stream, sms, false, W, nullptr, a);
+}
+
+// C = A @ B^T of two 4-bit operands; `overlap`: the kernel before this in the stream writes A.
+int mx4_product(cudaStream_t stream, bool overlap, const unsigned char* a_codes, long long stride_a,
+                const unsigned char* a_scales, long long stride_as, const unsigned char* b_codes, long long stride_b,
+                const unsigned char* b_scales, long long stride_bs, void* C, int dtype, long long ldc, long long stride_c, int l,
+                int m, int n, int k) {
+  int rc, sms;
+  if ((rc = check_shape(l, m, k)) != FBMM_OK) return rc;
+  if ((rc = check_shape(l, n, k)) != FBMM_OK) return rc;
+  if ((rc = check_mx("A", a_codes, stride_a, a_scales, stride_as, l)) != FBMM_OK) return rc;
+  if ((rc = check_mx("B", b_codes, stride_b, b_scales, stride_bs, l)) != FBMM_OK) return rc;
+  if ((rc = check_result(C, dtype, ldc, stride_c, l, m, n)) != FBMM_OK) return rc;
+  if ((rc = fbmm_host::device_sms(&sms)) != FBMM_OK) return rc;
+  MxGemmArgs a{};
+  a.C = C; a.ldc = ldc; a.stride_c = l > 1 ? stride_c : 0;
+  a.l = l; a.k = k; a.out_type = dtype;
+  const long long size = elem_size(dtype);
+  a.vec_ok = ((reinterpret_cast<uintptr_t>(C) | (ldc * size) | (a.stride_c * size)) & 15) == 0;
+  const MxSide A{a_codes, stride_a, a_scales, stride_as, m}, B{b_codes, stride_b, b_scales, stride_bs, n};
+  int splits, blocks;
+  rows_splits(sms, l, m, n, k, &splits, &blocks);
+  if (m <= kMxFewRows || splits > 1) {
+    MxRowsArgs r{};
+    r.C = C; r.ldc = ldc; r.stride_c = a.stride_c;
+    r.l = l; r.m = m; r.n = n; r.k = k;
+    r.out_type = dtype; r.vec_ok = a.vec_ok;
+    if (m > kMxFewRows) return launch_mx_rows<128, uint8_t>(stream, sms, overlap, B, &A, r);
+    return m <= 16 ? launch_mx_rows<16, uint8_t>(stream, sms, overlap, B, &A, r) : launch_mx_rows<64, uint8_t>(stream, sms, overlap, B, &A, r);
+  }
+  const long long pairs = static_cast<long long>((m + 255) / 256) * ((n + 255) / 256) * l;
+  const long long singles = static_cast<long long>((m + 127) / 128) * ((n + 127) / 128) * l;
+  const long long pair_waves = (pairs + sms / 2 - 1) / (sms / 2), single_waves = (singles + sms - 1) / sms;
+  if (5 * pair_waves <= 4 * single_waves) return launch_mx_pair(stream, sms, overlap, A, B, a);
+  return launch_mx_gemm(stream, sms, overlap, A, B, a);
 }
 
 // One operand of a 16-bit product: a dense matrix of `rows` x J (J contiguous, or the rows), or a
@@ -311,18 +356,8 @@ int launch_x16(cudaStream_t stream, int sms, const CUtensorMap& mx, const CUtens
   a.x_tiles = (a.x.rows + kTile - 1) / kTile;
   a.y_tiles = (a.y.rows + kTile - 1) / kTile;
   const long long units = static_cast<long long>(a.x_tiles) * a.y_tiles * a.l;
-  FBMM_HOST_CUDA(cudaFuncSetAttribute(x16_gemm_kernel<XK, YK, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(PAIR ? 2 * std::min<long long>(units, sms / 2) : std::min<long long>(units, sms)));
-  cfg.blockDim = dim3(S::kThreads);
-  cfg.dynamicSmemBytes = S::kSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-  if (PAIR) { cfg.attrs = &attr; cfg.numAttrs = 1; }
-  FBMM_HOST_CUDA(cudaLaunchKernelEx(&cfg, x16_gemm_kernel<XK, YK, PAIR>, mx, my, a));
-  return FBMM_OK;
+  return launch(stream, PAIR ? 2 * std::min<long long>(units, sms / 2) : std::min<long long>(units, sms), S::kThreads, S::kSmem,
+                PAIR ? 2 : 1, false, x16_gemm_kernel<XK, YK, PAIR>, mx, my, a);
 }
 
 template <int XK, int YK>
@@ -452,38 +487,11 @@ int fbmm_mx_dequantize(void* stream_, const unsigned char* codes, long long stri
   return launch_dequantize<8, __nv_bfloat16>(stream, a);
 }
 
-int fbmm_mx4_bmm(void* stream_, const unsigned char* a_codes, long long stride_a, const unsigned char* a_scales,
+int fbmm_mx4_bmm(void* stream, const unsigned char* a_codes, long long stride_a, const unsigned char* a_scales,
                  long long stride_as, const unsigned char* b_codes, long long stride_b, const unsigned char* b_scales,
                  long long stride_bs, void* C, int dtype, long long ldc, long long stride_c, int l, int m, int n, int k) {
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  int rc, sms;
-  if ((rc = check_shape(l, m, k)) != FBMM_OK) return rc;
-  if ((rc = check_shape(l, n, k)) != FBMM_OK) return rc;
-  if ((rc = check_mx("A", a_codes, stride_a, a_scales, stride_as, l)) != FBMM_OK) return rc;
-  if ((rc = check_mx("B", b_codes, stride_b, b_scales, stride_bs, l)) != FBMM_OK) return rc;
-  if ((rc = check_result(C, dtype, ldc, stride_c, l, m, n)) != FBMM_OK) return rc;
-  if ((rc = fbmm_host::device_sms(&sms)) != FBMM_OK) return rc;
-  MxGemmArgs a{};
-  a.C = C; a.ldc = ldc; a.stride_c = l > 1 ? stride_c : 0;
-  a.l = l; a.k = k; a.out_type = dtype;
-  const long long size = elem_size(dtype);
-  a.vec_ok = ((reinterpret_cast<uintptr_t>(C) | (ldc * size) | (a.stride_c * size)) & 15) == 0;
-  const MxSide A{a_codes, stride_a, a_scales, stride_as, m}, B{b_codes, stride_b, b_scales, stride_bs, n};
-  int splits, blocks;
-  rows_splits(sms, l, m, n, k, &splits, &blocks);
-  if (m <= kMxFewRows || splits > 1) {
-    MxRowsArgs r{};
-    r.C = C; r.ldc = ldc; r.stride_c = a.stride_c;
-    r.l = l; r.m = m; r.n = n; r.k = k;
-    r.out_type = dtype; r.vec_ok = a.vec_ok;
-    if (m > kMxFewRows) return launch_mx_rows<128, uint8_t>(stream, sms, B, &A, r);
-    return m <= 16 ? launch_mx_rows<16, uint8_t>(stream, sms, B, &A, r) : launch_mx_rows<64, uint8_t>(stream, sms, B, &A, r);
-  }
-  const long long pairs = static_cast<long long>((m + 255) / 256) * ((n + 255) / 256) * l;
-  const long long singles = static_cast<long long>((m + 127) / 128) * ((n + 127) / 128) * l;
-  const long long pair_waves = (pairs + sms / 2 - 1) / (sms / 2), single_waves = (singles + sms - 1) / sms;
-  if (5 * pair_waves <= 4 * single_waves) return launch_mx_pair(stream, sms, A, B, a);
-  return launch_mx_gemm(stream, sms, A, B, a);
+  return mx4_product(static_cast<cudaStream_t>(stream), false, a_codes, stride_a, a_scales, stride_as, b_codes, stride_b, b_scales,
+                     stride_bs, C, dtype, ldc, stride_c, l, m, n, k);
 }
 
 size_t fbmm_mx4_bmm_tensor_workspace_bytes(int l, int m, int n, int k, int a_layout) {
@@ -520,8 +528,8 @@ int fbmm_mx4_bmm_tensor(void* stream, const void* A, int a_dtype, int a_layout, 
   unsigned char* codes = static_cast<unsigned char*>(workspace);
   unsigned char* scales = codes + (need - fbmm_mx_scales_bytes(l, m, k));
   if ((rc = fbmm_mx_quantize(stream, A, a_dtype, a_layout, lda, stride_a, 4, codes, scales, l, m, k)) != FBMM_OK) return rc;
-  return fbmm_mx4_bmm(stream, codes, static_cast<long long>(m) * mx_pitch(k, 4), scales, mx_scale_bytes(m, k), b_codes,
-                      stride_b, b_scales, stride_bs, C, dtype, ldc, stride_c, l, m, n, k);
+  return mx4_product(static_cast<cudaStream_t>(stream), true, codes, static_cast<long long>(m) * mx_pitch(k, 4), scales,
+                     mx_scale_bytes(m, k), b_codes, stride_b, b_scales, stride_bs, C, dtype, ldc, stride_c, l, m, n, k);
 }
 
 int fbmm_dense_bmm_x16(void* stream, const void* A, int a_layout, long long lda, long long stride_a, const void* B,

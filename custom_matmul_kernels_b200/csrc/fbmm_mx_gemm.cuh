@@ -239,6 +239,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant_
   if (warp == 0) {
     uint32_t stage = 0, phase = 0;
     bool ok = true;
+    mx_wait_for_previous();
     for (long long u = blockIdx.x; u < units && ok; u += gridDim.x) {
       int b, pt, qt;
       decode(u, b, pt, qt);

@@ -56,7 +56,7 @@ struct MxPairBarriers {
 };
 static_assert(sizeof(MxPairBarriers) <= 256, "barrier block");
 
-__global__ void __launch_bounds__(kMxPairThreads, 1) __cluster_dims__(2, 1, 1)
+__global__ void __launch_bounds__(kMxPairThreads, 1)
 mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                     const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
                     const MxPairArgs a) {
@@ -100,6 +100,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     {
       uint32_t stage = 0, phase = 0;
       bool ok = true;
+      mx_wait_for_previous();
       for (long long u = u0; u < units && ok; u += du) {
         int b, mt, nt;
         x16_decode(u, a.m_tiles, a.n_tiles, b, mt, nt);

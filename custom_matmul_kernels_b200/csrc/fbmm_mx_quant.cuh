@@ -255,6 +255,12 @@ struct MxQuantArgs {
   int rows, k, l;
 };
 
+// A product that reads what the kernel before it in the stream has quantised is launched to overlap with it
+// (programmatic dependent launch): the quantisers let it start at once, and its copies of their
+// results wait until they are complete and visible. Without such a launch both do nothing.
+__device__ __forceinline__ void mx_let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void mx_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Blocks of the three kernels below count groups along k first, then along the rows, then batches.
 __device__ __forceinline__ void mx_group_of_block(int rows, int k, int& kg, int& rg, long long& b) {
   const uint32_t kgs = static_cast<uint32_t>((k + kMxGroupK - 1) / kMxGroupK);
@@ -281,6 +287,7 @@ __device__ __forceinline__ int mx_row_alignment(const void* p, long long ld, lon
 // block's largest magnitude: 54 us).
 template <int BITS, typename T>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
+  mx_let_next_start();
   int kg, rg;
   long long b;
   mx_group_of_block(a.rows, a.k, kg, rg, b);
@@ -358,6 +365,7 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const MxQuantArgs a) {
 // check: instruction issue was the limit).
 template <int BITS, typename T>
 __global__ void __launch_bounds__(256, 4) mx_quantize_t_kernel(const MxQuantArgs a) {
+  mx_let_next_start();
   constexpr int kRowBytes = kMxGroupK * BITS / 8;  // 64 or 128 bytes of codes per row of a group
   constexpr int kPad = 16;
   __shared__ __align__(16) uint8_t sc[kMxGroupBytes];

@@ -92,29 +92,33 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
   const int kblocks = (a.k + kMxStageK - 1) / kMxStageK;
   const int first = static_cast<int>(split) * a.blocks_per_split;
   const int count = max(0, min(a.blocks_per_split, kblocks - first));  // this CTA's blocks of 256 k
-  auto load = [&](int stage, int i) {  // block i of this CTA's range
+  auto load_weights = [&](int stage, int i) {  // block i of this CTA's range
     uint8_t* st = smem + stage * S::kStage;
     mbar_arrive_expect_tx(&bars->full[stage], S::kStage);
     tma_load_3d_normal(st, &map_w, &bars->full[stage], (first + i) * kMxRowBytes, n0, a.w_shared ? 0 : b);
     tma_load_3d_normal(st + kMxM * kMxRowBytes, &map_sw, &bars->full[stage], (first + i) * (kMxScaleStage / 4), n0 / kMxM,
                        a.sw_shared ? 0 : b);
-    if (S::kCodes) {
-      tma_load_3d(st + kMxRowsWeights, &map_a, &bars->full[stage], (first + i) * kMxRowBytes, m0, a.a_shared ? 0 : b,
-                  kL2EvictLast);
-      tma_load_3d(st + kMxRowsWeights + NT * kMxRowBytes, &map_sa, &bars->full[stage], (first + i) * (kMxScaleStage / 4), m0 / 128,
-                  a.sa_shared ? 0 : b, kL2EvictLast);
-    }
+  };
+  auto load_a = [&](int stage, int i) {
+    uint8_t* st = smem + stage * S::kStage + kMxRowsWeights;
+    tma_load_3d(st, &map_a, &bars->full[stage], (first + i) * kMxRowBytes, m0, a.a_shared ? 0 : b, kL2EvictLast);
+    tma_load_3d(st + NT * kMxRowBytes, &map_sa, &bars->full[stage], (first + i) * (kMxScaleStage / 4), m0 / 128,
+                a.sa_shared ? 0 : b, kL2EvictLast);
   };
   const int early = min(count, a.stages);
   if (warp == 0) {
-    // the first copies of the ring leave before anything else: nothing waits for them to be asked for
+    // the first copies of the ring leave before anything else, those of A once what may be quantising it is done
     if (elect_one()) {
       bars->abort_flag = 0;
       for (int s = 0; s < a.stages; ++s) { mbar_init(&bars->full[s], 1); mbar_init(&bars->empty[s], 1); }
       mbar_init(&bars->a_ready, S::kQuantWarps);
       mbar_init(&bars->acc_full, 1);
       fence_barrier_init();
-      for (int i = 0; i < early; ++i) load(i, i);
+      for (int i = 0; i < early; ++i) load_weights(i, i);
+      if (S::kCodes) {
+        mx_wait_for_previous();
+        for (int i = 0; i < early; ++i) load_a(i, i);
+      }
     }
     __syncwarp();
   }
@@ -134,7 +138,10 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     for (int i = early; i < count; ++i) {
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->empty[stage], phase ^ 1u, abort_flag));
       if (!ok) break;
-      if (elect_one()) load(stage, i);
+      if (elect_one()) {
+        load_weights(stage, i);
+        if (S::kCodes) load_a(stage, i);
+      }
       __syncwarp();
       if (++stage == a.stages) { stage = 0; phase ^= 1u; }
     }
