@@ -111,8 +111,9 @@ int codes_map(CUtensorMap* map, const unsigned char* codes, long long stride, in
   return fbmm_host::tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, dims, strides, box, true);
 }
 
-// A launch with a cluster and, where the kernel before it in the stream quantises its operand, the
-// right to start before that one has ended.
+// A launch with a cluster and the right to start (set up barriers and tensor memory) before the kernel ahead of it
+// in the stream has ended. Kernels whose copies all wait for that kernel always have it; the few-row kernel,
+// which asks for weights before it waits, only behind a quantiser, which cannot be writing them.
 template <typename... Args>
 int launch(cudaStream_t stream, long long grid, int threads, int smem, int cluster, bool overlap, void (*kernel)(Args...),
            Args... args) {
@@ -160,7 +161,7 @@ int scales_map(CUtensorMap* map, const unsigned char* scales, long long stride, 
   return fbmm_host::tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, scales, dims, strides, box, false);
 }
 
-int launch_mx_gemm(cudaStream_t stream, int sms, bool overlap, const MxSide& p, const MxSide& q, MxGemmArgs a) {
+int launch_mx_gemm(cudaStream_t stream, int sms, const MxSide& p, const MxSide& q, MxGemmArgs a) {
   CUtensorMap mp, mq, msp, msq;
   int rc;
   if ((rc = codes_map(&mp, p.codes, p.stride, a.l, p.rows, a.k, kMxM)) != FBMM_OK) return rc;
@@ -173,10 +174,10 @@ int launch_mx_gemm(cudaStream_t stream, int sms, bool overlap, const MxSide& p, 
   a.p_tiles = (p.rows + kMxM - 1) / kMxM;
   a.q_tiles = (q.rows + MxShape::BN - 1) / MxShape::BN;
   const long long units = static_cast<long long>(a.p_tiles) * a.q_tiles * a.l;
-  return launch(stream, std::min<long long>(units, sms), kMxThreads, MxShape::kSmem, 1, overlap, mx_gemm_kernel, mp, mq, msp, msq, a);
+  return launch(stream, std::min<long long>(units, sms), kMxThreads, MxShape::kSmem, 1, true, mx_gemm_kernel, mp, mq, msp, msq, a);
 }
 
-int launch_mx_pair(cudaStream_t stream, int sms, bool overlap, const MxSide& A, const MxSide& B, const MxGemmArgs& g) {
+int launch_mx_pair(cudaStream_t stream, int sms, const MxSide& A, const MxSide& B, const MxGemmArgs& g) {
   CUtensorMap ma, mb, msa, msb;
   int rc;
   if ((rc = codes_map(&ma, A.codes, A.stride, g.l, A.rows, g.k, 128)) != FBMM_OK) return rc;
@@ -192,7 +193,7 @@ int launch_mx_pair(cudaStream_t stream, int sms, bool overlap, const MxSide& A, 
   a.m_tiles = (a.m + 255) / 256;
   a.n_tiles = (a.n + 255) / 256;
   const long long units = static_cast<long long>(a.m_tiles) * a.n_tiles * a.l;
-  return launch(stream, 2 * std::min<long long>(units, sms / 2), kMxPairThreads, kMxPairSmem, 2, overlap, mx_gemm_pair_kernel, ma, mb,
+  return launch(stream, 2 * std::min<long long>(units, sms / 2), kMxPairThreads, kMxPairSmem, 2, true, mx_gemm_pair_kernel, ma, mb,
                 msa, msb, a);
 }
 
@@ -270,7 +271,7 @@ int launch_mx_rows_fused(cudaStream_t stream, int sms, int dtype, const MxSide& 
   return launch_mx_rows<NT, __nv_bfloat16>(stream, sms, false, W, nullptr, a);
 }
 
-// C = A @ B^T of two 4-bit operands; `overlap`: the kernel before this in the stream writes A.
+// C = A @ B^T of two 4-bit operands; `overlap`: the kernel ahead in the stream is the quantiser that writes A.
 int mx4_product(cudaStream_t stream, bool overlap, const unsigned char* a_codes, long long stride_a,
                 const unsigned char* a_scales, long long stride_as, const unsigned char* b_codes, long long stride_b,
                 const unsigned char* b_scales, long long stride_bs, void* C, int dtype, long long ldc, long long stride_c, int l,
@@ -301,8 +302,8 @@ int mx4_product(cudaStream_t stream, bool overlap, const unsigned char* a_codes,
   const long long pairs = static_cast<long long>((m + 255) / 256) * ((n + 255) / 256) * l;
   const long long singles = static_cast<long long>((m + 127) / 128) * ((n + 127) / 128) * l;
   const long long pair_waves = (pairs + sms / 2 - 1) / (sms / 2), single_waves = (singles + sms - 1) / sms;
-  if (5 * pair_waves <= 4 * single_waves) return launch_mx_pair(stream, sms, overlap, A, B, a);
-  return launch_mx_gemm(stream, sms, overlap, A, B, a);
+  if (5 * pair_waves <= 4 * single_waves) return launch_mx_pair(stream, sms, A, B, a);
+  return launch_mx_gemm(stream, sms, A, B, a);
 }
 
 // One operand of a 16-bit product: a dense matrix of `rows` x J (J contiguous, or the rows), or a
@@ -357,7 +358,7 @@ int launch_x16(cudaStream_t stream, int sms, const CUtensorMap& mx, const CUtens
   a.y_tiles = (a.y.rows + kTile - 1) / kTile;
   const long long units = static_cast<long long>(a.x_tiles) * a.y_tiles * a.l;
   return launch(stream, PAIR ? 2 * std::min<long long>(units, sms / 2) : std::min<long long>(units, sms), S::kThreads, S::kSmem,
-                PAIR ? 2 : 1, false, x16_gemm_kernel<XK, YK, PAIR>, mx, my, a);
+                PAIR ? 2 : 1, true, x16_gemm_kernel<XK, YK, PAIR>, mx, my, a);
 }
 
 template <int XK, int YK>

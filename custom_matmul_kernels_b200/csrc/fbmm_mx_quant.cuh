@@ -255,9 +255,9 @@ struct MxQuantArgs {
   int rows, k, l;
 };
 
-// A product that reads what the kernel before it in the stream has quantised is launched to overlap with it
-// (programmatic dependent launch): the quantisers let it start at once, and its copies of their
-// results wait until they are complete and visible. Without such a launch both do nothing.
+// Programmatic dependent launch: the products may start while the kernel ahead of them in the stream still
+// runs (the quantisers let them at once), and none of their copies of what it may have written leaves before it
+// is complete and visible. Without such a launch both do nothing.
 __device__ __forceinline__ void mx_let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void mx_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

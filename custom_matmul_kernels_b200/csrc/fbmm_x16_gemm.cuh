@@ -212,6 +212,7 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     {
       uint32_t stage = 0, phase = 0;
       bool ok = true;
+      mx_wait_for_previous();
       // 128 rows of one operand, from row r0: to the part's place, or its raw codes
       auto load = [&](const CUtensorMap* map, int kind, uint8_t* part, uint8_t* raw, int j0, int r0, int b,
                       const X16Operand& op) {

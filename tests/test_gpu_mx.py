@@ -544,6 +544,46 @@ def test_decoding_captured_on_another_stream(dev):
         assert torch.equal(o, want[i % 2])
 
 
+@pytest.mark.parametrize("m", [3, 100, 2300])
+def test_operands_written_right_before(dev, m):
+    """Every operand is rewritten by the kernel ahead of the product, over and over; the products may start early, but
+    read what is there when that kernel is done."""
+    k, n = 512, 2304
+    A, B = torch.zeros(1, m, k, device=dev, dtype=BF16), torch.zeros(1, k, n, device=dev, dtype=BF16)
+    W = MXQuantizeCUDA(4)(torch.zeros(1, k, n, device=dev), dim=-2)
+    one = MXQuantizeCUDA(4)(torch.ones(1, k, n, device=dev), dim=-2)
+    along = MXQuantizeCUDA(4)(torch.ones(1, k, n, device=dev))
+    big = torch.zeros(1 << 26, device=dev, dtype=torch.uint8)
+    outs = []
+    for i in range(24):
+        big.zero_()
+        if i % 3 == 0:
+            A.fill_(i + 1.0)
+            W.codes.copy_(one.codes)
+            W.scales.copy_(one.scales)
+        elif i % 3 == 1:
+            W.scales.fill_(127 + i % 5)  # 4 * 2^(i % 5), the codes being those of 4 (ones scaled by 1/4)
+        else:
+            B.fill_(i + 1.0)
+        outs.append((i, MXBMMCUDA()(A, W), MXBMMCUDA()(MXQuantizeCUDA(4)(A), W),
+                     CheckpointBMMCUDA()(A.requires_grad_(), B).detach(), MXDenseBMMCUDA()(A.detach(), along)))
+        A = A.detach()
+    a, w, b = 0.0, 0.0, 0.0
+    for i, y, z, c, d in outs:
+        if i % 3 == 0:
+            a, w = i + 1.0, 1.0
+        elif i % 3 == 1:
+            w = 4.0 * 2.0 ** (i % 5)
+        else:
+            b = i + 1.0
+        # all elements of a row alike; A itself is rounded to 4 bits in y and z
+        a4 = float(S.values(*S.quantize(torch.full((1, 32), a, dtype=BF16), 4), 4)[0, 0])
+        assert float(y.min()) == float(y.max()) == float(torch.tensor(a4 * w * k).to(BF16)), i
+        assert float(z.min()) == float(z.max()) == a4 * w * k, i
+        assert float(c.min()) == float(c.max()) == float(torch.tensor(a * b * k).to(BF16)), i
+        assert float(d.min()) == float(d.max()) == float(torch.tensor(a * k).to(BF16)), i
+
+
 def test_library_reports_no_trouble(dev, lib):
     assert lib.fbmm_check(None) == 0, lib.fbmm_last_error()
 
