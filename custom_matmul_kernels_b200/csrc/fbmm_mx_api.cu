@@ -1,5 +1,6 @@
 // Host side of the microscaled entry points: quantisation, its inverse and the 4-bit product.
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/fbmm.h"
@@ -114,9 +115,17 @@ int codes_map(CUtensorMap* map, const unsigned char* codes, long long stride, in
 // A launch with a cluster and the right to start (set up barriers and tensor memory) before the kernel ahead of it
 // in the stream has ended. Kernels whose copies all wait for that kernel always have it; the few-row kernel,
 // which asks for weights before it waits, only behind a quantiser, which cannot be writing them.
-template <typename... Args>
-int launch(cudaStream_t stream, long long grid, int threads, int smem, int cluster, bool overlap, void (*kernel)(Args...),
-           Args... args) {
+template <auto kKernel, typename... Args>
+int launch(cudaStream_t stream, long long grid, int threads, int smem, int cluster, bool overlap, const Args&... args) {
+  // the kernel's shared-memory limit is set once per device
+  static std::atomic<unsigned long long> ready{0};
+  int dev = 0;
+  FBMM_HOST_CUDA(cudaGetDevice(&dev));
+  const unsigned long long bit = 1ull << (dev & 63);
+  if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
+    FBMM_HOST_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMxSmemLimit)));
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
@@ -136,8 +145,7 @@ int launch(cudaStream_t stream, long long grid, int threads, int smem, int clust
     ++cfg.numAttrs;
   }
   cfg.attrs = attr;
-  FBMM_HOST_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMxSmemLimit)));
-  FBMM_HOST_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  FBMM_HOST_CUDA(cudaLaunchKernelEx(&cfg, kKernel, args...));
   return FBMM_OK;
 }
 
@@ -174,7 +182,7 @@ int launch_mx_gemm(cudaStream_t stream, int sms, const MxSide& p, const MxSide& 
   a.p_tiles = (p.rows + kMxM - 1) / kMxM;
   a.q_tiles = (q.rows + MxShape::BN - 1) / MxShape::BN;
   const long long units = static_cast<long long>(a.p_tiles) * a.q_tiles * a.l;
-  return launch(stream, std::min<long long>(units, sms), kMxThreads, MxShape::kSmem, 1, true, mx_gemm_kernel, mp, mq, msp, msq, a);
+  return launch<mx_gemm_kernel>(stream, std::min<long long>(units, sms), kMxThreads, MxShape::kSmem, 1, true, mp, mq, msp, msq, a);
 }
 
 int launch_mx_pair(cudaStream_t stream, int sms, const MxSide& A, const MxSide& B, const MxGemmArgs& g) {
@@ -193,8 +201,8 @@ int launch_mx_pair(cudaStream_t stream, int sms, const MxSide& A, const MxSide& 
   a.m_tiles = (a.m + 255) / 256;
   a.n_tiles = (a.n + 255) / 256;
   const long long units = static_cast<long long>(a.m_tiles) * a.n_tiles * a.l;
-  return launch(stream, 2 * std::min<long long>(units, sms / 2), kMxPairThreads, kMxPairSmem, 2, true, mx_gemm_pair_kernel, ma, mb,
-                msa, msb, a);
+  return launch<mx_gemm_pair_kernel>(stream, 2 * std::min<long long>(units, sms / 2), kMxPairThreads, kMxPairSmem, 2, true, ma, mb,
+                                     msa, msb, a);
 }
 
 constexpr int kMxFewRows = 64;  // rows of A up to which the weights take the 128-row side of the MMA
@@ -261,7 +269,7 @@ int launch_mx_rows(cudaStream_t stream, int sms, bool overlap, const MxSide& W, 
   while (a.stages > 1 && S::smem(a.stages, a.blocks_per_split) > budget) --a.stages;
   const int smem = S::smem(a.stages, a.blocks_per_split);
   if (smem > limit) return fail(FBMM_ERR_INVALID, "internal: few-row kernel wants %d bytes of shared memory", smem);
-  return launch(stream, grid, S::kThreads, smem, a.splits, overlap, mx_rows_kernel<NT, T>, mw, msw, ma, msa, a);
+  return launch<mx_rows_kernel<NT, T>>(stream, grid, S::kThreads, smem, a.splits, overlap, mw, msw, ma, msa, a);
 }
 
 template <int NT>
@@ -357,8 +365,8 @@ int launch_x16(cudaStream_t stream, int sms, const CUtensorMap& mx, const CUtens
   a.x_tiles = (a.x.rows + kTile - 1) / kTile;
   a.y_tiles = (a.y.rows + kTile - 1) / kTile;
   const long long units = static_cast<long long>(a.x_tiles) * a.y_tiles * a.l;
-  return launch(stream, PAIR ? 2 * std::min<long long>(units, sms / 2) : std::min<long long>(units, sms), S::kThreads, S::kSmem,
-                PAIR ? 2 : 1, true, x16_gemm_kernel<XK, YK, PAIR>, mx, my, a);
+  return launch<x16_gemm_kernel<XK, YK, PAIR>>(stream, PAIR ? 2 * std::min<long long>(units, sms / 2) : std::min<long long>(units, sms),
+                                               S::kThreads, S::kSmem, PAIR ? 2 : 1, true, mx, my, a);
 }
 
 template <int XK, int YK>

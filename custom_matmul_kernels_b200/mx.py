@@ -6,6 +6,8 @@ narrow forms of the same batched product.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -326,6 +328,12 @@ class MXDenseBMMCUDA(CustomKernel):
         return C[0] if two_d else C
 
 
+@functools.lru_cache(maxsize=4096)
+def _product_workspace(l: int, m: int, n: int, k: int, layout: int) -> int:
+    """Scratch bytes of a product with a tensor; it depends on nothing but these."""
+    return load_library().fbmm_mx4_bmm_tensor_workspace_bytes(l, m, n, k, layout)
+
+
 def _mx4_product(A, B: MXTensor, out_dtype: torch.dtype) -> torch.Tensor:
     two_d = B.two_d
     n, k = B.rows, B.k
@@ -341,8 +349,7 @@ def _mx4_product(A, B: MXTensor, out_dtype: torch.dtype) -> torch.Tensor:
             _call("fbmm_mx4_bmm", t.get_device(), *A._arguments(), *B._arguments(), *result)
         else:
             t, layout, ld, step = _dense_layout(t)
-            query = "fbmm_mx4_bmm_tensor_workspace_bytes"
-            need = (_functions.get(query) or _function(query))(l, m, n, k, layout)
+            need = _product_workspace(l, m, n, k, layout)
             ws = t.new_empty(need, dtype=torch.uint8) if need else None
             _call("fbmm_mx4_bmm_tensor", t.get_device(), t.data_ptr(), _DTYPES[t.dtype], layout, ld, step, *B._arguments(),
                   *result, ws.data_ptr() if need else None, need)
