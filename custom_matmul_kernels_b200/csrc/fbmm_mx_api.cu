@@ -18,9 +18,10 @@ using fbmm_host::fail;
 
 int check_shape(int l, int rows, int k) {
   if (l <= 0 || rows <= 0 || k <= 0) return fail(FBMM_ERR_INVALID, "l, rows, k must be positive, got %d %d %d", l, rows, k);
-  const long long groups = static_cast<long long>(l) * ((rows + 127) / 128) * ((k + 127) / 128);
-  if (groups > 0x7fffffffLL) return fail(FBMM_ERR_INVALID, "matrix of %d x %d x %d is too large", l, rows, k);
+  // extents that tile arithmetic can round up, and scale groups that a grid can count
   if (k > (1 << 29) || rows > 0x7fffff00) return fail(FBMM_ERR_INVALID, "matrix of %d x %d is too large", rows, k);
+  const long long groups = static_cast<long long>((rows + 127) / 128) * ((k + 127) / 128);
+  if (groups > 0x7fffffffLL / l) return fail(FBMM_ERR_INVALID, "matrix of %d x %d x %d is too large", l, rows, k);
   return FBMM_OK;
 }
 
@@ -149,6 +150,7 @@ int launch(cudaStream_t stream, long long grid, int threads, int smem, int clust
   return FBMM_OK;
 }
 
+// A 4-bit operand [l][rows][k]; strides in bytes.
 struct MxSide {
   const unsigned char* codes;
   long long stride;
@@ -156,7 +158,6 @@ struct MxSide {
   long long scale_stride;
   int rows;
 };
-
 
 // Tensor map over scales [l][row groups][k groups][512]: boxes of two k groups x row_groups.
 int scales_map(CUtensorMap* map, const unsigned char* scales, long long stride, int l, int rows, int k, int row_groups) {
@@ -439,12 +440,12 @@ int mx_status(unsigned int* bits) {
 extern "C" {
 
 size_t fbmm_mx_codes_bytes(int l, int rows, int k, int bits) {
-  if (l <= 0 || rows <= 0 || k <= 0 || (bits != 4 && bits != 8)) return 0;
+  if (l <= 0 || rows <= 0 || k <= 0 || k > (1 << 29) || (bits != 4 && bits != 8)) return 0;
   return static_cast<size_t>(l) * rows * static_cast<size_t>(mx_pitch(k, bits));
 }
 
 size_t fbmm_mx_scales_bytes(int l, int rows, int k) {
-  if (l <= 0 || rows <= 0 || k <= 0) return 0;
+  if (l <= 0 || rows <= 0 || rows > 0x7fffff00 || k <= 0 || k > (1 << 29)) return 0;
   return static_cast<size_t>(l) * static_cast<size_t>(mx_scale_bytes(rows, k));
 }
 
@@ -504,7 +505,8 @@ int fbmm_mx4_bmm(void* stream, const unsigned char* a_codes, long long stride_a,
 }
 
 size_t fbmm_mx4_bmm_tensor_workspace_bytes(int l, int m, int n, int k, int a_layout) {
-  if (l <= 0 || m <= 0 || n <= 0 || k <= 0 || few_rows_fused(fbmm_host::sms_or_default(), l, m, n, k, a_layout)) return 0;
+  if (l <= 0 || m <= 0 || n <= 0 || k <= 0 || n > 0x7fffff00 || m > 0x7fffff00 || k > (1 << 29)) return 0;
+  if (few_rows_fused(fbmm_host::sms_or_default(), l, m, n, k, a_layout)) return 0;
   return (fbmm_mx_codes_bytes(l, m, k, 4) + 255) / 256 * 256 + fbmm_mx_scales_bytes(l, m, k);
 }
 

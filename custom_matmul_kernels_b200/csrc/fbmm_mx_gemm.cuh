@@ -124,7 +124,7 @@ __device__ __forceinline__ void mx_store_one(void* C, int out_type, long long at
 // (v0, v1) of a 16-bit type, or 32 columns of fp32 in two calls. The lanes' 16-byte pieces cross the
 // warp's staging area (piece index xor row, free of bank conflicts) so that every store instruction covers
 // four whole 128-byte lines; with 64-byte pieces of rows 16-bit results left at 2.0 TB/s (8192 x 8192 with
-// k = 256: 68 us, xxx with whole lines). `c0`: element (row 0, column 0) of the block.
+// k = 256: 68 us, 44 us with whole lines; a plain fill writes 3.9 TB/s). `c0`: element (row 0, column 0) of the block.
 template <typename Word>
 __device__ __forceinline__ void mx_store_lines(uint8_t* stage, Word word, void* C, long long c0, long long ldc, int size,
                                                int rows, int cols, bool vec) {

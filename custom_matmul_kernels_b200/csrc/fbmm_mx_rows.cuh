@@ -1,15 +1,16 @@
-// The 4-bit product for few rows of A (a decoding step): C[m][n] for m <= NT rows, and for tiles of 128 rows where
-// whole tiles are too few for the SMs. The weights fill the
-// 128-row side of the MMA and are streamed once, which is what bounds the product (17/32 byte per weight).
-// A comes as codes (T = uint8_t), copied beside the weights, or as fp32 / fp16 / bf16, which every CTA
-// quantises for its own range of k (fbmm_mx_quant.cuh's rules, straight into the swizzled tiles and scale
-// groups that the MMA reads) while the first weights are on their way: no separate pass, no
-// workspace, one launch, as long as there is little to quantise (few_rows_fused in fbmm_mx_api.cu).
+// The 4-bit product for few rows of A (a decoding step): C[m][n] for m <= NT rows, and for tiles of 128 rows
+// where whole tiles are too few for the SMs. The weights fill the 128-row side of the MMA and are streamed once,
+// which is what bounds the product (17/32 byte per weight). A comes as codes (T = uint8_t), copied beside the
+// weights, or as fp32 / fp16 / bf16, which every CTA quantises for its own range of k (fbmm_mx_quant.cuh's rules,
+// straight into the swizzled tiles and scale groups that the MMA reads) while the first weights are on their
+// way: no separate pass, no workspace, one launch, as long as there is little to quantise (few_rows_fused
+// in fbmm_mx_api.cu).
 //
 // Few tiles of n leave SMs idle, so k is split over a cluster of S CTAs; the partial sums meet in
 // shared memory and every CTA of the cluster adds up its share of the rows over the cluster in rank
-// order: the result does not depend on timing. One token at 4096 x 4096: 5.1 us
-// (9.2 us as a quantising pass and an unsplit product); 16 rows at n = 16384, k = 8192: 11.1 us, 6.4 TB/s of weights.
+// order: the result does not depend on timing. One token at 4096 x 4096: 5.4 us (9.2 us as a quantising pass and
+// an unsplit product); 16 rows at n = 16384, k = 8192: 10.9 us with weights partly in L2, 16.5 us from memory,
+// where longer weights stream at 6.5 TB/s behind 5 us of launch, set-up, first bytes and joining.
 //
 // Roles: warp 0 copies, warp 1 issues MMAs, the others quantise, then warps 2-5 read the sums.
 #pragma once
