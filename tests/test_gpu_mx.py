@@ -584,6 +584,56 @@ def test_operands_written_right_before(dev, m):
         assert float(d.min()) == float(d.max()) == float(torch.tensor(a * k).to(BF16)), i
 
 
+def test_offsets_past_32_bits(dev):
+    """Sources, codes and results of more than 2^32 bytes, looked at where they end."""
+    # quantised and back: 36000 x 131072, 4.7 GB of 8-bit codes, 9.4 GB on either side
+    rows, k = 36000, 1 << 17
+    X = torch.zeros((1, rows, k), device=dev, dtype=BF16)
+    X[0, -200:] = rnd((200, k), 5, BF16).to(dev)
+    q = MXQuantizeCUDA(8)(X)
+    want = MXQuantizeCUDA(8)(X[:, -200:].clone()).dequantize(BF16)
+    back = q.dequantize(BF16)
+    assert q.codes.numel() > 1 << 32
+    assert torch.equal(back[:, -200:], want) and not bool(back[:, -500:-200].any())
+    # the weights' gradient over all of it: only the last rows count
+    dC = torch.randn((1, rows, 64), device=dev, dtype=BF16)
+    got = MXDenseBMMCUDA()(q.mT, dC)
+    v, d = want.double().transpose(1, 2), dC[:, -200:].double()
+    assert_sum_close(got, (v @ d).cpu(), (v.abs() @ d.abs()).cpu(), 200, BF16)
+    del back, q, got, v
+    # weights of 4.7 GB of 4-bit codes: few rows and many
+    W = MXQuantizeCUDA(4)(X.expand(2, -1, -1).reshape(1, 2 * rows, k)).mT  # [1, k, 72000], both halves alike
+    assert W.codes.numel() > 1 << 32
+    del X
+    torch.cuda.empty_cache()
+    for m in (2, 130):
+        A = torch.randn((1, m, k), device=dev, dtype=BF16)
+        C = MXBMMCUDA()(A, W)
+        assert torch.equal(C[:, :, rows - 200:rows], C[:, :, -200:]) and bool(C[:, :, -200:].any())
+        assert not bool(C[:, :, rows:-200].any())
+    del W, C
+    torch.cuda.empty_cache()
+    # a result of 2.6e9 elements
+    m = n = 51000
+    A, B = rnd((1, m, 64), 1, BF16).to(dev), rnd((1, n, 64), 2, BF16).to(dev)
+    QA, QB = MXQuantizeCUDA(4)(A), MXQuantizeCUDA(4)(B).mT
+    C = MXBMMCUDA(out_dtype=BF16)(QA, QB)
+    tail = MXBMMCUDA(out_dtype=BF16)(MXQuantizeCUDA(4)(A[:, -300:].clone()), QB)
+    assert torch.equal(C[:, -300:], tail)
+    D = MXDenseBMMCUDA()(A, MXQuantizeCUDA(4)(B.transpose(1, 2).contiguous()))
+    tail = MXDenseBMMCUDA()(A[:, -300:].clone(), MXQuantizeCUDA(4)(B.transpose(1, 2).contiguous()))
+    assert torch.equal(D[:, -300:], tail)
+
+
+def test_product_with_itself_and_slices(dev):
+    X = rnd((4, 70, 96), 3, BF16).to(dev)
+    q = MXQuantizeCUDA(4)(X)
+    v = q.dequantize().double()
+    for A, a in ((q, v), (MXTensor(q.codes[1:3], q.scales[1:3], k=96), v[1:3])):
+        C = MXBMMCUDA()(A, A.mT)
+        assert_sum_close(C, (a @ a.transpose(1, 2)).cpu(), (a.abs() @ a.abs().transpose(1, 2)).cpu(), 96, F32)
+
+
 def test_library_reports_no_trouble(dev, lib):
     assert lib.fbmm_check(None) == 0, lib.fbmm_last_error()
 
