@@ -301,15 +301,18 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     int turn = static_cast<int>(warp - 2) >> 2;  // stages until this group's next one
     for (long long u = u0; u < units && ok; u += du)
       for (int jb = 0; jb < jblocks; ++jb) {
+        // Every group waits for every stage's codes, its own turn or not: copies land out of order, and a group that
+        // only looked at its own stages could come to a barrier a whole round early and take the phase before the
+        // unfinished one for the one it wants.
+        ok = mbar_wait(&bars->raw[stage], phase, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         if (turn != 0) {
           --turn;
           if (++stage == kX16Stages) { stage = 0; phase ^= 1u; }
           continue;
         }
         turn = kX16Expanders - 1;
-        ok = mbar_wait(&bars->raw[stage], phase, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
         uint8_t* st = smem + stage * S::kStageBytes;
         uint8_t* dst = st + (XK >= kX16Mx4 ? 0 : kX16Part);
         if (a.dtype == 2) x16_expand<S::kBits, true>(st + 2 * kX16Part, dst, jb * kX16J, a.J, tid);

@@ -360,6 +360,23 @@ def test_dense_product_many_tiles(dev, dtype, bits):
                 assert_sum_close(got.detach(), (x @ y).cpu(), (x.abs() @ y.abs()).cpu(), x.shape[2], dtype)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("l,m,j,c", [(7, 6, 86, 14244), (7, 23, 199, 5477), (3, 500, 70, 2900)])
+def test_dense_product_short_sums(dev, l, m, j, c, bits):
+    """Many tiles of one to four stages each: the expanding warps' groups overtake one another at every turn."""
+    P = rnd((l, m, j), 3, BF16, 0.3).to(dev)
+    Q = MXQuantizeCUDA(bits)(rnd((l, j, c), 4, BF16, 0.3).to(dev))
+    q, p = Q.dequantize().double(), P.double()
+    want, mag = (p @ q).cpu(), (p.abs() @ q.abs()).cpu()
+    first = MXDenseBMMCUDA()(P, Q)
+    assert_sum_close(first, want, mag, j, BF16)
+    flipped = MXDenseBMMCUDA()(Q.mT, P.transpose(1, 2))
+    assert_sum_close(flipped, want.transpose(1, 2), mag.transpose(1, 2), j, BF16)
+    for _ in range(40):
+        assert torch.equal(MXDenseBMMCUDA()(P, Q), first)
+        assert torch.equal(MXDenseBMMCUDA()(Q.mT, P.transpose(1, 2)), flipped)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("l,m,n,k", [(1, 5, 40, 64), (2, 130, 200, 300)])
 def test_frozen_weights_gradient(dev, l, m, n, k, dtype):
