@@ -332,10 +332,34 @@ int check_x16_side(const char* name, const X16Side& s, int J, int l) {
   if (s.ptr == nullptr) return fail(FBMM_ERR_INVALID, "%s is null", name);
   const int inner = s.kind == kX16K ? J : s.rows;
   if (s.ld < inner) return fail(FBMM_ERR_INVALID, "%s pitch %lld smaller than its row length %d", name, s.ld, inner);
-  if ((reinterpret_cast<uintptr_t>(s.ptr) & 15u) != 0) return fail(FBMM_ERR_ALIGN, "%s is not 16-byte aligned", name);
-  if ((s.ld & 7) != 0) return fail(FBMM_ERR_ALIGN, "%s pitch %lld is not a multiple of 8 elements", name, s.ld);
-  if (l > 1 && ((s.stride & 7) != 0 || s.stride < 0))
-    return fail(FBMM_ERR_ALIGN, "%s batch stride %lld is not a non-negative multiple of 8 elements", name, s.stride);
+  if ((reinterpret_cast<uintptr_t>(s.ptr) & 1u) != 0) return fail(FBMM_ERR_ALIGN, "%s is not 2-byte aligned", name);
+  if (l > 1 && s.stride < 0) return fail(FBMM_ERR_INVALID, "%s batch stride is negative", name);
+  return FBMM_OK;
+}
+
+// Scratch for a dense operand that tensor maps cannot describe (base, pitch or batch stride not a multiple of 16
+// bytes); 0 for one that they can.
+size_t repack_bytes(const void* ptr, long long ld, long long stride, int l, int outer, int inner) {
+  const bool batched = l > 1 && stride != 0;
+  if (((reinterpret_cast<uintptr_t>(ptr) | static_cast<uint64_t>(ld * 2) | (batched ? static_cast<uint64_t>(stride * 2) : 0)) & 15) == 0)
+    return 0;
+  const size_t pitch = (static_cast<size_t>(inner) + 7) / 8 * 8;
+  return ((batched ? static_cast<size_t>(l) : 1) * outer * pitch * 2 + 255) / 256 * 256;
+}
+
+// Repacks such an operand into `need` bytes of the workspace and makes the side describe the copy.
+int repack_side(cudaStream_t stream, X16Side* s, int J, int l, size_t need, unsigned char** ws) {
+  const int outer = s->kind == kX16K ? s->rows : J, inner = s->kind == kX16K ? J : s->rows;
+  const bool batched = l > 1 && s->stride != 0;
+  const int pitch = (inner + 7) / 8 * 8;
+  const long long pieces = static_cast<long long>(batched ? l : 1) * outer * (pitch / 8);
+  x16_repack_kernel<<<static_cast<unsigned>(std::min<long long>((pieces + 255) / 256, 1 << 20)), 256, 0, stream>>>(
+      static_cast<const uint16_t*>(s->ptr), s->ld, batched ? s->stride : 0, reinterpret_cast<uint16_t*>(*ws), outer, inner, pitch, pieces);
+  FBMM_HOST_CUDA(cudaGetLastError());
+  s->ptr = *ws;
+  s->ld = pitch;
+  s->stride = batched ? static_cast<long long>(outer) * pitch : 0;
+  *ws += need;
   return FBMM_OK;
 }
 
@@ -382,8 +406,8 @@ int launch_x16_any(cudaStream_t stream, int sms, const CUtensorMap& mx, const CU
   return launch_x16<XK, YK, false>(stream, sms, mx, my, a);
 }
 
-int x16_product(cudaStream_t stream, const X16Side& x, const X16Side& y, int dtype, void* C, long long ldc,
-                long long stride_c, int l, int J, const char* xn, const char* yn) {
+int x16_product(cudaStream_t stream, X16Side x, X16Side y, int dtype, void* C, long long ldc, long long stride_c, int l, int J,
+                void* workspace, size_t workspace_bytes) {
   int rc, sms;
   if (l <= 0 || x.rows <= 0 || y.rows <= 0 || J <= 0)
     return fail(FBMM_ERR_INVALID, "l, m, n, k must be positive, got %d %d %d %d", l, x.rows, y.rows, J);
@@ -391,10 +415,22 @@ int x16_product(cudaStream_t stream, const X16Side& x, const X16Side& y, int dty
     return fail(FBMM_ERR_INVALID, "product of %d x %d x %d is too large", x.rows, y.rows, J);
   if (dtype != FBMM_F16 && dtype != FBMM_BF16)
     return fail(FBMM_ERR_INVALID, "dtype must be FBMM_F16 (1) or FBMM_BF16 (2), got %d", dtype);
-  if ((rc = check_x16_side(xn, x, J, l)) != FBMM_OK) return rc;
-  if ((rc = check_x16_side(yn, y, J, l)) != FBMM_OK) return rc;
+  if ((rc = check_x16_side("A", x, J, l)) != FBMM_OK) return rc;
+  if ((rc = check_x16_side("B", y, J, l)) != FBMM_OK) return rc;
   if ((rc = check_result(C, dtype, ldc, stride_c, l, x.rows, y.rows)) != FBMM_OK) return rc;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return fail(FBMM_ERR_ALIGN, "workspace is not 16-byte aligned");
+  // refused before a device is asked for
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  const size_t need_x = x.kind >= kX16Mx4 ? 0 : repack_bytes(x.ptr, x.ld, x.stride, l, x.kind == kX16K ? x.rows : J, x.kind == kX16K ? J : x.rows);
+  const size_t need_y = y.kind >= kX16Mx4 ? 0 : repack_bytes(y.ptr, y.ld, y.stride, l, y.kind == kX16K ? y.rows : J, y.kind == kX16K ? J : y.rows);
+  if (need_x + need_y > 0 && ws == nullptr)
+    return fail(FBMM_ERR_ALIGN, "%s is not addressable (16-byte base, pitch and batch stride) and there is no workspace to repack it in",
+                need_x ? "A" : "B");
+  if (need_x + need_y > 0 && workspace_bytes < need_x + need_y)
+    return fail(FBMM_ERR_WORKSPACE, "repacking needs %zu workspace bytes, got %zu", need_x + need_y, workspace_bytes);
   if ((rc = fbmm_host::device_sms(&sms)) != FBMM_OK) return rc;
+  if (need_x && (rc = repack_side(stream, &x, J, l, need_x, &ws)) != FBMM_OK) return rc;
+  if (need_y && (rc = repack_side(stream, &y, J, l, need_y, &ws)) != FBMM_OK) return rc;
   CUtensorMap mx, my;
   if ((rc = x16_map(&mx, x, J, l, dtype)) != FBMM_OK) return rc;
   if ((rc = x16_map(&my, y, J, l, dtype)) != FBMM_OK) return rc;
@@ -543,36 +579,44 @@ int fbmm_mx4_bmm_tensor(void* stream, const void* A, int a_dtype, int a_layout, 
                      mx_scale_bytes(m, k), b_codes, stride_b, b_scales, stride_bs, C, dtype, ldc, stride_c, l, m, n, k);
 }
 
+size_t fbmm_x16_repack_bytes(const void* X, long long ld, long long stride, int l, int outer, int inner) {
+  if (l <= 0 || outer <= 0 || inner <= 0) return 0;
+  return repack_bytes(X, ld, stride, l, outer, inner);
+}
+
 int fbmm_dense_bmm_x16(void* stream, const void* A, int a_layout, long long lda, long long stride_a, const void* B,
                        int b_layout, long long ldb, long long stride_b, int dtype, void* C, long long ldc,
-                       long long stride_c, int l, int m, int n, int k) {
+                       long long stride_c, int l, int m, int n, int k, void* workspace,
+                       size_t workspace_bytes) {
   X16Side x{0, A, lda, stride_a, nullptr, 0, m}, y{0, B, ldb, stride_b, nullptr, 0, n};
   int rc;
   if ((rc = layout_kind("A", a_layout, 'n', &x.kind)) != FBMM_OK) return rc;
   if ((rc = layout_kind("B", b_layout, 't', &y.kind)) != FBMM_OK) return rc;
-  return x16_product(static_cast<cudaStream_t>(stream), x, y, dtype, C, ldc, stride_c, l, k, "A", "B");
+  return x16_product(static_cast<cudaStream_t>(stream), x, y, dtype, C, ldc, stride_c, l, k, workspace, workspace_bytes);
 }
 
 int fbmm_dense_mx_bmm_x16(void* stream, const void* A, int a_layout, long long lda, long long stride_a, int dtype,
                           const unsigned char* b_codes, long long stride_b, const unsigned char* b_scales,
                           long long stride_bs, int bits, void* C, long long ldc, long long stride_c, int l, int m, int n,
-                          int k) {
+                          int k, void* workspace,
+                       size_t workspace_bytes) {
   int rc;
   if ((rc = check_bits(bits)) != FBMM_OK) return rc;
   X16Side x{0, A, lda, stride_a, nullptr, 0, m};
   const X16Side y{bits == 4 ? kX16Mx4 : kX16Mx8, b_codes, 0, stride_b, b_scales, stride_bs, n};
   if ((rc = layout_kind("A", a_layout, 'n', &x.kind)) != FBMM_OK) return rc;
-  return x16_product(static_cast<cudaStream_t>(stream), x, y, dtype, C, ldc, stride_c, l, k, "A", "B");
+  return x16_product(static_cast<cudaStream_t>(stream), x, y, dtype, C, ldc, stride_c, l, k, workspace, workspace_bytes);
 }
 
 int fbmm_mx_dense_bmm_x16(void* stream, const unsigned char* a_codes, long long stride_a, const unsigned char* a_scales,
                           long long stride_as, int bits, const void* B, long long ldb, long long stride_b, int dtype,
-                          void* C, long long ldc, long long stride_c, int l, int m, int n, int k) {
+                          void* C, long long ldc, long long stride_c, int l, int m, int n, int k, void* workspace,
+                       size_t workspace_bytes) {
   int rc;
   if ((rc = check_bits(bits)) != FBMM_OK) return rc;
   const X16Side x{bits == 4 ? kX16Mx4 : kX16Mx8, a_codes, 0, stride_a, a_scales, stride_as, m};
   const X16Side y{kX16MN, B, ldb, stride_b, nullptr, 0, n};
-  return x16_product(static_cast<cudaStream_t>(stream), x, y, dtype, C, ldc, stride_c, l, k, "A", "B");
+  return x16_product(static_cast<cudaStream_t>(stream), x, y, dtype, C, ldc, stride_c, l, k, workspace, workspace_bytes);
 }
 
 }  // extern "C"

@@ -375,4 +375,26 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   }
 }
 
+// Rows of `cols` 16-bit elements at any alignment -> rows padded to `pitch` (a multiple of 8) elements, zeros in the
+// padding: what the tensor maps of operands with odd pitches or bases are made over. Eight elements a thread.
+__global__ void __launch_bounds__(256) x16_repack_kernel(const uint16_t* __restrict__ src, long long ld, long long stride,
+                                                         uint16_t* __restrict__ dst, int rows, int cols, int pitch, long long pieces) {
+  mx_let_next_start();
+  const int per_row = pitch / 8;
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < pieces;
+       i += static_cast<long long>(gridDim.x) * 256) {
+    const long long row = i / per_row;  // over all batches
+    const int c = static_cast<int>(i - row * per_row) * 8;
+    const long long b = row / rows;
+    const uint16_t* p = src + b * stride + (row - b * rows) * ld + c;
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t lo = c + 2 * j < cols ? __ldg(p + 2 * j) : 0u, hi = c + 2 * j + 1 < cols ? __ldg(p + 2 * j + 1) : 0u;
+      w[j] = lo | (hi << 16);
+    }
+    *reinterpret_cast<uint4*>(dst + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 }  // namespace fbmm

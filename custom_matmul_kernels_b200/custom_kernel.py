@@ -106,11 +106,12 @@ SIGNATURES = {
     "fbmm_mx4_bmm_tensor_workspace_bytes": (_c_size, [_c_int] * 5),
     "fbmm_mx4_bmm_tensor": (_c_int, [_c_ptr, _c_ptr, _c_int, _c_int, _c_ll, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_ptr,
                                      _c_int, _c_ll, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_size]),
-    "fbmm_dense_bmm_x16": (_c_int, [_c_ptr] + _OPERANDS + [_c_int, _c_ptr, _c_ll, _c_ll] + [_c_int] * 4),
+    "fbmm_x16_repack_bytes": (_c_size, [_c_ptr, _c_ll, _c_ll, _c_int, _c_int, _c_int]),
+    "fbmm_dense_bmm_x16": (_c_int, [_c_ptr] + _OPERANDS + [_c_int, _c_ptr, _c_ll, _c_ll] + [_c_int] * 4 + [_c_ptr, _c_size]),
     "fbmm_dense_mx_bmm_x16": (_c_int, [_c_ptr, _c_ptr, _c_int, _c_ll, _c_ll, _c_int, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_int,
-                                       _c_ptr, _c_ll, _c_ll] + [_c_int] * 4),
+                                       _c_ptr, _c_ll, _c_ll] + [_c_int] * 4 + [_c_ptr, _c_size]),
     "fbmm_mx_dense_bmm_x16": (_c_int, [_c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_int, _c_ptr, _c_ll, _c_ll, _c_int,
-                                       _c_ptr, _c_ll, _c_ll] + [_c_int] * 4),
+                                       _c_ptr, _c_ll, _c_ll] + [_c_int] * 4 + [_c_ptr, _c_size]),
 }
 
 _lib = None

@@ -68,20 +68,16 @@ def _dense_layout(X: torch.Tensor):
     return X.contiguous(), _N, c, r * c
 
 
-def _aligned_layout(X: torch.Tensor):
-    """The same for the 16-bit products, whose copies need 16-byte aligned bases, pitches and batch
-    strides: other storage is copied to rows padded to 8 elements."""
-    X, letter, ld, sl = _dense_layout(X)
+def _x16_layout(X: torch.Tensor):
+    """The same with the bytes of workspace that the 16-bit products repack it in: 0 for storage that
+    their copies can address (base, pitch and batch stride multiples of 16 bytes)."""
+    X, letter, ld, step = _dense_layout(X)
     l, r, c = X.shape
-    if X.data_ptr() % 16 == 0 and ld % 8 == 0 and (l == 1 or (sl % 8 == 0 and sl >= 0)):
-        return X, letter, ld, sl
-    if letter == _T:
-        r, c = c, r
-        X = X.transpose(1, 2)
-    cp = (c + 7) // 8 * 8
-    buf = torch.empty((l, r, cp), dtype=X.dtype, device=X.device)
-    buf[:, :, :c] = X  # the padding is behind the extents that the kernels are given, never read
-    return buf, letter, cp, r * cp
+    batched = l > 1 and step != 0
+    if X.data_ptr() % 16 == 0 and ld % 8 == 0 and not (batched and step % 8):
+        return X, letter, ld, step, 0
+    outer, inner = (r, c) if letter == _N else (c, r)
+    return X, letter, ld, step, ((l if batched else 1) * outer * ((inner + 7) // 8 * 16) + 255) // 256 * 256
 
 
 class MXTensor:
@@ -285,10 +281,12 @@ def _dense_bmm(A: torch.Tensor, B: torch.Tensor) -> torch.Tensor:
     n = B.shape[2]
     C = A.new_empty((l, m, n))
     if l and m and n:
-        a, la, lda, sa = _aligned_layout(A)
-        b, lb, ldb, sb = _aligned_layout(B)
+        a, la, lda, sa, need_a = _x16_layout(A)
+        b, lb, ldb, sb, need_b = _x16_layout(B)
+        need = need_a + need_b
+        ws = A.new_empty(need, dtype=torch.uint8) if need else None
         _call("fbmm_dense_bmm_x16", A.get_device(), a.data_ptr(), la, lda, sa, b.data_ptr(), lb, ldb, sb, _DTYPES[A.dtype],
-              C.data_ptr(), n, m * n, l, m, n, k)
+              C.data_ptr(), n, m * n, l, m, n, k, ws.data_ptr() if need else None, need)
     return C
 
 
@@ -315,16 +313,18 @@ class MXDenseBMMCUDA(CustomKernel):
         C = D.new_empty((l, m, n))
         if C.numel() == 0 or k == 0:
             C.zero_()
-        elif mx is B:
-            d, letter, ld, step = _aligned_layout(D)
-            _call("fbmm_dense_mx_bmm_x16", D.get_device(), d.data_ptr(), letter, ld, step, _DTYPES[D.dtype], *mx._arguments(),
-                  mx.bits, C.data_ptr(), n, m * n, l, m, n, k)
         else:
-            d, letter, ld, step = _aligned_layout(D)
-            if letter != _N:
-                d, letter, ld, step = _aligned_layout(D.contiguous())
-            _call("fbmm_mx_dense_bmm_x16", D.get_device(), *mx._arguments(), mx.bits, d.data_ptr(), ld, step, _DTYPES[D.dtype],
-                  C.data_ptr(), n, m * n, l, m, n, k)
+            d, letter, ld, step, need = _x16_layout(D)
+            if mx is A and letter != _N:
+                d, letter, ld, step, need = _x16_layout(D.contiguous())
+            ws = D.new_empty(need, dtype=torch.uint8) if need else None
+            tail = C.data_ptr(), n, m * n, l, m, n, k, ws.data_ptr() if need else None, need
+            if mx is B:
+                _call("fbmm_dense_mx_bmm_x16", D.get_device(), d.data_ptr(), letter, ld, step, _DTYPES[D.dtype],
+                      *mx._arguments(), mx.bits, *tail)
+            else:
+                _call("fbmm_mx_dense_bmm_x16", D.get_device(), *mx._arguments(), mx.bits, d.data_ptr(), ld, step,
+                      _DTYPES[D.dtype], *tail)
         return C[0] if two_d else C
 
 

@@ -328,25 +328,30 @@ int fbmm_mx4_bmm_tensor(void* stream, const void* A, int a_dtype, int a_layout, 
                         int k, void* workspace, size_t workspace_bytes);
 
 /* 16-bit products (dtype FBMM_F16 / FBMM_BF16, fp32 sums, C [l][m][n] in the same type) in the layouts
- * that a training step meets, without a transposed copy of any operand. Dense operands: either
- * layout letter, bases 16-byte aligned, pitches and batch strides (elements) multiples of 8.
- *  - fbmm_dense_bmm_x16: A [m, k] @ B [k, n].
+ * that a training step meets, without a transposed copy of any operand.
+ *  - fbmm_dense_bmm_x16: A [m, k] @ B [k, n], either layout letter each.
  *  - fbmm_dense_mx_bmm_x16: B is microscaled, stored [k][n] with its blocks along n (what
  *    fbmm_mx_quantize makes of rows = k, k = n).
  *  - fbmm_mx_dense_bmm_x16: A is microscaled, stored [k][m] with its blocks along m; B stored
  *    [k][n], n contiguous.
  * A microscaled element enters as element * scale rounded to dtype: exact for bf16, and for fp16
- * wherever it is an fp16 value (always, if it was quantised from fp16 at 8 bits). */
+ * wherever it is an fp16 value (always, if it was quantised from fp16 at 8 bits).
+ * Dense operands are read where they lie when base, pitch and batch stride are multiples of 16 bytes. Any
+ * other is first repacked into the caller's workspace (16-byte aligned), which has to have the sum of the
+ * operands' fbmm_x16_repack_bytes (`outer` stored rows of `inner` elements; 0 where nothing is repacked);
+ * without a workspace such an operand is FBMM_ERR_ALIGN. */
+size_t fbmm_x16_repack_bytes(const void* X, long long ld, long long stride, int l, int outer, int inner);
 int fbmm_dense_bmm_x16(void* stream, const void* A, int a_layout, long long lda, long long stride_a, const void* B,
                        int b_layout, long long ldb, long long stride_b, int dtype, void* C, long long ldc,
-                       long long stride_c, int l, int m, int n, int k);
+                       long long stride_c, int l, int m, int n, int k, void* workspace, size_t workspace_bytes);
 int fbmm_dense_mx_bmm_x16(void* stream, const void* A, int a_layout, long long lda, long long stride_a, int dtype,
                           const unsigned char* b_codes, long long stride_b, const unsigned char* b_scales,
                           long long stride_bs, int bits, void* C, long long ldc, long long stride_c,
-                          int l, int m, int n, int k);
+                          int l, int m, int n, int k, void* workspace, size_t workspace_bytes);
 int fbmm_mx_dense_bmm_x16(void* stream, const unsigned char* a_codes, long long stride_a, const unsigned char* a_scales,
                           long long stride_as, int bits, const void* B, long long ldb, long long stride_b, int dtype,
-                          void* C, long long ldc, long long stride_c, int l, int m, int n, int k);
+                          void* C, long long ldc, long long stride_c, int l, int m, int n, int k, void* workspace,
+                          size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

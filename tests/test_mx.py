@@ -120,19 +120,29 @@ def test_product_refusals(lib):
 def test_dense_refusals(lib):
     n, t = ord("n"), ord("t")
 
-    def dense(A=OK_PTR, la=n, lda=64, sa=512, B=OK_PTR, lb=n, ldb=8, sb=512, dtype=2, C=OK_PTR, ldc=8, sc=64, l=1, m=8, nn=8, k=64):
-        return lib.fbmm_dense_bmm_x16(None, A, la, lda, sa, B, lb, ldb, sb, dtype, C, ldc, sc, l, m, nn, k)
+    def dense(A=OK_PTR, la=n, lda=64, sa=512, B=OK_PTR, lb=n, ldb=8, sb=512, dtype=2, C=OK_PTR, ldc=8, sc=64, l=1, m=8, nn=8, k=64,
+              ws=None, size=0):
+        return lib.fbmm_dense_bmm_x16(None, A, la, lda, sa, B, lb, ldb, sb, dtype, C, ldc, sc, l, m, nn, k, ws, size)
 
     for kw in ({"A": None}, {"la": 0}, {"lda": 56}, {"lb": t, "ldb": 56}, {"dtype": 0}, {"C": None}, {"ldc": 7}, {"l": 2, "sc": 10},
                {"k": 0}, {"la": t, "lda": 0}):
         assert dense(**kw) == ck.FBMM_ERR_INVALID, kw
-    for kw in ({"A": OK_PTR + 8}, {"lda": 65}, {"l": 2, "sb": 4}, {"l": 2, "sa": -8}, {"C": OK_PTR + 1}):
+    assert dense(l=2, sa=-8) == ck.FBMM_ERR_INVALID
+    for kw in ({"A": OK_PTR + 1}, {"C": OK_PTR + 1}, {"ws": OK_PTR + 8, "size": 1 << 20}):
         assert dense(**kw) == ck.FBMM_ERR_ALIGN, kw
-    rc = lib.fbmm_dense_mx_bmm_x16(None, OK_PTR, n, 64, 512, 2, OK_PTR, 256, OK_PTR, 512, 3, OK_PTR, 8, 64, 1, 8, 8, 64)
+    # storage that needs repacking: refused without a workspace, or with one that is too small
+    for kw, bytes_ in (({"A": OK_PTR + 8}, 8 * 64 * 2), ({"lda": 65}, 8 * 64 * 2), ({"l": 2, "sb": 4}, 2 * 64 * 8 * 2)):
+        assert dense(**kw) == ck.FBMM_ERR_ALIGN, kw
+        assert dense(ws=OK_PTR, size=bytes_ - 1, **kw) == ck.FBMM_ERR_WORKSPACE, kw
+    assert lib.fbmm_x16_repack_bytes(OK_PTR, 64, 512, 2, 8, 60) == 0
+    assert lib.fbmm_x16_repack_bytes(OK_PTR, 61, 488, 2, 8, 60) == 2 * 8 * 64 * 2
+    assert lib.fbmm_x16_repack_bytes(OK_PTR, 61, 0, 2, 8, 60) == 8 * 64 * 2  # one matrix for every batch
+    assert lib.fbmm_x16_repack_bytes(OK_PTR, 64, 4, 1, 8, 60) == 0 and lib.fbmm_x16_repack_bytes(OK_PTR, 64, 4, 0, 8, 60) == 0
+    rc = lib.fbmm_dense_mx_bmm_x16(None, OK_PTR, n, 64, 512, 2, OK_PTR, 256, OK_PTR, 512, 3, OK_PTR, 8, 64, 1, 8, 8, 64, None, 0)
     assert rc == ck.FBMM_ERR_INVALID and b"bits" in lib.fbmm_last_error()
-    rc = lib.fbmm_dense_mx_bmm_x16(None, OK_PTR, n, 64, 512, 2, OK_PTR + 8, 256, OK_PTR, 512, 4, OK_PTR, 8, 64, 1, 8, 8, 64)
+    rc = lib.fbmm_dense_mx_bmm_x16(None, OK_PTR, n, 64, 512, 2, OK_PTR + 8, 256, OK_PTR, 512, 4, OK_PTR, 8, 64, 1, 8, 8, 64, None, 0)
     assert rc == ck.FBMM_ERR_ALIGN
-    rc = lib.fbmm_mx_dense_bmm_x16(None, None, 256, OK_PTR, 512, 8, OK_PTR, 8, 64, 1, OK_PTR, 8, 64, 1, 8, 8, 64)
+    rc = lib.fbmm_mx_dense_bmm_x16(None, None, 256, OK_PTR, 512, 8, OK_PTR, 8, 64, 1, OK_PTR, 8, 64, 1, 8, 8, 64, None, 0)
     assert rc == ck.FBMM_ERR_INVALID
 
 
