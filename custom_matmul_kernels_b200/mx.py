@@ -3,6 +3,10 @@ that read them, and a training product that keeps its activations in 8 bits.
 
 The reference stops at fp32 (its kernels take float* only, kernels/bmm.cu:185); these are the
 narrow forms of the same batched product.
+
+All calls work on the stream that is current on their tensors' device and can be captured into CUDA
+graphs, backward passes too. As for every torch operation, an eager graph of the same leaves must
+not be alive while a backward pass is captured: torch then ends the capture with an error.
 """
 from __future__ import annotations
 

@@ -318,9 +318,9 @@ int fbmm_mx4_bmm(void* stream, const unsigned char* a_codes, long long stride_a,
                  long long stride_as, const unsigned char* b_codes, long long stride_b, const unsigned char* b_scales,
                  long long stride_bs, void* C, int dtype, long long ldc, long long stride_c, int l, int m, int n, int k);
 /* The same product with A a dense matrix of any FBMM_* element type and layout ('n' [l][m][k] or 't'
- * [l][k][m]), quantised on the way (fbmm_mx_quantize's rules at 4 bits). Up to 64 rows of A in layout 'n' take one
- * kernel and no workspace (the query then answers 0, except for a k of tens of thousands); otherwise the
- * workspace holds the quantised A, 16-byte aligned. */
+ * [l][k][m]), quantised on the way (fbmm_mx_quantize's rules at 4 bits). Few rows of A in layout 'n' are quantised
+ * inside the product, in one kernel without a workspace (the query answers 0 then); otherwise the workspace,
+ * 16-byte aligned, holds the quantised A. */
 size_t fbmm_mx4_bmm_tensor_workspace_bytes(int l, int m, int n, int k, int a_layout);
 int fbmm_mx4_bmm_tensor(void* stream, const void* A, int a_dtype, int a_layout, long long lda, long long stride_a,
                         const unsigned char* b_codes, long long stride_b, const unsigned char* b_scales,
