@@ -29,7 +29,8 @@ enum X16Kind { kX16K = 0, kX16MN = 1, kX16Mx4 = 2, kX16Mx8 = 3 };
 constexpr int kX16J = 64;                   // j per stage: 128 bytes of a K-major row
 constexpr int kX16Part = 128 * kX16J * 2;   // 16 KB: 128 rows of one operand
 constexpr int kX16Stages = 5;
-constexpr int kX16Expanders = 3;            // groups of four warps that expand codes, each its own stages
+constexpr int kX16Expanders = 3;            // groups of four warps that expand codes, in turn
+static_assert(kX16Expanders <= kX16Stages, "a group's stages must not be further apart than the ring");
 constexpr int kX16Chunk = 64 * kX16J * 2;   // MN-major: 64 rows x 64 j
 
 struct X16Operand {
@@ -301,18 +302,19 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     int turn = static_cast<int>(warp - 2) >> 2;  // stages until this group's next one
     for (long long u = u0; u < units && ok; u += du)
       for (int jb = 0; jb < jblocks; ++jb) {
-        // Every group waits for every stage's codes, its own turn or not: copies land out of order, and a group that
-        // only looked at its own stages could come to a barrier a whole round early and take the phase before the
-        // unfinished one for the one it wants.
-        ok = mbar_wait(&bars->raw[stage], phase, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
         if (turn != 0) {
           --turn;
           if (++stage == kX16Stages) { stage = 0; phase ^= 1u; }
           continue;
         }
         turn = kX16Expanders - 1;
+        // First the stage's release by its last use, as the copies wait for it. Copies land out of order, and the last
+        // use was another group's: with the codes' barrier alone a group could come a round early and take
+        // the phase before the unfinished one for the one it wants. (The release itself is never a round behind: this
+        // group's last stage was loaded, so the MMAs eight stages back, and all before them, are done.)
+        ok = wait(&bars->empty[stage], phase ^ 1u) && mbar_wait(&bars->raw[stage], phase, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         uint8_t* st = smem + stage * S::kStageBytes;
         uint8_t* dst = st + (XK >= kX16Mx4 ? 0 : kX16Part);
         if (a.dtype == 2) x16_expand<S::kBits, true>(st + 2 * kX16Part, dst, jb * kX16J, a.J, tid);
