@@ -113,20 +113,53 @@ int codes_map(CUtensorMap* map, const unsigned char* codes, long long stride, in
   return fbmm_host::tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, dims, strides, box, true);
 }
 
+constexpr int kMxMaxSplits = 8;  // CTAs that share a tile's sum: the portable cluster size
+
+// The kernel's shared-memory limit is set once per device.
+template <auto kKernel>
+int prepare(int* dev) {
+  static std::atomic<unsigned long long> ready{0};
+  FBMM_HOST_CUDA(cudaGetDevice(dev));
+  const unsigned long long bit = 1ull << (*dev & 63);
+  if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
+    FBMM_HOST_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMxSmemLimit)));
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  return FBMM_OK;
+}
+
+// How many clusters of this size run at once: fewer than the SMs divided by it, since a cluster stays within a group
+// of SMs (15 clusters of eight on 148 SMs). Asked once per device and size.
+template <auto kKernel>
+int clusters_at_once(int threads, int smem, int cluster, int* count) {
+  static std::atomic<int> known[64][kMxMaxSplits + 1];  // count + 1
+  int rc, dev = 0;
+  if ((rc = prepare<kKernel>(&dev)) != FBMM_OK) return rc;
+  std::atomic<int>& slot = known[dev & 63][cluster];
+  *count = slot.load(std::memory_order_relaxed) - 1;
+  if (*count >= 0) return FBMM_OK;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(cluster));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  FBMM_HOST_CUDA(cudaOccupancyMaxActiveClusters(count, kKernel, &cfg));
+  slot.store(*count + 1, std::memory_order_relaxed);
+  return FBMM_OK;
+}
+
 // A launch with a cluster and the right to start (set up barriers and tensor memory) before the kernel ahead of it
 // in the stream has ended. Kernels whose copies all wait for that kernel always have it; the few-row kernel,
 // which asks for weights before it waits, only behind a quantiser, which cannot be writing them.
 template <auto kKernel, typename... Args>
 int launch(cudaStream_t stream, long long grid, int threads, int smem, int cluster, bool overlap, const Args&... args) {
-  // the kernel's shared-memory limit is set once per device
-  static std::atomic<unsigned long long> ready{0};
-  int dev = 0;
-  FBMM_HOST_CUDA(cudaGetDevice(&dev));
-  const unsigned long long bit = 1ull << (dev & 63);
-  if ((ready.load(std::memory_order_relaxed) & bit) == 0) {
-    FBMM_HOST_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMxSmemLimit)));
-    ready.fetch_or(bit, std::memory_order_relaxed);
-  }
+  int rc, dev = 0;
+  if ((rc = prepare<kKernel>(&dev)) != FBMM_OK) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
@@ -217,10 +250,12 @@ void rows_splits(int sms, int l, int m, int n, int k, int* splits, int* blocks) 
   const int kblocks = (k + kMxStageK - 1) / kMxStageK;
   const bool tall = m > kMxFewRows;
   const long long base = static_cast<long long>((n + kMxM - 1) / kMxM) * l * (tall ? (m + 127) / 128 : 1);
-  const long long slots = tall ? sms : 2ll * sms;
   long long best = 0;
-  for (int s = 1; s <= 8 && (s == 1 || s <= kblocks); s *= 2) {
-    const long long ctas = base * s, per = (kblocks + s - 1) / s;
+  for (int s = 1; s <= kMxMaxSplits && (s == 1 || s <= kblocks); s *= 2) {
+    // a cluster stays within a group of SMs: of four and eight 33 and 15 run at once on 148 SMs, with two
+    // CTAs to an SM 71 and 33 (128 rows, n = 2048, k = 8192: 9.3 us in fours against 14.8 in eights, two waves)
+    const int permille = s <= 2 ? 1000 : tall ? (s == 4 ? 900 : 813) : (s == 4 ? 960 : 900);
+    const long long ctas = base * s, per = (kblocks + s - 1) / s, slots = (tall ? 1ll : 2ll) * sms * permille / 1000;
     const long long cost = (s > 1 ? (tall ? 4000 : 700) : 0) + (tall ? 350 : 250) * per * ((ctas + slots - 1) / slots) +
                            700 * ((ctas - 1) / sms);
     if (s == 1 || cost < best) {
@@ -383,26 +418,46 @@ int x16_map(CUtensorMap* map, const X16Side& s, int J, int l, int dtype) {
                                   s.ptr, dims, strides, box, true);
 }
 
-template <int XK, int YK, bool PAIR>
+template <int XK, int YK, bool PAIR, bool SPLIT = false>
 int launch_x16(cudaStream_t stream, int sms, const CUtensorMap& mx, const CUtensorMap& my, X16Args a) {
   using S = X16Shape<XK, YK>;
   constexpr int kTile = PAIR ? 256 : 128;
   a.x_tiles = (a.x.rows + kTile - 1) / kTile;
   a.y_tiles = (a.y.rows + kTile - 1) / kTile;
   const long long units = static_cast<long long>(a.x_tiles) * a.y_tiles * a.l;
-  return launch<x16_gemm_kernel<XK, YK, PAIR>>(stream, PAIR ? 2 * std::min<long long>(units, sms / 2) : std::min<long long>(units, sms),
-                                               S::kThreads, S::kSmem, PAIR ? 2 : 1, true, mx, my, a);
+  const long long grid = SPLIT ? units * a.splits : PAIR ? 2 * std::min<long long>(units, sms / 2) : std::min<long long>(units, sms);
+  return launch<x16_gemm_kernel<XK, YK, PAIR, SPLIT>>(stream, grid, S::kThreads, S::kSmem, PAIR ? 2 : SPLIT ? a.splits : 1, true, mx,
+                                                      my, a);
 }
 
 template <int XK, int YK>
-int launch_x16_any(cudaStream_t stream, int sms, const CUtensorMap& mx, const CUtensorMap& my, const X16Args& a) {
+int launch_x16_any(cudaStream_t stream, int sms, const CUtensorMap& mx, const CUtensorMap& my, X16Args a) {
   // 256 x 256 tiles on pairs unless they leave SMs idle: a wave of pair tiles is twice the work of a
   // wave of 128 x 128 tiles and takes 1.25 times as long (1570 against 980 TFLOP/s at 4096^3)
-  auto waves = [&](int tile, long long workers) {
-    const long long units = static_cast<long long>((a.x.rows + tile - 1) / tile) * ((a.y.rows + tile - 1) / tile) * a.l;
-    return (units + workers - 1) / workers;
+  auto tiles = [&](int tile) {
+    return static_cast<long long>((a.x.rows + tile - 1) / tile) * ((a.y.rows + tile - 1) / tile) * a.l;
   };
+  auto waves = [&](int tile, long long workers) { return (tiles(tile) + workers - 1) / workers; };
   if (5 * waves(256, sms / 2) <= 4 * waves(128, sms)) return launch_x16<XK, YK, true>(stream, sms, mx, my, a);
+  // Fewer tiles than SMs: j over a cluster of up to eight CTAs per tile, while all clusters run at once, where it pays.
+  // In ns: a stage takes about 250, an expanded one 340; joining the sums 4500 (8-bit dB of 4096 x 64 over 8192:
+  // 46.1 us whole, 17.5 in fours; 512 x 512 over 4096: 25.6 and 11.2; dense 4096 x 64 over 4096: 19.2 and 11.1).
+  using S = X16Shape<XK, YK>;
+  constexpr long long kStageNs = XK >= kX16Mx4 || YK >= kX16Mx4 ? 340 : 250, kJoinNs = 4500;
+  const int blocks = (a.J + kX16J - 1) / kX16J;
+  long long best = kStageNs * blocks;
+  a.splits = 1;
+  for (int s = 2; s <= kMxMaxSplits && tiles(128) * s <= sms && kJoinNs < best; ++s) {
+    const int each = (blocks + s - 1) / s;
+    if (kJoinNs + kStageNs * each >= best) continue;
+    int rc, at_once;
+    if ((rc = clusters_at_once<x16_gemm_kernel<XK, YK, false, true>>(S::kThreads, S::kSmem, s, &at_once)) != FBMM_OK) return rc;
+    if (tiles(128) > at_once) continue;
+    best = kJoinNs + kStageNs * each;
+    a.splits = s;
+    a.blocks_per_split = each;
+  }
+  if (a.splits > 1) return launch_x16<XK, YK, false, true>(stream, sms, mx, my, a);
   return launch_x16<XK, YK, false>(stream, sms, mx, my, a);
 }
 

@@ -120,6 +120,12 @@ __device__ __forceinline__ void mx_store_one(void* C, int out_type, long long at
   else static_cast<__nv_bfloat16*>(C)[at] = __float2bfloat16_rn(v);
 }
 
+// Four neighbouring partial sums in the shared memory of a CTA of the cluster.
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 // 32 rows of a warp's accumulators (lane = row) -> row-major C, 128 bytes of every row at a time: 64 columns
 // (v0, v1) of a 16-bit type, or 32 columns of fp32 in two calls. The lanes' 16-byte pieces cross the
 // warp's staging area (piece index xor row, free of bank conflicts) so that every store instruction covers

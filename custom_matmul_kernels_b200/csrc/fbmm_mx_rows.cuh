@@ -58,11 +58,6 @@ struct MxRowsShape {
   static constexpr int smem(int stages, int blocks) { return 1024 + ring(stages) + (kCodes ? 0 : blocks * kABlock) + 256; }
 };
 
-__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
 // Without an eviction priority: a decoding step's weights may or may not fit L2 until the next one.
 __device__ __forceinline__ void tma_load_3d_normal(void* smem_dst, const void* tmap, uint64_t* bar, int32_t c0, int32_t c1,
                                                    int32_t c2) {

@@ -377,6 +377,28 @@ def test_dense_product_short_sums(dev, l, m, j, c, bits):
         assert torch.equal(MXDenseBMMCUDA()(Q.mT, P.transpose(1, 2)), flipped)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("l,m,j,c", [(1, 64, 5000, 130), (2, 200, 3001, 33), (1, 1, 9000, 700), (1, 129, 2600, 257)])
+def test_dense_product_long_sums(dev, l, m, j, c, dtype):
+    """Few tiles and a long sum: clusters share it; every layout, both widths, and the dense products."""
+    P = rnd((l, m, j), 3, dtype, 0.3).to(dev)
+    R = rnd((l, j, c), 4, dtype, 0.3).to(dev)
+    p, r = P.double(), R.double()
+    for bits in (4, 8):
+        Q = MXQuantizeCUDA(bits)(R)
+        q = Q.dequantize(dtype).double()
+        want, mag = (p @ q).cpu(), (p.abs() @ q.abs()).cpu()
+        for X in (P, P.transpose(1, 2).contiguous().transpose(1, 2)):
+            C, D = MXDenseBMMCUDA()(X, Q), MXDenseBMMCUDA()(Q.mT, X.transpose(1, 2))
+            assert_sum_close(C, want, mag, j, dtype)
+            assert_sum_close(D, want.transpose(1, 2), mag.transpose(1, 2), j, dtype)
+            assert torch.equal(MXDenseBMMCUDA()(X, Q), C)
+    for X in (P, P.transpose(1, 2).contiguous().transpose(1, 2)):
+        for Y in (R, R.transpose(1, 2).contiguous().transpose(1, 2)):
+            C = CheckpointBMMCUDA()(X.requires_grad_(), Y)
+            assert_sum_close(C.detach(), (p @ r).cpu(), (p.abs() @ r.abs()).cpu(), j, dtype)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("l,m,n,k", [(1, 5, 40, 64), (2, 130, 200, 300)])
 def test_frozen_weights_gradient(dev, l, m, n, k, dtype):
