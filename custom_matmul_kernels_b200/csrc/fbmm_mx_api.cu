@@ -382,20 +382,25 @@ size_t repack_bytes(const void* ptr, long long ld, long long stride, int l, int 
   return ((batched ? static_cast<size_t>(l) : 1) * outer * pitch * 2 + 255) / 256 * 256;
 }
 
-// Repacks such an operand into `need` bytes of the workspace and makes the side describe the copy.
-int repack_side(cudaStream_t stream, X16Side* s, int J, int l, size_t need, unsigned char** ws) {
+// The repacking of such an operand into the workspace; makes the side describe the copy.
+X16Repack repack_side(X16Side* s, int J, int l, unsigned char* ws) {
   const int outer = s->kind == kX16K ? s->rows : J, inner = s->kind == kX16K ? J : s->rows;
   const bool batched = l > 1 && s->stride != 0;
-  const int pitch = (inner + 7) / 8 * 8;
-  const long long pieces = static_cast<long long>(batched ? l : 1) * outer * (pitch / 8);
-  x16_repack_kernel<<<static_cast<unsigned>(std::min<long long>((pieces + 255) / 256, 1 << 20)), 256, 0, stream>>>(
-      static_cast<const uint16_t*>(s->ptr), s->ld, batched ? s->stride : 0, reinterpret_cast<uint16_t*>(*ws), outer, inner, pitch, pieces);
-  FBMM_HOST_CUDA(cudaGetLastError());
-  s->ptr = *ws;
-  s->ld = pitch;
-  s->stride = batched ? static_cast<long long>(outer) * pitch : 0;
-  *ws += need;
-  return FBMM_OK;
+  X16Repack r{};
+  r.src = static_cast<const uint16_t*>(s->ptr);
+  r.ld = s->ld;
+  r.stride = batched ? s->stride : 0;
+  r.dst = reinterpret_cast<uint16_t*>(ws);
+  r.rows = outer;
+  r.cols = inner;
+  r.pitch = (inner + 7) / 8 * 8;
+  r.pieces = static_cast<long long>(batched ? l : 1) * outer * (r.pitch / 8);
+  const uint64_t low = reinterpret_cast<uintptr_t>(s->ptr) | static_cast<uint64_t>(s->ld * 2) | static_cast<uint64_t>(r.stride * 2);
+  r.align = (low & 7) == 0 ? 8 : (low & 3) == 0 ? 4 : 2;
+  s->ptr = ws;
+  s->ld = r.pitch;
+  s->stride = batched ? static_cast<long long>(outer) * r.pitch : 0;
+  return r;
 }
 
 int x16_map(CUtensorMap* map, const X16Side& s, int J, int l, int dtype) {
@@ -475,7 +480,7 @@ int x16_product(cudaStream_t stream, X16Side x, X16Side y, int dtype, void* C, l
   if ((rc = check_result(C, dtype, ldc, stride_c, l, x.rows, y.rows)) != FBMM_OK) return rc;
   if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return fail(FBMM_ERR_ALIGN, "workspace is not 16-byte aligned");
   // refused before a device is asked for
-  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  unsigned char* const ws = static_cast<unsigned char*>(workspace);
   const size_t need_x = x.kind >= kX16Mx4 ? 0 : repack_bytes(x.ptr, x.ld, x.stride, l, x.kind == kX16K ? x.rows : J, x.kind == kX16K ? J : x.rows);
   const size_t need_y = y.kind >= kX16Mx4 ? 0 : repack_bytes(y.ptr, y.ld, y.stride, l, y.kind == kX16K ? y.rows : J, y.kind == kX16K ? J : y.rows);
   if (need_x + need_y > 0 && ws == nullptr)
@@ -484,8 +489,14 @@ int x16_product(cudaStream_t stream, X16Side x, X16Side y, int dtype, void* C, l
   if (need_x + need_y > 0 && workspace_bytes < need_x + need_y)
     return fail(FBMM_ERR_WORKSPACE, "repacking needs %zu workspace bytes, got %zu", need_x + need_y, workspace_bytes);
   if ((rc = fbmm_host::device_sms(&sms)) != FBMM_OK) return rc;
-  if (need_x && (rc = repack_side(stream, &x, J, l, need_x, &ws)) != FBMM_OK) return rc;
-  if (need_y && (rc = repack_side(stream, &y, J, l, need_y, &ws)) != FBMM_OK) return rc;
+  if (need_x + need_y > 0) {
+    X16Repack p{}, q{};
+    if (need_x) p = repack_side(&x, J, l, ws);
+    if (need_y) q = repack_side(&y, J, l, ws + need_x);
+    auto blocks = [](const X16Repack& r) { return std::min<long long>((r.pieces + 255) / 256, 1 << 20); };
+    if ((rc = launch<x16_repack_kernel>(stream, blocks(p) + blocks(q), 256, 0, 1, true, p, q, static_cast<unsigned>(blocks(p)))) != FBMM_OK)
+      return rc;
+  }
   CUtensorMap mx, my;
   if ((rc = x16_map(&mx, x, J, l, dtype)) != FBMM_OK) return rc;
   if ((rc = x16_map(&my, y, J, l, dtype)) != FBMM_OK) return rc;

@@ -445,24 +445,45 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 }
 
 // Rows of `cols` 16-bit elements at any alignment -> rows padded to `pitch` (a multiple of 8) elements, zeros in the
-// padding: what the tensor maps of operands with odd pitches or bases are made over. Eight elements a thread.
-__global__ void __launch_bounds__(256) x16_repack_kernel(const uint16_t* __restrict__ src, long long ld, long long stride,
-                                                         uint16_t* __restrict__ dst, int rows, int cols, int pitch, long long pieces) {
+// padding: what the tensor maps of operands with odd pitches or bases are made over. Eight elements a thread, by the
+// widest loads (`align` bytes, 2 to 8) that every row allows. One launch serves both operands of a product: the
+// first `blocks` blocks take p, the others q.
+struct X16Repack {
+  const uint16_t* src;
+  long long ld, stride;
+  uint16_t* dst;
+  int rows, cols, pitch, align;
+  long long pieces;
+};
+
+__global__ void __launch_bounds__(256) x16_repack_kernel(const X16Repack p, const X16Repack q, const unsigned blocks) {
   mx_let_next_start();
-  const int per_row = pitch / 8;
-  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < pieces;
-       i += static_cast<long long>(gridDim.x) * 256) {
-    const long long row = i / per_row;  // over all batches
+  mx_wait_for_previous();
+  const bool first = blockIdx.x < blocks;
+  const X16Repack s = first ? p : q;
+  const int per_row = s.pitch / 8;
+  const long long step = static_cast<long long>(first ? blocks : gridDim.x - blocks) * 256;
+  for (long long i = static_cast<long long>(first ? blockIdx.x : blockIdx.x - blocks) * 256 + threadIdx.x; i < s.pieces; i += step) {
+    // over all batches; in 32 bits where they suffice
+    const long long row = s.pieces <= 0x7fffffff ? static_cast<unsigned>(i) / static_cast<unsigned>(per_row) : i / per_row;
     const int c = static_cast<int>(i - row * per_row) * 8;
-    const long long b = row / rows;
-    const uint16_t* p = src + b * stride + (row - b * rows) * ld + c;
+    const long long b = s.pieces <= 0x7fffffff ? static_cast<unsigned>(row) / static_cast<unsigned>(s.rows) : row / s.rows;
+    const uint16_t* from = s.src + b * s.stride + (row - b * s.rows) * s.ld + c;
     uint32_t w[4];
+    if (s.align == 8 && c + 8 <= s.cols) {
+      const uint2 lo = __ldg(reinterpret_cast<const uint2*>(from)), hi = __ldg(reinterpret_cast<const uint2*>(from) + 1);
+      w[0] = lo.x; w[1] = lo.y; w[2] = hi.x; w[3] = hi.y;
+    } else if (s.align >= 4 && c + 8 <= s.cols) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t lo = c + 2 * j < cols ? __ldg(p + 2 * j) : 0u, hi = c + 2 * j + 1 < cols ? __ldg(p + 2 * j + 1) : 0u;
-      w[j] = lo | (hi << 16);
+      for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const uint32_t*>(from) + j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t lo = c + 2 * j < s.cols ? __ldg(from + 2 * j) : 0u, hi = c + 2 * j + 1 < s.cols ? __ldg(from + 2 * j + 1) : 0u;
+        w[j] = lo | (hi << 16);
+      }
     }
-    *reinterpret_cast<uint4*>(dst + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(s.dst + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
