@@ -113,6 +113,12 @@ int codes_map(CUtensorMap* map, const unsigned char* codes, long long stride, in
   return fbmm_host::tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, dims, strides, box, true);
 }
 
+// Bytes that every row of a matrix is aligned to: 16, 8, 4 or 2; pitch and batch stride in bytes.
+int row_align(const void* base, long long pitch, long long stride) {
+  const uint64_t low = reinterpret_cast<uintptr_t>(base) | static_cast<uint64_t>(pitch) | static_cast<uint64_t>(stride);
+  return (low & 15) == 0 ? 16 : (low & 7) == 0 ? 8 : (low & 3) == 0 ? 4 : 2;
+}
+
 constexpr int kMxMaxSplits = 8;  // CTAs that share a tile's sum: the portable cluster size
 
 // The kernel's shared-memory limit is set once per device.
@@ -231,7 +237,7 @@ int launch_mx_pair(cudaStream_t stream, int sms, const MxSide& A, const MxSide& 
   a.l = g.l; a.m = A.rows; a.n = B.rows; a.k = g.k;
   a.a_shared = A.stride == 0; a.b_shared = B.stride == 0;
   a.as_shared = A.scale_stride == 0; a.bs_shared = B.scale_stride == 0;
-  a.out_type = g.out_type; a.vec_ok = g.vec_ok;
+  a.out_type = g.out_type; a.align = g.align;
   a.m_tiles = (a.m + 255) / 256;
   a.n_tiles = (a.n + 255) / 256;
   const long long units = static_cast<long long>(a.m_tiles) * a.n_tiles * a.l;
@@ -331,7 +337,7 @@ int mx4_product(cudaStream_t stream, bool overlap, const unsigned char* a_codes,
   a.C = C; a.ldc = ldc; a.stride_c = l > 1 ? stride_c : 0;
   a.l = l; a.k = k; a.out_type = dtype;
   const long long size = elem_size(dtype);
-  a.vec_ok = ((reinterpret_cast<uintptr_t>(C) | (ldc * size) | (a.stride_c * size)) & 15) == 0;
+  a.align = row_align(C, ldc * size, a.stride_c * size);
   const MxSide A{a_codes, stride_a, a_scales, stride_as, m}, B{b_codes, stride_b, b_scales, stride_bs, n};
   int splits, blocks;
   rows_splits(sms, l, m, n, k, &splits, &blocks);
@@ -339,7 +345,7 @@ int mx4_product(cudaStream_t stream, bool overlap, const unsigned char* a_codes,
     MxRowsArgs r{};
     r.C = C; r.ldc = ldc; r.stride_c = a.stride_c;
     r.l = l; r.m = m; r.n = n; r.k = k;
-    r.out_type = dtype; r.vec_ok = a.vec_ok;
+    r.out_type = dtype; r.align = a.align;
     if (m > kMxFewRows) return launch_mx_rows<128, uint8_t>(stream, sms, overlap, B, &A, r);
     return m <= 16 ? launch_mx_rows<16, uint8_t>(stream, sms, overlap, B, &A, r) : launch_mx_rows<64, uint8_t>(stream, sms, overlap, B, &A, r);
   }
@@ -395,8 +401,7 @@ X16Repack repack_side(X16Side* s, int J, int l, unsigned char* ws) {
   r.cols = inner;
   r.pitch = (inner + 7) / 8 * 8;
   r.pieces = static_cast<long long>(batched ? l : 1) * outer * (r.pitch / 8);
-  const uint64_t low = reinterpret_cast<uintptr_t>(s->ptr) | static_cast<uint64_t>(s->ld * 2) | static_cast<uint64_t>(r.stride * 2);
-  r.align = (low & 7) == 0 ? 8 : (low & 3) == 0 ? 4 : 2;
+  r.align = row_align(s->ptr, s->ld * 2, r.stride * 2);
   s->ptr = ws;
   s->ld = r.pitch;
   s->stride = batched ? static_cast<long long>(outer) * r.pitch : 0;
@@ -505,7 +510,7 @@ int x16_product(cudaStream_t stream, X16Side x, X16Side y, int dtype, void* C, l
   a.y = X16Operand{y.scales, l > 1 ? y.scale_stride : 0, y.rows, l > 1 && y.stride == 0};
   a.C = C; a.ldc = ldc; a.stride_c = l > 1 ? stride_c : 0;
   a.l = l; a.J = J; a.dtype = dtype;
-  a.vec_ok = ((reinterpret_cast<uintptr_t>(C) | (ldc * 2) | (a.stride_c * 2)) & 15) == 0;
+  a.align = row_align(C, ldc * 2, a.stride_c * 2);
 #define FBMM_X16(XK, YK) \
   if (x.kind == XK && y.kind == YK) return launch_x16_any<XK, YK>(stream, sms, mx, my, a)
   FBMM_X16(kX16K, kX16K);
@@ -629,7 +634,7 @@ int fbmm_mx4_bmm_tensor(void* stream, const void* A, int a_dtype, int a_layout, 
     a.l = l; a.m = m; a.n = n; a.k = k;
     a.out_type = dtype;
     const long long size = elem_size(dtype);
-    a.vec_ok = ((reinterpret_cast<uintptr_t>(C) | (ldc * size) | (a.stride_c * size)) & 15) == 0;
+    a.align = row_align(C, ldc * size, a.stride_c * size);
     const MxSide W{b_codes, stride_b, b_scales, stride_bs, n};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return m <= 16 ? launch_mx_rows_fused<16>(s, sms, a_dtype, W, a) : launch_mx_rows_fused<64>(s, sms, a_dtype, W, a);

@@ -37,7 +37,7 @@ struct MxGemmArgs {
   int p_shared, q_shared, sp_shared, sq_shared;  // one matrix of codes / scales for every batch
   int out_type;  // 0 fp32, 1 fp16, 2 bf16
   int p_tiles, q_tiles;
-  int vec_ok;    // C's rows are 16-byte aligned
+  int align;     // bytes that C's rows are aligned to: 16, 8, 4 or 2
 };
 
 struct MxShape {
@@ -129,66 +129,107 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
 // 32 rows of a warp's accumulators (lane = row) -> row-major C, 128 bytes of every row at a time: 64 columns
 // (v0, v1) of a 16-bit type, or 32 columns of fp32 in two calls. The lanes' 16-byte pieces cross the
 // warp's staging area (piece index xor row, free of bank conflicts) so that every store instruction covers
-// four whole 128-byte lines; with 64-byte pieces of rows 16-bit results left at 2.0 TB/s (8192 x 8192 with
-// k = 256: 68 us, 44 us with whole lines; a plain fill writes 3.9 TB/s). `c0`: element (row 0, column 0) of the block.
+// four whole 128-byte lines (16-bit results of 8192 x 8192 with k = 256: 68 us with 64-byte pieces of rows, 44 us
+// with lines; a plain fill writes 3.9 TB/s). The staging area is read ahead of the stores, which the compiler must take
+// for writes to it and would wait on (the same 41 us; 4-bit operands 45 -> 35 us, fp32 results 73 -> 47).
+// Rows on 8-byte boundaries leave in pieces of that size (bf16 8192 x 4092, k = 1024: 62 -> 49 us), others by element (8192 x 4091: 54 us).
+// `c0`: element (row 0, column 0) of the block.
 template <typename Word>
 __device__ __forceinline__ void mx_store_lines(uint8_t* stage, Word word, void* C, long long c0, long long ldc, int size,
-                                               int rows, int cols, bool vec) {
+                                               int rows, int cols, int align) {
   const int lane = static_cast<int>(lane_id());
   uint4* st = reinterpret_cast<uint4*>(stage);
+  cols = min(cols, 128 / size);
   __syncwarp();
 #pragma unroll
   for (int c = 0; c < 8; ++c) st[lane * 8 + (c ^ (lane & 7))] = word(c);
   __syncwarp();
-  if (vec) {
-    const int c = lane & 7, per = 16 / size;  // piece of a row, its elements
+  if (align == 16) {
+    const int c = lane & 7, r0 = lane >> 3, left = cols * size - c * 16;  // left: bytes of the row from this piece on
+    const int end = left > 0 ? min(rows, 32) : 0;
+    uint8_t* at = static_cast<uint8_t*>(C) + (c0 + r0 * ldc) * size + c * 16;
+    uint4 x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int r = i * 4 + (lane >> 3);
-      const uint4 x = st[r * 8 + (c ^ (r & 7))];
-      if (r < rows) {
-        uint8_t* at = static_cast<uint8_t*>(C) + (c0 + r * ldc) * size + c * 16;
-        if ((c + 1) * per <= cols) {
-          *reinterpret_cast<uint4*>(at) = x;
-        } else {
-          const uint32_t e[4] = {x.x, x.y, x.z, x.w};
-          if (size == 4) {
+      const int r = r0 + 4 * i;
+      x[i] = st[r * 8 + (c ^ (r & 7))];
+    }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) if (c * 4 + j < cols) reinterpret_cast<uint32_t*>(at)[j] = e[j];
-          } else {
+    for (int i = 0; i < 8; ++i, at += 4 * ldc * size) {
+      if (r0 + 4 * i >= end) break;
+      if (left >= 16) {
+        *reinterpret_cast<uint4*>(at) = x[i];
+      } else {
+        const uint32_t e[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (c * 8 + j < cols) reinterpret_cast<uint16_t*>(at)[j] = static_cast<uint16_t>(e[j >> 1] >> (16 * (j & 1)));
-          }
+        for (int j = 0; j < 16 / size; ++j) {
+          if (j * size >= left) break;
+          if (size == 4) reinterpret_cast<uint32_t*>(at)[j] = e[j];
+          else reinterpret_cast<uint16_t*>(at)[j] = static_cast<uint16_t>(e[j >> 1] >> (16 * (j & 1)));
         }
       }
     }
-  } else {  // rows at any alignment: neighbouring lanes store neighbouring elements of one row
-    const int end = rows < 32 ? rows : 32;
-#pragma unroll 4
-    for (int r = 0; r < end; ++r) {
-      uint8_t* row = static_cast<uint8_t*>(C) + (c0 + r * ldc) * size;
-      if (size == 4) {
-        const uint32_t x = reinterpret_cast<const uint32_t*>(st + r * 8 + ((lane >> 2) ^ (r & 7)))[lane & 3];
-        if (lane < cols) reinterpret_cast<uint32_t*>(row)[lane] = x;
-      } else {
+  } else if (align == 8) {  // two rows at a time in 8-byte pieces
+    const int c = lane & 15, left = cols * size - c * 8;  // bytes of the row from this piece on
+    const int end = left > 0 ? min(rows, 32) : 0;
+    uint8_t* at = static_cast<uint8_t*>(C) + (c0 + (lane >> 4) * ldc) * size + c * 8;
+#pragma unroll 1
+    for (int r0 = lane >> 4; r0 < end; r0 += 8) {
+      uint2 x[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int e = h * 32 + lane;
-          const uint16_t x = reinterpret_cast<const uint16_t*>(st + r * 8 + ((e >> 3) ^ (r & 7)))[e & 7];
-          if (e < cols) reinterpret_cast<uint16_t*>(row)[e] = x;
+      for (int i = 0; i < 4; ++i) {
+        const int r = r0 + 2 * i;
+        x[i] = reinterpret_cast<const uint2*>(st + r * 8 + ((c >> 1) ^ (r & 7)))[c & 1];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i, at += 2 * ldc * size) {
+        if (r0 + 2 * i >= end) break;
+        if (left >= 8) {
+          *reinterpret_cast<uint2*>(at) = x[i];
+        } else {
+          if (left >= 4) reinterpret_cast<uint32_t*>(at)[0] = x[i].x;
+          if (size == 2 && (left & 2)) reinterpret_cast<uint16_t*>(at)[left >> 1 & 2] = static_cast<uint16_t>(left & 4 ? x[i].y : x[i].x);
+        }
+      }
+    }
+  } else {  // rows at any alignment: neighbouring lanes store neighbouring elements of one row (pairs of 16-bit
+            // elements, where rows are 4-byte aligned, measured the same)
+    const int end = min(rows, 32);
+    uint8_t* row = static_cast<uint8_t*>(C) + (c0 + lane) * size;
+#pragma unroll 1
+    for (int r0 = 0; r0 < end; r0 += 8) {
+      uint32_t x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = r0 + i;
+        if (size == 4) {
+          x[i] = reinterpret_cast<const uint32_t*>(st + r * 8 + ((lane >> 2) ^ (r & 7)))[lane & 3];
+        } else {  // elements `lane` and 32 + lane
+          const int p = lane >> 3, e = lane & 7;
+          x[i] = reinterpret_cast<const uint16_t*>(st + r * 8 + (p ^ (r & 7)))[e] |
+                 static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(st + r * 8 + ((4 + p) ^ (r & 7)))[e]) << 16;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i, row += ldc * size) {
+        if (r0 + i >= end) break;
+        if (size == 4) {
+          if (lane < cols) *reinterpret_cast<uint32_t*>(row) = x[i];
+        } else {
+          if (lane < cols) *reinterpret_cast<uint16_t*>(row) = static_cast<uint16_t>(x[i]);
+          if (lane + 32 < cols) reinterpret_cast<uint16_t*>(row)[32] = static_cast<uint16_t>(x[i] >> 16);
         }
       }
     }
   }
 }
 __device__ __forceinline__ void mx_store_rows(uint8_t* stage, const uint32_t (&v0)[32], const uint32_t (&v1)[32], void* C,
-                                              long long c0, long long ldc, int out_type, int rows, int cols, bool vec) {
+                                              long long c0, long long ldc, int out_type, int rows, int cols, int align) {
   if (out_type == 0) {
     mx_store_lines(stage, [&](int c) { return make_uint4(v0[4 * c], v0[4 * c + 1], v0[4 * c + 2], v0[4 * c + 3]); }, C, c0,
-                   ldc, 4, rows, cols, vec);
+                   ldc, 4, rows, cols, align);
     mx_store_lines(stage, [&](int c) { return make_uint4(v1[4 * c], v1[4 * c + 1], v1[4 * c + 2], v1[4 * c + 3]); }, C,
-                   c0 + 32, ldc, 4, rows, cols - 32, vec);
+                   c0 + 32, ldc, 4, rows, cols - 32, align);
   } else {
     mx_store_lines(stage, [&](int c) {
       const uint32_t (&v)[32] = c < 4 ? v0 : v1;
@@ -197,7 +238,7 @@ __device__ __forceinline__ void mx_store_rows(uint8_t* stage, const uint32_t (&v
       for (int j = 0; j < 4; ++j)
         p[j] = mx_pack_out(out_type, __uint_as_float(v[8 * (c & 3) + 2 * j]), __uint_as_float(v[8 * (c & 3) + 2 * j + 1]));
       return make_uint4(p[0], p[1], p[2], p[3]);
-    }, C, c0, ldc, 2, rows, cols, vec);
+    }, C, c0, ldc, 2, rows, cols, align);
   }
 }
 
@@ -334,7 +375,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant_
         tmem_ld_wait();
         if (c + 64 >= BN || q0 + 64 >= a.q_rows) release();
         mx_store_rows(stage_mem, v0, v1, a.C, b * a.stride_c + static_cast<long long>(p0) * a.ldc + q0, a.ldc, a.out_type,
-                      a.p_rows - p0, a.q_rows - q0, a.vec_ok != 0);
+                      a.p_rows - p0, a.q_rows - q0, a.align);
       }
       if (held) release();
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }

@@ -31,7 +31,7 @@ struct MxPairArgs {
   int a_shared, b_shared, as_shared, bs_shared;  // one matrix of codes / scales for every batch
   int out_type;
   int m_tiles, n_tiles;
-  int vec_ok;
+  int align;
 };
 
 __device__ __forceinline__ void mx_umma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa,
@@ -190,7 +190,7 @@ mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         const int n0 = nt * 256 + half * 128 + c * 32;
         if (n0 < a.n && m0 < a.m)
           mx_store_rows(stage_mem, v[c], v[c + 1], a.C, b * a.stride_c + static_cast<long long>(m0) * a.ldc + n0, a.ldc,
-                        a.out_type, a.m - m0, a.n - n0, a.vec_ok != 0);
+                        a.out_type, a.m - m0, a.n - n0, a.align);
       }
     }
   }

@@ -31,7 +31,7 @@ struct MxRowsArgs {
   int l, m, n, k;
   int w_shared, sw_shared, a_shared, sa_shared;
   int out_type;
-  int vec_ok;               // C's rows are 16-byte aligned
+  int align;                // bytes that C's rows are aligned to
   int n_tiles, m_tiles, splits, blocks_per_split;  // blocks of 256 k
   int stages;
 };
@@ -253,7 +253,7 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
     const int col = n0 + static_cast<int>(lane) * 4;
     const uint32_t at = smem_u32(sums) + lane * 16;
     const int size = a.out_type == 0 ? 4 : 2;
-    const bool vec = a.vec_ok && col + 4 <= a.n;
+    const bool vec = a.align >= (a.out_type == 0 ? 16 : 8) && col + 4 <= a.n;
     for (int r = static_cast<int>(split) + a.splits * static_cast<int>(warp); r < rows; r += kWarps * a.splits) {
       float s[4] = {0.f, 0.f, 0.f, 0.f};
       for (int q0 = 0; q0 < a.splits; q0 += 4) {

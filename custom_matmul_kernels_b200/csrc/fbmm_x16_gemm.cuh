@@ -51,7 +51,7 @@ struct X16Args {
   int l, J;
   int dtype;     // 1 fp16, 2 bf16
   int x_tiles, y_tiles;
-  int vec_ok;
+  int align;  // as MxGemmArgs
   int splits, blocks_per_split;  // SPLIT: CTAs per tile, stages of j each
 };
 
@@ -394,7 +394,7 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             p[j] = mx_pack_out(a.dtype, __uint_as_float(v[8 * (i & 3) + 2 * j]), __uint_as_float(v[8 * (i & 3) + 2 * j + 1]));
           return make_uint4(p[0], p[1], p[2], p[3]);
         }, a.C, b * a.stride_c + static_cast<long long>(x0) * a.ldc + y0, a.ldc, 2, a.x.rows - x0, a.y.rows - y0,
-                       a.vec_ok != 0);
+                       a.align);
       }
       if (held) release();
       if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
@@ -414,7 +414,7 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       int b, xt, yt;
       x16_decode(u0, a.x_tiles, a.y_tiles, b, xt, yt);
       const int rows = min(128, a.x.rows - xt * 128), col = yt * 128 + static_cast<int>(lane) * 4;
-      const bool vec = a.vec_ok && col + 4 <= a.y.rows;
+      const bool vec = a.align >= 8 && col + 4 <= a.y.rows;
       const uint32_t base = smem_u32(smem);
       for (int r = static_cast<int>(split) + a.splits * static_cast<int>(warp); r < rows; r += (S::kThreads / 32) * a.splits) {
         const uint32_t at = base + static_cast<uint32_t>(r) * 512 + ((lane ^ (static_cast<uint32_t>(r) & 31u)) << 4);
@@ -446,7 +446,7 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 
 // Rows of `cols` 16-bit elements at any alignment -> rows padded to `pitch` (a multiple of 8) elements, zeros in the
 // padding: what the tensor maps of operands with odd pitches or bases are made over. Eight elements a thread, by the
-// widest loads (`align` bytes, 2 to 8) that every row allows. One launch serves both operands of a product: the
+// widest loads (`align` bytes, 2 to 16) that every row allows. One launch serves both operands of a product: the
 // first `blocks` blocks take p, the others q.
 struct X16Repack {
   const uint16_t* src;
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(256) x16_repack_kernel(const X16Repack p, cons
     const long long b = s.pieces <= 0x7fffffff ? static_cast<unsigned>(row) / static_cast<unsigned>(s.rows) : row / s.rows;
     const uint16_t* from = s.src + b * s.stride + (row - b * s.rows) * s.ld + c;
     uint32_t w[4];
-    if (s.align == 8 && c + 8 <= s.cols) {
+    if (s.align >= 8 && c + 8 <= s.cols) {
       const uint2 lo = __ldg(reinterpret_cast<const uint2*>(from)), hi = __ldg(reinterpret_cast<const uint2*>(from) + 1);
       w[0] = lo.x; w[1] = lo.y; w[2] = hi.x; w[3] = hi.y;
     } else if (s.align >= 4 && c + 8 <= s.cols) {

@@ -399,6 +399,25 @@ def test_dense_product_long_sums(dev, l, m, j, c, dtype):
             assert_sum_close(C.detach(), (p @ r).cpu(), (p.abs() @ r.abs()).cpu(), j, dtype)
 
 
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 6, 129, 130, 131, 132, 134, 136, 195, 196, 198, 257, 258, 260])
+@pytest.mark.parametrize("l,m", [(1, 3), (1, 150), (3, 97), (1, 20001)])
+def test_result_rows_at_every_alignment(dev, l, m, n):
+    """Result rows 2, 4, 8 and 16 bytes apart from a line, in every kernel that writes them, and their last pieces."""
+    k = 96
+    A, B = rnd((l, m, k), 5, BF16).to(dev), rnd((l, k, n), 6, BF16).to(dev)
+    A4, B4, B8 = MXQuantizeCUDA(4)(A), MXQuantizeCUDA(4)(B, dim=-2), MXQuantizeCUDA(8)(B)
+    a, b = A4.dequantize(F32).double(), B4.dequantize(F32).double()
+    want, mag = (a @ b).cpu(), (a.abs() @ b.abs()).cpu()
+    for dtype in (F32, F16, BF16):
+        C = MXBMMCUDA(out_dtype=dtype)(A4, B4).cpu()
+        # fp16 ends at 65504: a sum of 65520 or more rounds to infinity (20001 x 3 has four: the largest is 80999)
+        over = want.abs() >= 65520 if dtype == F16 else torch.zeros_like(want, dtype=torch.bool)
+        assert torch.equal(C[over].double(), want[over].sign() * float("inf"))
+        assert_sum_close(C.masked_fill(over, 0), want.masked_fill(over, 0), mag, k, dtype)
+    a, b = A.double(), B8.dequantize(BF16).double()
+    assert_sum_close(MXDenseBMMCUDA()(A, B8), (a @ b).cpu(), (a.abs() @ b.abs()).cpu(), k, BF16)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("l,m,n,k", [(1, 5, 40, 64), (2, 130, 200, 300)])
 def test_frozen_weights_gradient(dev, l, m, n, k, dtype):
