@@ -102,12 +102,17 @@ __device__ __forceinline__ uint64_t x16_desc(uint32_t smem_addr, bool mn_major) 
          (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
 
-// Reports to the pair's issuing CTA what concerns only THIS CTA's memories: that this warp's values lie in its
-// shared memory, behind their proxy fence, where its own tensor core reads them, or that the warp has
-// read its accumulators. So the release covers this CTA; with one at cluster scope the arrival itself took about 1400 cycles beside 16 writing warps, twice the expansion
-// (8-bit gradient of weights at 4096^3: 145 us with it, 115 us without).
+// Reports to the pair's issuing CTA, by cluster-window address, that this warp's values lie in its own CTA's shared
+// memory (behind their proxy fence), or that the warp has read its accumulators. A release at cluster scope, as two CTAs
+// are ordered by nothing less, but of shared memory only: one that covers global memory too took each warp about
+// 1400 cycles beside 16 writing warps, twice the expansion (8-bit gradient of weights at 4096^3: 145 us against
+// 119 us). Passing the reports on through one warp of the CTA measured the same as this.
 __device__ __forceinline__ void mbar_arrive_values(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile(
+      "fence.release.sync_restrict::shared::cta.cluster;\n"
+      "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];"
+      ::"r"(cluster_addr)
+      : "memory");
 }
 
 // A stage's raw codes -> 16-bit values in MN-major order; 128 threads, 16 codes of a row of 128 at a time.
