@@ -41,7 +41,7 @@ struct X16Operand {
   const uint8_t* scales;   // microscaled: groups [j / 128][rows / 128][512]
   long long scale_stride;  // bytes, 0 = shared
   int rows;
-  int shared;
+  int shared;              // one matrix of elements or codes for every batch; the scales have a stride of their own
 };
 
 struct X16Args {
@@ -233,23 +233,23 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       // 128 rows of one operand, from row r0: to the part's place, or its raw codes
       auto load = [&](const CUtensorMap* map, int kind, uint8_t* part, uint8_t* raw, int j0, int r0, int b,
                       const X16Operand& op) {
-        if (op.shared) b = 0;
+        const int mb = op.shared ? 0 : b;  // of the elements or codes
         uint64_t* full = &bars->full[stage];
         if (kind == kX16K) {
-          if (PAIR) tma_load_3d_pair(part, map, bars0 + off(full), j0, r0, b, kL2EvictLast);
-          else tma_load_3d(part, map, full, j0, r0, b, kL2EvictLast);
+          if (PAIR) tma_load_3d_pair(part, map, bars0 + off(full), j0, r0, mb, kL2EvictLast);
+          else tma_load_3d(part, map, full, j0, r0, mb, kL2EvictLast);
         } else if (kind == kX16MN) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            if (PAIR) tma_load_3d_pair(part + c * kX16Chunk, map, bars0 + off(full), r0 + c * 64, j0, b, kL2EvictLast);
-            else tma_load_3d(part + c * kX16Chunk, map, full, r0 + c * 64, j0, b, kL2EvictLast);
+            if (PAIR) tma_load_3d_pair(part + c * kX16Chunk, map, bars0 + off(full), r0 + c * 64, j0, mb, kL2EvictLast);
+            else tma_load_3d(part + c * kX16Chunk, map, full, r0 + c * 64, j0, mb, kL2EvictLast);
           }
         } else {
           const int bytes = kX16J * 128 * S::kBits / 8;
           const int groups = (op.rows + 127) / 128;
           const bool exists = r0 < op.rows;
           mbar_arrive_expect_tx(&bars->raw[stage], bytes + (exists ? kMxGroupBytes : 0));
-          tma_load_3d(raw, map, &bars->raw[stage], r0 * S::kBits / 8, j0, b, kL2EvictLast);
+          tma_load_3d(raw, map, &bars->raw[stage], r0 * S::kBits / 8, j0, mb, kL2EvictLast);
           if (exists)
             mx_bulk_load(raw + bytes,
                          op.scales + b * op.scale_stride +
