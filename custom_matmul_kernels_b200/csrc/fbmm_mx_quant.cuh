@@ -479,7 +479,7 @@ struct MxDequantArgs {
 // packed pairs by the power of two that is left: four or five integer instructions and one
 // multiplication per pair, where converting through fp16 and fp32 takes one slow conversion and five
 // more instructions. It rounds once, in that multiplication. Scales whose remaining power the
-// type cannot hold as a normal number, and the NaN scale, take the general form.
+// type cannot hold as a normal number, the NaN scale, and 8-bit NaN codes (mx_nan_codes) take the general form.
 template <int BITS, bool BF16>
 struct MxFast {
   static constexpr int kBias = BF16 ? (BITS == 8 ? 120 : 126) : (BITS == 8 ? -104 : -98);  // E + kBias = exponent field
@@ -492,6 +492,19 @@ struct MxFast {
     return ((E + static_cast<uint32_t>(kBias)) << (BF16 ? 7 : 10)) * 0x10001u;
   }
 };
+// Non-zero where one of 8-bit codes is 0x7f or 0xff: adding one to every byte carries into bit 7 where the lower seven
+// bits are all set. A carry that leaves a byte comes from 0xff, so what it does to the next changes no answer.
+// Two instructions per four codes: 8-bit gradient of weights 8192 x 4096 x 4096 212 -> 220 us (with three-input maxima of the
+// shifted codes 223 us).
+template <int BITS>
+__device__ __forceinline__ uint32_t mx_nan_codes(const uint32_t (&c)[BITS / 2]) {
+  uint32_t any = 0;
+  if (BITS == 8) {
+#pragma unroll
+    for (int q = 0; q < BITS / 2; ++q) any |= (c[q] + 0x01010101u) ^ c[q];
+  }
+  return any & 0x80808080u;
+}
 template <bool BF16>
 __device__ __forceinline__ uint32_t mx_mul2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -609,7 +622,7 @@ __global__ void __launch_bounds__(256) mx_dequantize_kernel(const MxDequantArgs 
     if (sizeof(T) == 2) {
       constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
       uint32_t v[8];
-      mx_values16<BITS, kBf16>(c[j], E[j], MxFast<BITS, kBf16>::in_range(E[j]), v);
+      mx_values16<BITS, kBf16>(c[j], E[j], MxFast<BITS, kBf16>::in_range(E[j]) && mx_nan_codes<BITS>(c[j]) == 0, v);
 #pragma unroll
       for (int q = 0; q < 8; ++q) w[q] = v[q];
     } else {

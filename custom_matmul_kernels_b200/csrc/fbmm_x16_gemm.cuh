@@ -127,6 +127,7 @@ __device__ __forceinline__ void x16_expand(const uint8_t* raw, uint8_t* dst, int
   const int base = (tid >> 4) & 3, flip = (tid & 4) ? 5 : 0;
   uint32_t c[4][BITS / 2], E[4];
   bool in_range = true;
+  uint32_t nan = 0;
 #pragma unroll
   for (int it = 0; it < 4; ++it) {
     const int j = (((tid >> 6) * 4 + it) << 3) | (base ^ flip);
@@ -140,8 +141,9 @@ __device__ __forceinline__ void x16_expand(const uint8_t* raw, uint8_t* dst, int
     E[it] = sc[mx_scale_at((j0 + j) & 127, u >> 1)];
     if (j0 + j >= j_end) E[it] = 127;
     in_range = in_range && MxFast<BITS, BF16>::in_range(E[it]);
+    nan |= mx_nan_codes<BITS>(c[it]);
   }
-  const bool fast = __all_sync(0xffffffffu, in_range);
+  const bool fast = __all_sync(0xffffffffu, in_range && nan == 0);
   auto expand = [&](bool quick) {
 #pragma unroll
     for (int it = 0; it < 4; ++it) {

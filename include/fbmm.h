@@ -296,7 +296,7 @@ int fbmm_kmeans_update_f32(void* stream, const float* X, long long ldx, const lo
  *  - scales: [l][ceil(rows/128)][ceil(k/128)][512] bytes; in a group of 128 rows x 4 blocks, row r
  *    and block b at byte (r % 32) * 16 + (r / 32) * 4 + b. A byte E stands for 2^(E - 127); bytes of
  *    rows and blocks that do not exist are 0. 255 marks a block that held an infinity or a NaN:
- *    all of its elements read as NaN (the 8-bit codes 0x7f and 0xff are not used).
+ *    all of its elements read as NaN. The 8-bit codes 0x7f and 0xff read as NaN; the quantiser writes neither.
  *  - The scale of a block with largest magnitude a: 4 bits 2^(floor(log2 a) - 2), elements above
  *    6 * scale saturate; 8 bits the least power of two that keeps a <= 448 * scale, bounded so that
  *    every element * scale is a finite value of the source's type. Elements are rounded to
