@@ -368,8 +368,10 @@ struct X16Side {
 };
 
 int check_x16_side(const char* name, const X16Side& s, int J, int l) {
-  if (s.kind >= kX16Mx4)
-    return check_mx(name, static_cast<const unsigned char*>(s.ptr), s.stride, s.scales, s.scale_stride, l);
+  if (s.kind >= kX16Mx4) {  // [J][rows], its blocks along the rows
+    const int rc = check_shape(l, J, s.rows);
+    return rc != FBMM_OK ? rc : check_mx(name, static_cast<const unsigned char*>(s.ptr), s.stride, s.scales, s.scale_stride, l);
+  }
   if (s.ptr == nullptr) return fail(FBMM_ERR_INVALID, "%s is null", name);
   const int inner = s.kind == kX16K ? J : s.rows;
   if (s.ld < inner) return fail(FBMM_ERR_INVALID, "%s pitch %lld smaller than its row length %d", name, s.ld, inner);

@@ -251,7 +251,7 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           const int groups = (op.rows + 127) / 128;
           const bool exists = r0 < op.rows;
           mbar_arrive_expect_tx(&bars->raw[stage], bytes + (exists ? kMxGroupBytes : 0));
-          tma_load_3d(raw, map, &bars->raw[stage], r0 * S::kBits / 8, j0, mb, kL2EvictLast);
+          tma_load_3d(raw, map, &bars->raw[stage], r0 / (8 / S::kBits), j0, mb, kL2EvictLast);
           if (exists)
             mx_bulk_load(raw + bytes,
                          op.scales + b * op.scale_stride +
