@@ -13,6 +13,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from .bmm import BMMCUDA
@@ -361,12 +362,20 @@ def _mx4_product(A, B: MXTensor, out_dtype: torch.dtype) -> torch.Tensor:
     return C[0] if two_d else C
 
 
+def _refuse_tangents(*tensors) -> None:
+    """The differentiable products have reverse mode only; without this a tangent would be dropped."""
+    for t in tensors:
+        if unpack_dual(t).tangent is not None:
+            raise NotImplementedError("this product has no forward-mode derivative: its operands must not carry a tangent")
+
+
 def _once(backward):
     """A backward pass that can itself not be differentiated. The wrapper that says so to a graph
     of higher order (10 us a call) is only entered where such a graph is being made."""
     guarded = once_differentiable(backward)
 
     def run(ctx, dC):
+        _refuse_tangents(dC)
         return guarded(ctx, dC) if torch.is_grad_enabled() else backward(ctx, dC)
     return run
 
@@ -395,9 +404,9 @@ class MXBMMCUDA(CustomKernel):
     (``MXTensor``, blocks along k: ``dim=-1`` for A, ``dim=-2`` for B). A may be a fp32 / fp16 /
     bf16 tensor, which is quantised on the way; C then has its type unless `out_dtype` says
     otherwise, and is differentiable in A (the gradient passes straight through A's rounding:
-    dA = dC @ B^T with B's values, computed in A's type). With a microscaled A, C is fp32 unless
-    `out_dtype` says otherwise. Products and scales are exact, sums are kept in fp32, C is rounded
-    once."""
+    dA = dC @ B^T with B's values, computed in A's type; forward-mode tangents are refused). With a
+    microscaled A, C is fp32 unless `out_dtype` says otherwise. Products and scales are exact, sums
+    are kept in fp32, C is rounded once."""
 
     def __init__(self, out_dtype: torch.dtype | None = None):
         super().__init__()
@@ -416,6 +425,7 @@ class MXBMMCUDA(CustomKernel):
                 raise ValueError("A must hold 4-bit elements with their blocks along k (dim=-1)")
             return _mx4_product(A, B, self.out_dtype or torch.float32)
         _code(A.dtype)
+        _refuse_tangents(A)
         out_dtype = self.out_dtype or A.dtype
         if A.requires_grad and torch.is_grad_enabled():
             return _MX4Product.apply(A, B, out_dtype)
@@ -460,9 +470,11 @@ class CheckpointBMMCUDA(BMMCUDA):
     along k: 1.03 bytes per element) instead of their own type. C and dA = dC @ B^T are what the full
     A gives; dB = A8^T @ dC uses the kept values, each within 2^-4 of its own size or, where it is
     far below its block's largest, within half of the block's finest step. A itself is not
-    kept; B is. Differentiable once. Without a gradient to compute it is ``BMMCUDA``."""
+    kept; B is. Differentiable once, in reverse mode (forward-mode tangents are refused). Without a
+    gradient to compute it is ``BMMCUDA``."""
 
     def __call__(self, A: torch.Tensor, B: torch.Tensor) -> torch.Tensor:
+        _refuse_tangents(A, B)
         if not (torch.is_grad_enabled() and (A.requires_grad or B.requires_grad)):
             return super().__call__(A, B)
         A3, B3, two_d = self.check_inputs(A, B, (torch.float32,) + _X16)
