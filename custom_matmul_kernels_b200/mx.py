@@ -335,9 +335,11 @@ class MXDenseBMMCUDA(CustomKernel):
 
 
 @functools.lru_cache(maxsize=4096)
-def _product_workspace(l: int, m: int, n: int, k: int, layout: int) -> int:
-    """Scratch bytes of a product with a tensor; it depends on nothing but these."""
-    return load_library().fbmm_mx4_bmm_tensor_workspace_bytes(l, m, n, k, layout)
+def _product_workspace(index: int, l: int, m: int, n: int, k: int, layout: int) -> int:
+    """Scratch bytes of a product with a tensor on device `index`, by whose SM count the library decides whether the
+    rows are quantised inside the product."""
+    with torch.cuda.device(index):
+        return load_library().fbmm_mx4_bmm_tensor_workspace_bytes(l, m, n, k, layout)
 
 
 def _mx4_product(A, B: MXTensor, out_dtype: torch.dtype) -> torch.Tensor:
@@ -355,7 +357,7 @@ def _mx4_product(A, B: MXTensor, out_dtype: torch.dtype) -> torch.Tensor:
             _call("fbmm_mx4_bmm", t.get_device(), *A._arguments(), *B._arguments(), *result)
         else:
             t, layout, ld, step = _dense_layout(t)
-            need = _product_workspace(l, m, n, k, layout)
+            need = _product_workspace(t.get_device(), l, m, n, k, layout)
             ws = t.new_empty(need, dtype=torch.uint8) if need else None
             _call("fbmm_mx4_bmm_tensor", t.get_device(), t.data_ptr(), _DTYPES[t.dtype], layout, ld, step, *B._arguments(),
                   *result, ws.data_ptr() if need else None, need)
