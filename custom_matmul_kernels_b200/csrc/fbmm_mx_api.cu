@@ -249,9 +249,11 @@ constexpr int kMxFewRows = 64;  // rows of A up to which the weights take the 12
 
 // How many CTAs share the k of a tile in the few-row kernel. A CTA takes about 0.25 us per 256 k (one
 // stage's latency over the depth of the ring; 0.35 us with 128 rows), joining the sums 0.7 us (4), and a second CTA
-// on an SM starts 0.7 us late; two fit an SM (one with 128 rows). The least sum of these decides (measured: n = 16384,
-// k = 8192 11.0 us on 256 CTAs against 12.4 on 128; n = 1024, k = 8192 4.9 us on 64 against 11.2 on 8;
-// 128 rows at 4096 x 4096 8.1 us on 128 against 9.0 on 32, 256 rows 10.8 on 128 against 9.3 on 64).
+// on an SM starts 0.7 us late; two fit an SM. The least sum of these decides (measured: n = 16384,
+// k = 8192 11.0 us on 256 CTAs against 12.4 on 128; n = 1024, k = 8192 4.9 us on 64 against 11.2 on 8).
+// Tiles of 128 rows share k only while all their CTAs run at once, one to an SM: beyond, whole tiles or pairs of them
+// reuse more of what they copy (512 rows, n = 5120, k = 8192: 15.3 us on 40 pairs, 30.0 us on 640 CTAs; 128 rows at
+// 4096 x 4096 8.1 us on 128 against 9.0 on 32, 256 rows 10.8 on 128 against 9.3 on 64).
 void rows_splits(int sms, int l, int m, int n, int k, int* splits, int* blocks) {
   const int kblocks = (k + kMxStageK - 1) / kMxStageK;
   const bool tall = m > kMxFewRows;
@@ -262,6 +264,7 @@ void rows_splits(int sms, int l, int m, int n, int k, int* splits, int* blocks) 
     // CTAs to an SM 71 and 33 (128 rows, n = 2048, k = 8192: 9.3 us in fours against 14.8 in eights, two waves)
     const int permille = s <= 2 ? 1000 : tall ? (s == 4 ? 900 : 813) : (s == 4 ? 960 : 900);
     const long long ctas = base * s, per = (kblocks + s - 1) / s, slots = (tall ? 1ll : 2ll) * sms * permille / 1000;
+    if (tall && s > 1 && ctas > slots) break;
     const long long cost = (s > 1 ? (tall ? 4000 : 700) : 0) + (tall ? 350 : 250) * per * ((ctas + slots - 1) / slots) +
                            700 * ((ctas - 1) / sms);
     if (s == 1 || cost < best) {
