@@ -93,7 +93,9 @@ class MXTensor:
     of the axis the blocks run along, ``dim``: -1 (the matrix is [l, rows, k]) or -2 (it is
     [l, k, rows], held k-contiguous all the same). A batch stride of 0 (an expanded tensor)
     serves every batch with one matrix. 2-D codes with 3-D scales make a 2-D matrix. The codes
-    behind k must be zero, as ``MXQuantizeCUDA`` leaves them. A scale byte of 255 makes its block NaN; an
+    behind k must be zero, and so must the scale bytes of rows and blocks that do not exist, as
+    ``MXQuantizeCUDA`` leaves them: the 4-bit products multiply the padding behind k too, where a scale
+    byte of 255 would make a whole row of the result NaN. A scale byte of 255 makes its block NaN; an
     8-bit code of 0x7f or 0xff is NaN by itself."""
 
     # Storage is either the caller's two tensors or one buffer (codes, then scales), of which `codes`
