@@ -456,7 +456,7 @@ int launch_x16_any(cudaStream_t stream, int sms, const CUtensorMap& mx, const CU
   if (5 * waves(256, sms / 2) <= 4 * waves(128, sms)) return launch_x16<XK, YK, true>(stream, sms, mx, my, a);
   // Fewer tiles than SMs: j over a cluster of up to eight CTAs per tile, while all clusters run at once, where it pays.
   // In ns: a stage takes about 250, an expanded one 340; joining the sums 4500 (8-bit dB of 4096 x 64 over 8192:
-  // 46.1 us whole, 17.5 in fours; 512 x 512 over 4096: 25.6 and 11.2; dense 4096 x 64 over 4096: 19.2 and 11.1).
+  // 46.1 us whole, 18.0 in fours; 512 x 512 over 4096: 25.6 and 11.5; dense 4096 x 64 over 4096: 19.2 and 11.1).
   using S = X16Shape<XK, YK>;
   constexpr long long kStageNs = XK >= kX16Mx4 || YK >= kX16Mx4 ? 340 : 250, kJoinNs = 4500;
   const int blocks = (a.J + kX16J - 1) / kX16J;

@@ -89,10 +89,9 @@ __device__ __forceinline__ void mx_umma(uint32_t d_tmem, uint64_t a_desc, uint64
 __device__ __forceinline__ void mx_copy_scales(uint32_t tmem, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
-// One lane of the (converged) warp, always the same one. The loops that issue copies and MMAs run on the whole
-// warp, so that descriptors and addresses stay in uniform registers, and only the issuing instructions are
-// under this predicate: with the loop itself on one lane every tcgen05 instruction took about 100
-// cycles to issue (its operands moved to uniform registers one by one), which bound all three kernels.
+// One lane of the (converged) warp, always the same one. The loops that issue copies and MMAs run on the whole warp
+// and only the issuing instructions are under this predicate: with the loop itself on one lane every tcgen05
+// instruction took about 100 cycles to issue, which bound all three kernels (4-bit 8192^3 236 us, on the whole warp 183 us).
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile(
@@ -131,7 +130,8 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
 // warp's staging area (piece index xor row, free of bank conflicts) so that every store instruction covers
 // four whole 128-byte lines (16-bit results of 8192 x 8192 with k = 256: 68 us with 64-byte pieces of rows, 44 us
 // with lines; a plain fill writes 3.9 TB/s). The staging area is read ahead of the stores, which the compiler must take
-// for writes to it and would wait on (the same 41 us; 4-bit operands 45 -> 35 us, fp32 results 73 -> 47).
+// for writes to it and would wait on (4-bit operands of that size: bf16 results 45 -> 35 us, fp32 results 73 -> 47 us;
+// 16-bit operands 44 -> 41 us).
 // Rows on 8-byte boundaries leave in pieces of that size (bf16 8192 x 4092, k = 1024: 62 -> 49 us), others by element (8192 x 4091: 54 us).
 // `c0`: element (row 0, column 0) of the block.
 template <typename Word>

@@ -8,9 +8,10 @@
 //
 // Few tiles of n leave SMs idle, so k is split over a cluster of S CTAs; the partial sums meet in
 // shared memory and every CTA of the cluster adds up its share of the rows over the cluster in rank
-// order: the result does not depend on timing. One token at 4096 x 4096: 5.4 us (9.2 us as a quantising pass and
-// an unsplit product); 16 rows at n = 16384, k = 8192: 10.9 us with weights partly in L2, 16.5 us from memory,
-// where longer weights stream at 6.5 TB/s behind 5 us of launch, set-up, first bytes and joining.
+// order: the result does not depend on timing. One token at 4096 x 4096: 5.8 us over three weights in
+// turn, 6.1 us over thirty (9.2 us as a quantising pass and an unsplit product); 16 rows of codes at n = 16384, k = 8192:
+// 11.0 us with weights partly in L2, 15.7 us from memory (17.6 us with the quantiser ahead of it), where
+// longer weights stream at 6.5 TB/s behind 5 us of launch, set-up, first bytes and joining.
 //
 // Roles: warp 0 copies, warp 1 issues MMAs, the others quantise, then warps 2-5 read the sums.
 #pragma once

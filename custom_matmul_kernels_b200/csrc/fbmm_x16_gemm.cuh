@@ -19,7 +19,7 @@
 //
 // SPLIT (single CTAs): few tiles and a long j, as where one side of a weight is narrow. A cluster of CTAs shares a
 // tile's j; the partial sums meet in shared memory and every CTA adds up and stores its share of the rows, in
-// rank order. 8-bit dB of 4096 x 64 over 8192: 17.5 us on 128 CTAs against 46.1 on 32.
+// rank order. 8-bit dB of 4096 x 64 over 8192: 18 us on 128 CTAs against 46 on 32.
 //
 // Roles of a CTA: warp 0 copies, warp 1 (the even CTA's) MMAs, four warps for codes where an operand
 // is microscaled, four warps for the epilogue. Two accumulator stages, persistent.
@@ -106,7 +106,7 @@ __device__ __forceinline__ uint64_t x16_desc(uint32_t smem_addr, bool mn_major) 
 // memory (behind their proxy fence), or that the warp has read its accumulators. A release at cluster scope, as two CTAs
 // are ordered by nothing less, but of shared memory only: one that covers global memory too took each warp about
 // 1400 cycles beside 16 writing warps, twice the expansion (8-bit gradient of weights at 4096^3: 145 us against
-// 119 us). Passing the reports on through one warp of the CTA measured the same as this.
+// 110 us). Passing the reports on through one warp of the CTA measured the same as this.
 __device__ __forceinline__ void mbar_arrive_values(uint32_t cluster_addr) {
   asm volatile(
       "fence.release.sync_restrict::shared::cta.cluster;\n"
