@@ -125,6 +125,15 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
+// The last barrier of a cluster whose CTAs have read one another's shared memory: none goes while it is being read. Its
+// release is one of shared memory only, since one that covers the results just stored would wait for them to land
+// (about a microsecond).
+__device__ __forceinline__ void cluster_leave() {
+  asm volatile(
+      "fence.release.sync_restrict::shared::cta.cluster;\n"
+      "barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // 32 rows of a warp's accumulators (lane = row) -> row-major C, 128 bytes of every row at a time: 64 columns
 // (v0, v1) of a 16-bit type, or 32 columns of fp32 in two calls. The lanes' 16-byte pieces cross the
 // warp's staging area (piece index xor row, free of bank conflicts) so that every store instruction covers

@@ -277,10 +277,7 @@ mx_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant_
       }
     }
   }
-  // Nobody leaves while its sums are being read. The values read are in the results stored above, so the
-  // arrival needs no release, which would wait for those stores to land (about a microsecond).
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_leave();
   if (threadIdx.x == 0 && failed) atomicOr(&g_mx_status[0], 1u);
 }
 

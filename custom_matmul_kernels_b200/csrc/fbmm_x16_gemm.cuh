@@ -445,9 +445,7 @@ x16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
       }
     }
-    // nobody leaves while its sums are being read; what was read is in the stores above
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_leave();
   }
 }
 
